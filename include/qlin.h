@@ -42,6 +42,7 @@ typedef enum {
     QLIN_DT_U8 = 4,
     QLIN_DT_I32 = 5,
     QLIN_DT_E4M3 = 6,
+    QLIN_DT_I64 = 7,   /* positions and cache slots */
 } qlin_dtype;
 
 /* Strided tensor view.  shape/stride are in elements; unused dims are ignored. */
@@ -67,6 +68,8 @@ typedef enum {
     QLIN_OP_W4A8_LINEAR_RESIDUAL = 9,  /* qlin_w4a8_linear_residual: param as QLIN_OP_W4A8_LINEAR */
     QLIN_OP_GGUF_LINEAR_RESIDUAL = 10, /* qlin_gguf_linear_residual: param = the ggml type */
     QLIN_OP_GGUF_LINEAR_LORA = 11,     /* qlin_gguf_linear_lora: param = the ggml type | R << 8 */
+    QLIN_OP_QK_NORM_ROPE_GRAD = 12,    /* qlin_qk_norm_rope_grad: M tokens, N heads of q and k together, K the head size */
+    QLIN_OP_PAGED_ATTENTION = 13,      /* qlin_paged_attention: M rows, N query heads, K the head size, param = kv heads */
 } qlin_op;
 
 /* ggml type ids accepted by the GGUF entry points (enum ggml_type). */
@@ -297,6 +300,87 @@ qlin_status qlin_dequantize_w4a8(const qlin_tensor* qdata, const qlin_tensor* s_
  * xrot (optional, may be NULL): receives the rotated activation in x's dtype. */
 qlin_status qlin_quantize_act_int8(const qlin_tensor* x, qlin_tensor* q, qlin_tensor* scale,
                                    int convrot_groupsize, qlin_tensor* xrot, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * The attention side of a block, between its packed QKV projection and its output projection.
+ *
+ * Head tensors are [tokens, heads, D], f32/f16/bf16, any strides with unit stride along D (the slices
+ * of a fused projection's output go in as they are), D <= 512.  16-byte aligned rows whose D and rotated size
+ * are multiples of 16 move in 16-byte pieces, of 8 in 8-byte ones; any other size is taken too, value
+ * by value.
+ *
+ * Rotation: inv_freq f32 [P] gives the frequency of each of P pairs (2P <= D; the values from 2P on pass
+ * through unrotated; P = 0 rotates nothing), axis i32 [P] the row of `positions` that turns it (NULL: row
+ * 0; an entry outside the rows counts as the nearest row), positions i32/i64/f32 [axes, tokens] (or
+ * [tokens]).  Pair i is (i, i + P), or (2i, 2i + 1) with QLIN_ROPE_INTERLEAVED; it turns by the angle
+ * positions[axis[i], t] * inv_freq[i], formed in 64 bits, by its negative with QLIN_ROPE_INVERSE.
+ * ---------------------------------------------------------------------------------------------- */
+enum { QLIN_ROPE_INTERLEAVED = 1, QLIN_ROPE_INVERSE = 2 };
+
+/* q_out = rotate(q), k_out = rotate(k), in fp32 with one rounding.  k and k_out may both be NULL.  The
+ * gradient of a rotation is the rotation by the negative angles (QLIN_ROPE_INVERSE).  An output may be its own input
+ * (the same memory and strides); it may not overlap it otherwise. */
+qlin_status qlin_axis_rope(const qlin_tensor* q, const qlin_tensor* k, const qlin_tensor* positions,
+                           const qlin_tensor* inv_freq, const qlin_tensor* axis, int flags, qlin_tensor* q_out,
+                           qlin_tensor* k_out, void* stream);
+
+/* q_out = rotate(q_weight * q / rms(q)) per head, k alike: rms(x) = sqrt(mean(x^2) + eps) over D, in fp32 with one
+ * rounding.  q_weight, k_weight: optional (NULL = 1) f32/f16/bf16 [D].  k, k_weight and k_out may be NULL.
+ * Outputs as for qlin_axis_rope. */
+qlin_status qlin_qk_norm_rope(const qlin_tensor* q, const qlin_tensor* k, const qlin_tensor* q_weight,
+                              const qlin_tensor* k_weight, float eps, const qlin_tensor* positions,
+                              const qlin_tensor* inv_freq, const qlin_tensor* axis, int flags, qlin_tensor* q_out,
+                              qlin_tensor* k_out, void* stream);
+
+/* The same with k and v [tokens, kv heads, D] written into a paged cache instead: k_cache, v_cache
+ * [blocks, page, kv heads, D] in k's dtype, any strides with unit stride along D; token t goes to place
+ * slots[t] % page of block slots[t] / page (slots i32/i64 [tokens]).  A slot below 0 or past the cache
+ * stores nothing; two tokens with one slot leave either's values.  eps < 0: no norms (the weights must be NULL). */
+qlin_status qlin_qk_norm_rope_store(const qlin_tensor* q, const qlin_tensor* k, const qlin_tensor* v,
+                                    const qlin_tensor* q_weight, const qlin_tensor* k_weight, float eps,
+                                    const qlin_tensor* positions, const qlin_tensor* inv_freq, const qlin_tensor* axis,
+                                    int flags, const qlin_tensor* slots, qlin_tensor* q_out, qlin_tensor* k_cache,
+                                    qlin_tensor* v_cache, void* stream);
+
+/* Gradients of qlin_qk_norm_rope from those of its outputs: with g = rotate^-1(dq_out), x^ = q / rms(q) and w the
+ * weight, dq = (w g - x^ mean(w g x^)) / rms(q) and dq_weight = sum over tokens and heads of g x^ (NULL: not
+ * formed; f32/f16/bf16 [D], summed in fp32 in a fixed order); k alike (all of k's NULL: none).  dq in dq_out's
+ * dtype, which is q's.  flags as in the forward call.
+ * Workspace: qlin_workspace_size(QLIN_OP_QK_NORM_ROPE_GRAD, tokens, q heads + k heads, D, 0, q's dtype). */
+qlin_status qlin_qk_norm_rope_grad(const qlin_tensor* dq_out, const qlin_tensor* dk_out, const qlin_tensor* q,
+                                   const qlin_tensor* k, const qlin_tensor* q_weight, const qlin_tensor* k_weight, float eps,
+                                   const qlin_tensor* positions, const qlin_tensor* inv_freq, const qlin_tensor* axis,
+                                   int flags, qlin_tensor* dq, qlin_tensor* dk, qlin_tensor* dq_weight,
+                                   qlin_tensor* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Largest number of requests of one qlin_paged_plan call. */
+#define QLIN_PLAN_MAX_REQUESTS 4096
+
+/* The tables of one step over a paged cache, from lengths on the GPU.  Request b has context[b] tokens in
+ * the cache and gets added[b] new ones (i32 [B], negative counts as 0).  Requests take the pages that they lack from
+ * free_blocks (i32 [F]) in order, entries are appended to its row of block_table (i32 [B, W], unit column stride,
+ * updated in place; distinct rows).  Token j of request b, at place starts[b] + j of the step, gets
+ *   positions = context[b] + j,  rows = b,  slots = block_table[b, position / page] * page + position % page
+ * (i32, i32, i64 [N], N >= the new tokens; the places behind the last token get -1 in all three, new
+ * tokens behind N get no place).  starts i32 [B + 1]: the running sum of added; lengths i32 [B]: context + added; used
+ * i32 [1]: the pages that the step needs.  When used > F the free list was too short: pages past it are
+ * -1 in the table and so are their tokens' slots; the same for pages past W, which have no entry. */
+qlin_status qlin_paged_plan(const qlin_tensor* context, const qlin_tensor* added, const qlin_tensor* free_blocks,
+                            int64_t page, qlin_tensor* block_table, qlin_tensor* slots, qlin_tensor* positions,
+                            qlin_tensor* rows, qlin_tensor* starts, qlin_tensor* lengths, qlin_tensor* used, void* stream);
+
+/* Attention of one new token a row over a paged cache: out[b, h] = sum_s softmax_s(scale * q[b, h] . k[s, g]) v[s, g]
+ * over the tokens s < lengths[b] (the last `window` of them when window > 0), g = h / (heads / kv heads).
+ * q, out [rows, heads, D] f16/bf16, any strides with unit stride along D; k_cache, v_cache [blocks, page, kv heads, D] in q's
+ * dtype, any strides with unit stride along D; block_table i32 [rows, W], unit column stride, any row stride (0
+ * shares one row: the tokens of one prompt are rows with lengths 1, 2, ...); lengths i32 [rows], at most W * page
+ * counts.  D a multiple of 8 up to 256, 16-byte aligned rows (QLIN_EUNSUPPORTED otherwise).  A row with no token gives
+ * zeros; a token whose table entry is outside the cache counts as absent.  What the cache holds behind a row's last
+ * token is never used, whatever it is.  Scores, their running maximum and sum and the output are fp32.
+ * Workspace: qlin_workspace_size(QLIN_OP_PAGED_ATTENTION, rows, heads, D, kv heads, q's dtype). */
+qlin_status qlin_paged_attention(const qlin_tensor* q, const qlin_tensor* k_cache, const qlin_tensor* v_cache,
+                                 const qlin_tensor* block_table, const qlin_tensor* lengths, float scale, int64_t window,
+                                 qlin_tensor* out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

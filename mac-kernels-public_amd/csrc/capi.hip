@@ -11,6 +11,7 @@
 #include "hadamard.h"
 #include "gguf_exact.h"
 #include "qlin_internal.h"
+#include "attention.h"
 
 using namespace qlin;
 
@@ -41,6 +42,15 @@ qlin_status fail(qlin_status s, const char* fmt, ...) {
     g_err = buf;
     return s;
 }
+
+}  // namespace
+
+qlin_status qlin::report(qlin_status s, const char* message) {
+    g_err = message;
+    return s;
+}
+
+namespace {
 
 qlin_status hip_status(hipError_t e, const char* what) {
     if (e == hipSuccess) return QLIN_OK;
@@ -375,6 +385,8 @@ size_t qlin_workspace_size(int op, int64_t M, int64_t N, int64_t K, int param, i
             return ws_w4a8(M, N, K, param >> 8) + align_up((size_t)(M * N * 4)) + 256;
         case QLIN_OP_GGUF_LINEAR_RESIDUAL:
             return ws_gguf(M, N, K, param) + ws_gguf_decoded(M, N, K, param) + align_up((size_t)(M * N * 4)) + 256;
+        case QLIN_OP_QK_NORM_ROPE_GRAD: return ws_head_grad(M, N, K);
+        case QLIN_OP_PAGED_ATTENTION: return ws_paged_attention(M, N, param, K);
         case QLIN_OP_LORA: {  // the split partials, then their sum
             const int S = lora_splits(M, K, param);
             return align_up((size_t)(S > 1 ? S + 1 : 1) * M * (size_t)(param > 0 ? param : 0) * 4);

@@ -8,7 +8,7 @@
 
 namespace qlin {
 
-enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2, DT_I8 = 3, DT_U8 = 4, DT_I32 = 5, DT_E4M3 = 6, DT_NONE = -1 };
+enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2, DT_I8 = 3, DT_U8 = 4, DT_I32 = 5, DT_E4M3 = 6, DT_I64 = 7, DT_NONE = -1 };
 enum { PROLOGUE_WO = 0, PROLOGUE_A8 = 1, PROLOGUE_ROT_F32 = 2 };
 
 // ---- activation prologue (prologue.hip) ----

@@ -1,9 +1,9 @@
-// Eager entry points for PyTorch: the plain linears (no LoRA, no residual) called straight from
-// Python with torch tensors.  Each builds the qlin_tensor descriptors, takes the output and the
+// Eager entry points for PyTorch: the plain linears (no LoRA, no residual) and the attention side
+// called straight from Python with torch tensors.  Each builds the qlin_tensor descriptors, takes the output and the
 // workspace from torch's allocator and calls the C ABI (include/qlin.h) on the current stream,
 // so an eager call costs one Python -> C++ crossing instead of the descriptor packing and ctypes
-// marshalling of qlin/_lib.py.  The argument rules and declines are those of qlin/ops.py, which
-// runs every other call (LoRA, residual) through ctypes.
+// marshalling of qlin/_lib.py.  The argument rules and declines are those of qlin/ops.py and
+// qlin/attention.py, which run every other call (LoRA, residual) through ctypes.
 //
 // Errors leave as QlinStatusError("<status>:<message>"); qlin/ops.py turns a status into
 // NoCapableBackendError (QLIN_EUNSUPPORTED), ValueError (QLIN_EINVAL, QLIN_EWORKSPACE) or
@@ -40,6 +40,7 @@ int dtype_of(at::ScalarType t) {
         case at::kByte: return QLIN_DT_U8;
         case at::kInt: return QLIN_DT_I32;
         case at::kFloat8_e4m3fn: return QLIN_DT_E4M3;
+        case at::kLong: return QLIN_DT_I64;
         default: return -1;
     }
 }
@@ -261,6 +262,162 @@ at::Tensor w4a8_int8_linear(const at::Tensor& x, const at::Tensor& qdata, const 
     return shaped(y, lead, n);
 }
 
+// ---- the attention side (qlin/attention.py) ----
+using OptTensor = c10::optional<at::Tensor>;
+
+// t with unit stride along its last dimension (a copy if need be).
+at::Tensor dense(const at::Tensor& t) {
+    return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+// [.., heads, D] as [tokens, heads, D].
+at::Tensor heads_of(const char* op, const at::Tensor& t, const char* name) {
+    if (t.dim() < 3)
+        fail(QLIN_EINVAL, std::string(op) + ": " + name + " must be [.., heads, D], it has " + std::to_string(t.dim()) +
+                              " dimensions");
+    return dense(t.dim() == 3 ? t : t.reshape({-1, t.size(-2), t.size(-1)}));
+}
+
+at::Tensor packed(const at::Tensor& t, c10::optional<at::ScalarType> dt = c10::nullopt) {
+    const at::Tensor u = !dt || t.scalar_type() == *dt ? t : t.to(*dt);
+    return u.is_contiguous() ? u : u.contiguous();
+}
+
+// An optional tensor's descriptor, with the tensor kept alive until the call has been made.
+struct Opt {
+    at::Tensor t;
+    qlin_tensor d{};
+    bool there = false;
+    Opt() = default;
+    explicit Opt(const at::Tensor& x) : t(x), d(desc(x)), there(true) {}
+    qlin_tensor* p() { return there ? &d : nullptr; }
+};
+
+Opt vec(const OptTensor& t, c10::optional<at::ScalarType> dt = c10::nullopt) { return t ? Opt(packed(*t, dt)) : Opt(); }
+
+void all_on_device(const char* op, std::initializer_list<const OptTensor*> ts) {
+    int dev = -1;
+    for (const OptTensor* t : ts)
+        if (t->has_value()) on_device(op, **t, dev);
+}
+
+// An output like x [tokens, heads, D], contiguous.
+at::Tensor like(const at::Tensor& x) { return at::empty(x.sizes(), x.options()); }
+
+pybind11::object as(const Opt& o, const OptTensor& shape) {
+    if (!o.there) return pybind11::none();
+    return pybind11::cast(shape->dim() == 3 ? o.t : o.t.view(shape->sizes()));
+}
+
+// The forward call with or without the norms (eps < 0: without).
+pybind11::tuple rope_forward(const char* op, const at::Tensor& q, const OptTensor& k, const OptTensor& wq, const OptTensor& wk,
+                             bool norm, double eps, const at::Tensor& positions, const at::Tensor& inv_freq,
+                             const OptTensor& axis, int64_t flags) {
+    const OptTensor qt = q, pt = positions, ft = inv_freq;
+    all_on_device(op, {&qt, &k, &wq, &wk, &pt, &ft, &axis});
+    Opt q3(heads_of(op, q, "q")), k3, qo(like(q3.t)), ko, pos(positions), freq = vec(ft, at::kFloat), ax = vec(axis, at::kInt);
+    if (k) {
+        k3 = Opt(heads_of(op, *k, "k"));
+        ko = Opt(like(k3.t));
+    }
+    const hipStream_t st = current_stream(q);
+    if (norm) {
+        Opt a = vec(wq), b = vec(wk);
+        check(qlin_qk_norm_rope(q3.p(), k3.p(), a.p(), b.p(), (float)eps, pos.p(), freq.p(), ax.p(), (int)flags, qo.p(), ko.p(), st));
+    } else {
+        check(qlin_axis_rope(q3.p(), k3.p(), pos.p(), freq.p(), ax.p(), (int)flags, qo.p(), ko.p(), st));
+    }
+    return pybind11::make_tuple(as(qo, qt), as(ko, k));
+}
+
+pybind11::tuple axis_rope(const at::Tensor& q, const OptTensor& k, const at::Tensor& positions, const at::Tensor& inv_freq,
+                          const OptTensor& axis, int64_t flags) {
+    return rope_forward("axis_rope", q, k, c10::nullopt, c10::nullopt, false, 0.0, positions, inv_freq, axis, flags);
+}
+
+pybind11::tuple qk_norm_rope(const at::Tensor& q, const OptTensor& k, const OptTensor& wq, const OptTensor& wk, double eps,
+                             const at::Tensor& positions, const at::Tensor& inv_freq, const OptTensor& axis, int64_t flags) {
+    return rope_forward("qk_norm_rope", q, k, wq, wk, true, eps, positions, inv_freq, axis, flags);
+}
+
+at::Tensor qk_norm_rope_store(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& wq,
+                              const OptTensor& wk, double eps, const at::Tensor& positions, const at::Tensor& inv_freq,
+                              const OptTensor& axis, int64_t flags, const at::Tensor& slots, const at::Tensor& k_cache,
+                              const at::Tensor& v_cache) {
+    const char* op = "qk_norm_rope_store";
+    const OptTensor qt = q, kt = k, vt = v, pt = positions, ft = inv_freq, st_ = slots, kc = k_cache, vc = v_cache;
+    all_on_device(op, {&qt, &kt, &vt, &wq, &wk, &pt, &ft, &axis, &st_, &kc, &vc});
+    Opt q3(heads_of(op, q, "q")), k3(heads_of(op, k, "k")), v3(heads_of(op, v, "v")), qo(like(q3.t)), pos(positions);
+    Opt freq = vec(ft, at::kFloat), ax = vec(axis, at::kInt), a = vec(wq), b = vec(wk), s(slots), dk(k_cache), dv(v_cache);
+    check(qlin_qk_norm_rope_store(q3.p(), k3.p(), v3.p(), a.p(), b.p(), (float)eps, pos.p(), freq.p(), ax.p(), (int)flags, s.p(),
+                                  qo.p(), dk.p(), dv.p(), current_stream(q)));
+    return q.dim() == 3 ? qo.t : qo.t.view(q.sizes());
+}
+
+pybind11::tuple qk_norm_rope_grad(const at::Tensor& gq, const OptTensor& gk, const at::Tensor& q, const OptTensor& k,
+                                  const OptTensor& wq, const OptTensor& wk, double eps, const at::Tensor& positions,
+                                  const at::Tensor& inv_freq, const OptTensor& axis, int64_t flags, bool weight_grads) {
+    const char* op = "qk_norm_rope_grad";
+    const OptTensor gt = gq, qt = q, pt = positions, ft = inv_freq;
+    all_on_device(op, {&gt, &gk, &qt, &k, &wq, &wk, &pt, &ft, &axis});
+    Opt q3(heads_of(op, q, "q")), k3, dq(like(q3.t)), dk, g3(heads_of(op, gq, "dq_out")), h3, pos(positions);
+    Opt freq = vec(ft, at::kFloat), ax = vec(axis, at::kInt), a = vec(wq), b = vec(wk), da, db;
+    if (k) {
+        k3 = Opt(heads_of(op, *k, "k"));
+        dk = Opt(like(k3.t));
+    }
+    if (gk) h3 = Opt(heads_of(op, *gk, "dk_out"));
+    if (weight_grads && wq) da = Opt(at::empty_like(a.t));
+    if (weight_grads && wk) db = Opt(at::empty_like(b.t));
+    const hipStream_t st = current_stream(q);
+    at::Tensor ws;
+    if (da.there || db.there)
+        ws = workspace_for(qlin_workspace_size(QLIN_OP_QK_NORM_ROPE_GRAD, q3.t.size(0), q3.t.size(1) + (k ? k3.t.size(1) : 0),
+                                               q3.t.size(2), 0, q3.d.dtype),
+                           q, st);
+    check(qlin_qk_norm_rope_grad(g3.p(), h3.p(), q3.p(), k3.p(), a.p(), b.p(), (float)eps, pos.p(), freq.p(), ax.p(), (int)flags,
+                                 dq.p(), dk.p(), da.p(), db.p(), ws.defined() ? ws.data_ptr() : nullptr,
+                                 ws.defined() ? (size_t)ws.numel() : 0, st));
+    const auto weight = [](const Opt& o) { return o.there ? pybind11::cast(o.t) : pybind11::object(pybind11::none()); };
+    return pybind11::make_tuple(as(dq, qt), as(dk, k), weight(da), weight(db));
+}
+
+pybind11::tuple paged_plan(const at::Tensor& context, const at::Tensor& added, const at::Tensor& table,
+                           const at::Tensor& free_blocks, int64_t page, int64_t tokens) {
+    const char* op = "paged_plan";
+    const OptTensor ct = context, at_ = added, tt = table, ft = free_blocks;
+    all_on_device(op, {&ct, &at_, &tt, &ft});
+    if (tokens < 0) fail(QLIN_EINVAL, std::string(op) + ": tokens must not be negative");
+    const int64_t B = context.dim() == 1 ? context.size(0) : 0;
+    const auto i32 = context.options().dtype(at::kInt);
+    // the int32 results share one allocation
+    const at::Tensor all = at::empty({2 * tokens + 2 * B + 2}, i32), slots = at::empty({tokens}, i32.dtype(at::kLong));
+    const at::Tensor positions = all.narrow(0, 0, tokens), rows = all.narrow(0, tokens, tokens),
+                     starts = all.narrow(0, 2 * tokens, B + 1), lengths = all.narrow(0, 2 * tokens + B + 1, B),
+                     used = all.narrow(0, 2 * tokens + 2 * B + 1, 1);
+    qlin_tensor dc = desc(context), da = desc(added), df = desc(free_blocks), dt = desc(table), ds = desc(slots),
+                dp = desc(positions), dr = desc(rows), dst = desc(starts), dl = desc(lengths), du = desc(used);
+    check(qlin_paged_plan(&dc, &da, &df, page, &dt, &ds, &dp, &dr, &dst, &dl, &du, current_stream(context)));
+    return pybind11::make_tuple(slots, positions, rows, starts, lengths, used);
+}
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table,
+                           const at::Tensor& lengths, double scale, int64_t window, const OptTensor& out) {
+    const char* op = "paged_attention";
+    const OptTensor qt = q, kt = k_cache, vt = v_cache, tt = table, lt = lengths;
+    all_on_device(op, {&qt, &kt, &vt, &tt, &lt, &out});
+    if (q.dim() != 3 || k_cache.dim() != 4)
+        fail(QLIN_EINVAL, std::string(op) + ": q must be [rows, heads, D] and the caches [blocks, page, kv heads, D]");
+    const at::Tensor q3 = dense(q), o = out ? *out : like(q);
+    const hipStream_t st = current_stream(q);
+    const at::Tensor ws = workspace_for(qlin_workspace_size(QLIN_OP_PAGED_ATTENTION, q.size(0), q.size(1), q.size(2),
+                                                            (int)k_cache.size(2), dtype_of(q.scalar_type())),
+                                        q, st);
+    qlin_tensor dq = desc(q3), dk = desc(k_cache), dv = desc(v_cache), dt = desc(table), dl = desc(lengths), d_o = desc(o);
+    check(qlin_paged_attention(&dq, &dk, &dv, &dt, &dl, (float)scale, window, &d_o, ws.data_ptr(), (size_t)ws.numel(), st));
+    return o;
+}
+
 // The cached workspace for (device of `like`, current stream), at least nbytes (for the ctypes
 // calls of qlin/ops.py, so that both routes share one buffer per stream).
 at::Tensor workspace(int64_t nbytes, const at::Tensor& like) {
@@ -284,6 +441,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gguf_linear", &gguf_linear);
     m.def("int8_linear", &int8_linear);
     m.def("w4a8_int8_linear", &w4a8_int8_linear);
+    m.def("axis_rope", &axis_rope);
+    m.def("qk_norm_rope", &qk_norm_rope);
+    m.def("qk_norm_rope_store", &qk_norm_rope_store);
+    m.def("qk_norm_rope_grad", &qk_norm_rope_grad);
+    m.def("paged_plan", &paged_plan);
+    m.def("paged_attention", &paged_attention);
     m.def("workspace", &workspace);
     m.def("release_workspaces", &release_workspaces);
 }

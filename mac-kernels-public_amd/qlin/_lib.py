@@ -18,15 +18,17 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libqlin.so")
 
 QLIN_OK, QLIN_EUNSUPPORTED, QLIN_EINVAL, QLIN_EHIP, QLIN_EWORKSPACE = 0, 1, 2, 3, 4
-DT_F32, DT_F16, DT_BF16, DT_I8, DT_U8, DT_I32, DT_E4M3 = 0, 1, 2, 3, 4, 5, 6
+DT_F32, DT_F16, DT_BF16, DT_I8, DT_U8, DT_I32, DT_E4M3, DT_I64 = 0, 1, 2, 3, 4, 5, 6, 7
 OP_INT8_LINEAR, OP_W4A8_LINEAR, OP_GGUF_LINEAR, OP_LORA, OP_INT8_GRAD_INPUT, OP_W4A8_GRAD_INPUT = 0, 1, 2, 3, 4, 5
 OP_INT8_LINEAR_LORA, OP_W4A8_LINEAR_LORA = 6, 7
 OP_INT8_LINEAR_RESIDUAL, OP_W4A8_LINEAR_RESIDUAL, OP_GGUF_LINEAR_RESIDUAL = 8, 9, 10
 OP_GGUF_LINEAR_LORA = 11
+OP_QK_NORM_ROPE_GRAD, OP_PAGED_ATTENTION = 12, 13
+ROPE_INTERLEAVED, ROPE_INVERSE = 1, 2
 
 _TORCH_DT = {
     torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int8: DT_I8,
-    torch.uint8: DT_U8, torch.int32: DT_I32, torch.float8_e4m3fn: DT_E4M3,
+    torch.uint8: DT_U8, torch.int32: DT_I32, torch.float8_e4m3fn: DT_E4M3, torch.int64: DT_I64,
 }
 
 # Every symbol include/qlin.h declares.
@@ -38,6 +40,8 @@ EXPORTS = (
     "qlin_int8_linear_grad_input", "qlin_w4a8_linear_grad_input",
     "qlin_int8_linear_residual", "qlin_w4a8_linear_residual", "qlin_gguf_linear_residual",
     "qlin_gguf_linear_lora",
+    "qlin_axis_rope", "qlin_qk_norm_rope", "qlin_qk_norm_rope_store", "qlin_qk_norm_rope_grad", "qlin_paged_plan",
+    "qlin_paged_attention",
 )
 
 
@@ -90,6 +94,12 @@ def load():
         "qlin_residual_epilogue": (I, [T, T, T, T, P]),
         "qlin_int8_linear_grad_input": (I, [T, T, T, I, T, P, SZ, P]),
         "qlin_w4a8_linear_grad_input": (I, [T, T, T, T, T, T, I, I, I, P, SZ, P]),
+        "qlin_axis_rope": (I, [T, T, T, T, T, I, T, T, P]),
+        "qlin_qk_norm_rope": (I, [T, T, T, T, ctypes.c_float, T, T, T, I, T, T, P]),
+        "qlin_qk_norm_rope_store": (I, [T, T, T, T, T, ctypes.c_float, T, T, T, I, T, T, T, T, P]),
+        "qlin_qk_norm_rope_grad": (I, [T, T, T, T, T, T, ctypes.c_float, T, T, T, I, T, T, T, T, P, SZ, P]),
+        "qlin_paged_plan": (I, [T, T, T, I64, T, T, T, T, T, T, T, P]),
+        "qlin_paged_attention": (I, [T, T, T, T, T, ctypes.c_float, I64, T, P, SZ, P]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import os
 
-from . import ops
+from . import attention, ops
 from .exceptions import NoCapableBackendError
 
 # func name -> (callable, keyword arguments the backend accepts beyond the plain signature)
@@ -25,6 +25,12 @@ _HIP = {
     "dequantize_int8_convrot_weight": (ops.dequantize_int8_convrot_weight, set()),
     "dequantize_w4a8_int8_weight": (ops.dequantize_w4a8_int8_weight, set()),
     "quantize_int8_rowwise": (ops.quantize_int8_rowwise, set()),
+    "axis_rope": (attention.axis_rope, set()),
+    "qk_norm_rope": (attention.qk_norm_rope, set()),
+    "qk_norm_rope_store": (attention.qk_norm_rope_store, set()),
+    "qk_norm_rope_grad": (attention.qk_norm_rope_grad, set()),
+    "paged_plan": (attention.paged_plan, set()),
+    "paged_attention": (attention.paged_attention, set()),
 }
 _OPT_IN = {"lora_down", "lora_up", "lora_scale", "correction"}
 
