@@ -14,10 +14,11 @@
 // output would carry their rounding on top of its own.  Up to 8 heads the second part rides in the 8 columns that the
 // heads leave free; 9 to 16 heads take a second instruction.
 //
-// Work split: a row's tokens in units of 128 (4 waves x 32), joined in LDS; rows of more than `per` units are split
-// over workgroups that leave (O, m, l) in fp32 for a second kernel.  `per` follows on the GPU from all
-// rows' lengths, which the host does not know: about TARGET workgroups for the whole batch, so that one long
-// row among short ones is spread like the rest.  Every workgroup forms the same plan from the lengths.
+// Work split: a row's tokens count in units of 128 (4 waves x 32), all rows' units are laid end to end and every
+// workgroup takes an equal run of them, as many workgroups as the chip holds at once.  So one long row among short ones
+// is spread like the rest, and the host need not know the lengths: every workgroup forms the running sum from them.
+// A row that crosses from one workgroup's run into the next leaves its parts as (O, m, l) in fp32, and a second
+// kernel joins them.
 #include "attention.h"
 
 namespace qlin {
@@ -28,19 +29,27 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 256, WAVES = 4, TILE = 32, UNIT = WAVES * TILE;
 constexpr int MAX_ROWS = 1024;       // rows of one launch (their lengths are summed by every workgroup)
-constexpr int TARGET = 1024;         // workgroups that a batch is split into
+constexpr int CUS = 256;
+constexpr int MOST_GROUPS = 4 * CUS;  // of any head size: see held()
+
+// Workgroups of the kernel for this head size that the chip holds at once (registers: 4, 2 and 1 on a compute unit).
+int64_t held(int64_t D) { return CUS * (D <= 64 ? 4 : D <= 128 ? 2 : 1); }
 
 struct Launch {
     PagedAttentionArgs a;
     int ng;                 // head groups of a kv head
     int hpg;                // heads of a group (the last one may have fewer)
-    int per_group;          // chunks to aim for, for each head group
+    int shares;             // workgroups of a head group
     uint64_t page_magic;    // floor(2^64 / d) + 1 for d = page / 16 or page; 0 for d = 1
-    float* part_o;          // [chunk][kv head, group][head][D]
-    float* part_ml;         // [chunk][kv head, group][head][2]
-    int2* meta;             // [rows]: chunks, the first one's place
+    float* part_o;          // [share, first or last row][kv head, group][head][D]
+    float* part_ml;         // [share, first or last row][kv head, group][head][2]
+    int4* meta;             // [rows]: the first share, shares, whether the row is not the first of its first share
     bool join;
 };
+
+// What no kernel writes while this one runs is read through the scalar cache: its loads do not queue with
+// those of keys and values.
+typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
 
 template <int DT> struct Mma;
 template <> struct Mma<DT_F16> {
@@ -72,99 +81,85 @@ __device__ __forceinline__ uint32_t divided(uint32_t n, uint64_t magic) {
 }
 
 // The range of row b's tokens that count.
-__device__ __forceinline__ void range_of(const PagedAttentionArgs& a, int b, int& lo, int& hi) {
-    const int64_t n = min((int64_t)max(a.lengths[b], 0), a.W * a.page);
+__device__ __forceinline__ void range_of(const PagedAttentionArgs& a, int length, int& lo, int& hi) {
+    const int64_t n = min((int64_t)max(length, 0), a.W * a.page);
     hi = (int)n;
     lo = a.window && n > a.window ? (int)(n - a.window) : 0;
 }
-__device__ __forceinline__ int units_of(int lo, int hi) { return (hi - (lo & ~(TILE - 1)) + UNIT - 1) / UNIT; }
+// Units of a row; one, of no token, for an empty row.
+__device__ __forceinline__ int units_of(const PagedAttentionArgs& a, int length) {
+    int lo, hi;
+    range_of(a, length, lo, hi);
+    return max(1, (hi - (lo & ~(TILE - 1)) + UNIT - 1) / UNIT);
+}
 
-// What a workgroup computes: tokens [start, end) of row b, which counts [lo, hi).
-struct Item {
-    int b, chunk, chunks, place, lo, hi, start, end;
+// A workgroup's run of units, [unit, end) in the running sum; the row of its first one, which starts at `first`.
+struct Share {
+    int b, first, unit, end, per;
 };
 
-// The plan from all rows' lengths: `per` units a chunk, and the item of this number; false past the last.
-__device__ bool find_item(const Launch& p, int item, Item& it) {
-    __shared__ int64_t sum_units[WAVES];
-    __shared__ int sum_chunks[WAVES], sum_split[WAVES];
-    __shared__ int found[5];
+// Running sum over a wave, this lane's own value included.
+__device__ __forceinline__ int scan(int a, int lane) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int x = __shfl_up(a, m);
+        if (lane >= m) a += x;
+    }
+    return a;
+}
+
+__device__ __forceinline__ bool set_share(const Launch& p, int w, int total, Share& s) {
+    s.per = (total + p.shares - 1) / p.shares;
+    s.unit = w * s.per;
+    s.end = min(s.unit + s.per, total);
+    return s.unit < total;
+}
+
+// The share of this number; false past the last.  Up to 64 rows every wave forms the sums for itself, a row a lane,
+// without a barrier.
+__device__ __forceinline__ bool find_share_wave(const Launch& p, int w, Share& s) {
+    const int lane = threadIdx.x & 63;
+    const int units = lane < p.a.B ? units_of(p.a, p.a.lengths[lane]) : 0;
+    const int sum = scan(units, lane);
+    if (!set_share(p, w, __builtin_amdgcn_readlane(sum, 63), s)) return false;
+    const uint64_t here = __ballot(s.unit < sum && s.unit >= sum - units);
+    s.b = __ffsll((unsigned long long)here) - 1;
+    s.first = __builtin_amdgcn_readlane(sum, s.b) - __builtin_amdgcn_readlane(units, s.b);
+    return true;
+}
+
+// The same for up to MAX_ROWS rows, over the workgroup.
+__device__ bool find_share(const Launch& p, int w, Share& s) {
+    __shared__ int sums[WAVES], found[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int rows = (int)p.a.B, each = (rows + THREADS - 1) / THREADS;
-    int units[MAX_ROWS / THREADS];
-    int64_t mine = 0;
+    int units[MAX_ROWS / THREADS], mine = 0;
 #pragma unroll
     for (int i = 0; i < MAX_ROWS / THREADS; ++i) {
         const int b = tid * each + i;
-        units[i] = 0;
-        if (i < each && b < rows) {
-            int lo, hi;
-            range_of(p.a, b, lo, hi);
-            units[i] = units_of(lo, hi);
-        }
+        units[i] = i < each && b < rows ? units_of(p.a, p.a.lengths[b]) : 0;
         mine += units[i];
     }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) mine += __shfl_xor(mine, m);
-    if (lane == 0) sum_units[wave] = mine;
-    if (tid == 0) found[0] = -1;
+    const int sum = scan(mine, lane);
+    if (lane == 63) sums[wave] = sum;
     __syncthreads();
-    int64_t total = 0;
-    for (int w = 0; w < WAVES; ++w) total += sum_units[w];
-    const int per = (int)max<int64_t>(1, (total + p.per_group - 1) / p.per_group);
-    int chunks = 0, split = 0;
-#pragma unroll
-    for (int i = 0; i < MAX_ROWS / THREADS; ++i)
-        if (i < each && tid * each + i < rows) {
-            const int c = max(1, (units[i] + per - 1) / per);
-            chunks += c;
-            split += c > 1 ? c : 0;
-        }
-    int before = chunks, place = split;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int x = __shfl_up(before, m), y = __shfl_up(place, m);
-        if (lane >= m) {
-            before += x;
-            place += y;
-        }
+    int total = 0, at = sum - mine;
+    for (int v = 0; v < WAVES; ++v) {
+        at += v < wave ? sums[v] : 0;
+        total += sums[v];
     }
-    if (lane == 63) {
-        sum_chunks[wave] = before;
-        sum_split[wave] = place;
+    if (!set_share(p, w, total, s)) return false;
+#pragma unroll
+    for (int i = 0; i < MAX_ROWS / THREADS; ++i) {
+        if (s.unit >= at && s.unit < at + units[i]) {
+            found[0] = tid * each + i;
+            found[1] = at;
+        }
+        at += units[i];
     }
     __syncthreads();
-    before -= chunks;
-    place -= split;
-    for (int w = 0; w < wave; ++w) {
-        before += sum_chunks[w];
-        place += sum_split[w];
-    }
-#pragma unroll
-    for (int i = 0; i < MAX_ROWS / THREADS; ++i)
-        if (i < each && tid * each + i < rows) {
-            const int c = max(1, (units[i] + per - 1) / per);
-            if (item >= before && item < before + c) {
-                found[0] = tid * each + i;
-                found[1] = item - before;
-                found[2] = c;
-                found[3] = place;
-            }
-            before += c;
-            place += c > 1 ? c : 0;
-        }
-    __syncthreads();
-    it.b = __builtin_amdgcn_readfirstlane(found[0]);
-    if (it.b < 0) return false;
-    it.chunk = __builtin_amdgcn_readfirstlane(found[1]);
-    it.chunks = __builtin_amdgcn_readfirstlane(found[2]);
-    it.place = __builtin_amdgcn_readfirstlane(found[3]);
-    range_of(p.a, it.b, it.lo, it.hi);
-    it.lo = __builtin_amdgcn_readfirstlane(it.lo);
-    it.hi = __builtin_amdgcn_readfirstlane(it.hi);
-    const int64_t start = (it.lo & ~(TILE - 1)) + (int64_t)it.chunk * per * UNIT;
-    it.start = (int)min<int64_t>(start, it.hi);
-    it.end = (int)min<int64_t>(start + (int64_t)per * UNIT, it.hi);
+    s.b = __builtin_amdgcn_readfirstlane(found[0]);
+    s.first = __builtin_amdgcn_readfirstlane(found[1]);
     return true;
 }
 
@@ -208,25 +203,12 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
     const PagedAttentionArgs& a = p.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;  // column (a head) and row group
-    const int hg = a.Hk * p.ng, hgi = blockIdx.x % hg;
-    Item it;
-    if (!find_item(p, blockIdx.x / hg, it)) return;
+    const int hg = a.Hk * p.ng, hgi = blockIdx.x % hg, share = blockIdx.x / hg;
+    Share sh;
+    if (a.B <= 64 ? !find_share_wave(p, share, sh) : !find_share(p, share, sh)) return;
     const int kvh = hgi / p.ng, G = a.H / a.Hk, h0 = (hgi % p.ng) * p.hpg, heads = min(p.hpg, G - h0);
-    if (p.join && hgi == 0 && it.chunk == 0 && threadIdx.x == 0) p.meta[it.b] = make_int2(it.chunks, it.place);
-
-    // Q^T: column n is a head; up to 8 heads the columns 8 .. 15 repeat them for the weights' second part
-    const int col = WIDE ? n : n & 7;
-    u32x4 q[KS];
-#pragma unroll
-    for (int j = 0; j < KS; ++j) {
-        q[j] = u32x4{0, 0, 0, 0};
-        if (col < heads && 32 * j + 8 * g < a.D)
-            q[j] = *reinterpret_cast<const u32x4*>((const uint16_t*)a.q.p + it.b * a.q.st +
-                                                   (int64_t)(kvh * G + h0 + col) * a.q.sh + 32 * j + 8 * g);
-    }
     const uint16_t* kbase = (const uint16_t*)a.kc.p + kvh * a.kc.sh;
     const uint16_t* vbase = (const uint16_t*)a.vc.p + kvh * a.vc.sh;
-    const int32_t* table = a.table + it.b * a.ldt;
 
     // byte offsets within 16 tokens of a page
     uint32_t kofs[KS], vofs[VL];
@@ -241,23 +223,39 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
 
     u32x4 kr[2][KS];
     VT vr[8][VL];
-    // A tile's place: P16 the two halves' block and first place in it; else lane t & 31 has token t's.
+    int lo = 0, hi = 0;                  // the row's tokens that count
+    int64_t row = 0;                     // the row's entries in the table
+    // A tile's table entries: P16 the two halves'; else lane t & 31 has token t's.  Read a tile ahead of their use.
+    struct Entries {
+        int block[2];
+    };
+    auto entries = [&](int t) {
+        Entries x;
+        if constexpr (P16) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                x.block[h] = ((ScalarInts)a.table)[row + min((int64_t)divided((uint32_t)t / 16 + h, p.page_magic), a.W - 1)];
+        } else {
+            x.block[0] = a.table[row + min((int64_t)divided((uint32_t)t + (lane & 31), p.page_magic), a.W - 1)];
+        }
+        return x;
+    };
+    // Its places in the cache: block and first place in it, tokens that are there.
     struct Tile {
         int block[2], place[2];
         uint32_t mask;
     };
-    auto locate = [&](int t) {
+    auto locate = [&](int t, const Entries& from) {
         Tile x;
-        x.mask = bits_in(t, it.lo, it.hi);
+        x.mask = bits_in(t, lo, hi);
         if constexpr (P16) {
             const uint32_t per_page = (uint32_t)(a.page >> 4);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t s = (uint32_t)t / 16 + h, pg = divided(s, p.page_magic);
-                x.place[h] = (int)(s - pg * per_page) * 16;
-                x.block[h] = -1;
-                if ((x.mask >> (16 * h)) & 0xFFFFu) x.block[h] = __builtin_amdgcn_readfirstlane(table[pg]);
-                if ((uint32_t)x.block[h] >= (uint32_t)a.blocks) {
+                const uint32_t s = (uint32_t)t / 16 + h;
+                x.place[h] = (int)(s - divided(s, p.page_magic) * per_page) * 16;
+                x.block[h] = from.block[h];
+                if (!((x.mask >> (16 * h)) & 0xFFFFu) || (uint32_t)x.block[h] >= (uint32_t)a.blocks) {
                     x.block[h] = 0;
                     x.place[h] = 0;
                     x.mask &= h ? 0x0000FFFFu : 0xFFFF0000u;
@@ -265,12 +263,10 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
             }
         } else {
             const int tok = lane & 31;
-            const uint32_t s = (uint32_t)t + tok, pg = divided(s, p.page_magic);
-            int block = -1;
-            if ((x.mask >> tok) & 1) block = table[pg];
-            const bool ok = (uint32_t)block < (uint32_t)a.blocks;
-            x.block[0] = ok ? block : 0;
-            x.place[0] = ok ? (int)(s - pg * (uint32_t)a.page) : 0;
+            const uint32_t s = (uint32_t)t + tok;
+            const bool ok = ((x.mask >> tok) & 1) && (uint32_t)from.block[0] < (uint32_t)a.blocks;
+            x.block[0] = ok ? from.block[0] : 0;
+            x.place[0] = ok ? (int)(s - divided(s, p.page_magic) * (uint32_t)a.page) : 0;
             x.mask = (uint32_t)__ballot(ok);
         }
         return x;
@@ -328,185 +324,225 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
     };
 
     const float c = a.scale * 1.4426950408889634f;  // weights are powers of two
-    f32x4 acc[EPL] = {};
-    float m = -INFINITY, l = 0.0f;
-    int t = it.start + wave * TILE;
-    if (t < it.end) {
-        Tile x = locate(t);
-        load_k(x);
-        load_v(x);
-        while (true) {
-            f32x4 s0 = {}, s1 = {};
+    for (; sh.unit < sh.end; ++sh.b) {
+        const int length = ((ScalarInts)a.lengths)[sh.b];
+        range_of(a, length, lo, hi);
+        row = sh.b * a.ldt;
+        const int units = units_of(a, length), last = min(sh.end, sh.first + units);
+        const int start = (lo & ~(TILE - 1)) + (sh.unit - sh.first) * UNIT;
+        const int end = (int)min((int64_t)start + (int64_t)(last - sh.unit) * UNIT, (int64_t)hi);
+        const int share0 = sh.first / sh.per, shares = (sh.first + units - 1) / sh.per - share0 + 1;
+        if (p.join && hgi == 0 && sh.unit == sh.first && threadIdx.x == 0)
+            p.meta[sh.b] = make_int4(share0, shares, sh.first != share0 * sh.per, 0);
+
+        // Q^T: column n is a head; up to 8 heads the columns 8 .. 15 repeat them for the weights' second part
+        const int col = WIDE ? n : n & 7;
+        u32x4 q[KS];
 #pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                s0 = Mma<DT>::mul(kr[0][j], q[j], s0);
-                s1 = Mma<DT>::mul(kr[1][j], q[j], s1);
-            }
-            const int tn = t + UNIT;
-            const bool more = tn < it.end;
-            Tile y = x;
-            if (more) {
-                y = locate(tn);
-                load_k(y);
-            }
-            float s[8];
+        for (int j = 0; j < KS; ++j) {
+            q[j] = u32x4{0, 0, 0, 0};
+            if (col < heads && 32 * j + 8 * g < a.D)
+                q[j] = *reinterpret_cast<const u32x4*>((const uint16_t*)a.q.p + sh.b * a.q.st +
+                                                       (int64_t)(kvh * G + h0 + col) * a.q.sh + 32 * j + 8 * g);
+        }
+        f32x4 acc[EPL] = {};
+        float m = -INFINITY, l = 0.0f;
+        int t = start + wave * TILE;
+        if (t < end) {
+            Tile x = locate(t, entries(t));
+            Entries ahead = entries(t + UNIT);
+            load_k(x);
+            load_v(x);
+            while (true) {
+                f32x4 s0 = {}, s1 = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[i] = s0[i] * c;
-                s[4 + i] = s1[i] * c;
-            }
-            if (x.mask != ~0u) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (!((x.mask >> (16 * (i / 4) + 4 * g + i % 4)) & 1)) s[i] = -INFINITY;
-            }
-            float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-            mt = fmaxf(mt, __shfl_xor(mt, 16));
-            mt = fmaxf(mt, __shfl_xor(mt, 32));
-            const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.0f : mn;
-            const float keep = __builtin_amdgcn_exp2f(m - base);
-            m = mn;
-            float w[8], sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(s[i] - base);
-                sum += w[i];
-            }
-            l = l * keep + sum;
-            u32x4 ph, pl;
-            if constexpr (WIDE) {
+                for (int j = 0; j < KS; ++j) {
+                    s0 = Mma<DT>::mul(kr[0][j], q[j], s0);
+                    s1 = Mma<DT>::mul(kr[1][j], q[j], s1);
+                }
+                const int tn = t + UNIT;
+                const bool more = tn < end;
+                Tile y = x;
+                if (more) {
+                    y = locate(tn, ahead);
+                    ahead = entries(tn + UNIT);
+                    load_k(y);
+                }
+                float s[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
-                    pl[i] = Mma<DT>::pack(w[2 * i] - Mma<DT>::rounded(w[2 * i]), w[2 * i + 1] - Mma<DT>::rounded(w[2 * i + 1]));
+                    s[i] = s0[i] * c;
+                    s[4 + i] = s1[i] * c;
                 }
-            } else {
-                const bool second = n & 8;
+                if (x.mask != ~0u) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] -= second ? Mma<DT>::rounded(w[i]) : 0.0f;
+                    for (int i = 0; i < 8; ++i)
+                        if (!((x.mask >> (16 * (i / 4) + 4 * g + i % 4)) & 1)) s[i] = -INFINITY;
+                }
+                float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+                mt = fmaxf(mt, __shfl_xor(mt, 16));
+                mt = fmaxf(mt, __shfl_xor(mt, 32));
+                const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.0f : mn;
+                const float keep = __builtin_amdgcn_exp2f(m - base);
+                m = mn;
+                float w[8], sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
+                for (int i = 0; i < 8; ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(s[i] - base);
+                    sum += w[i];
+                }
+                l = l * keep + sum;
+                u32x4 ph, pl;
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
+                        pl[i] = Mma<DT>::pack(w[2 * i] - Mma<DT>::rounded(w[2 * i]), w[2 * i + 1] - Mma<DT>::rounded(w[2 * i + 1]));
+                    }
+                } else {
+                    const bool second = n & 8;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] -= second ? Mma<DT>::rounded(w[i]) : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
+                }
+                if (__ballot(keep != 1.0f)) {
+#pragma unroll
+                    for (int j = 0; j < EPL; ++j) acc[j] *= keep;
+                }
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) {
+                    const int ld = j / 8, word = (j % 8) / 2;  // values j of the lane's 16 bytes, over its 8 tokens
+                    const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+                    u32x4 vt;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vr[2 * i + 1][ld][word], vr[2 * i][ld][word], sel);
+                    acc[j] = Mma<DT>::mul(vt, ph, acc[j]);
+                    if constexpr (WIDE) acc[j] = Mma<DT>::mul(vt, pl, acc[j]);
+                }
+                if (!more) break;
+                load_v(y);
+                x = y;
+                t = tn;
             }
-            if (__ballot(keep != 1.0f)) {
-#pragma unroll
-                for (int j = 0; j < EPL; ++j) acc[j] *= keep;
-            }
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-                const int ld = j / 8, word = (j % 8) / 2;  // values j of the lane's 16 bytes, over its 8 tokens
-                const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
-                u32x4 vt;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vr[2 * i + 1][ld][word], vr[2 * i][ld][word], sel);
-                acc[j] = Mma<DT>::mul(vt, ph, acc[j]);
-                if constexpr (WIDE) acc[j] = Mma<DT>::mul(vt, pl, acc[j]);
-            }
-            if (!more) break;
-            load_v(y);
-            x = y;
-            t = tn;
         }
-    }
 
-    // join of the four waves: lane (n, g) has dims of rows 4 g + i of its head: EPL (or 8 + 8) consecutive ones each
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if constexpr (!WIDE) {
+        // join of the four waves: lane (n, g) has dims of rows 4 g + i of its head: EPL (or 8 + 8) consecutive ones each
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if constexpr (!WIDE) {
 #pragma unroll
-        for (int j = 0; j < EPL; ++j)
+            for (int j = 0; j < EPL; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], 8);
-    }
-    if (n < OH) {
-        if (g == 0) {
-            lds_m[wave][n] = m;
-            lds_l[wave][n] = l;
+                for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], 8);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < EPL; j += 4) {
-                const int d = (EPL < 8 ? EPL : 8) * (4 * g + i) + (j / 8) * 128 + j % 8;
-                *reinterpret_cast<f32x4*>(&lds_o[wave][n][d]) = f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+        if (n < OH) {
+            if (g == 0) {
+                lds_m[wave][n] = m;
+                lds_l[wave][n] = l;
             }
-    }
-    __syncthreads();
-    const int quads = a.D / 4;
-    for (int idx = threadIdx.x; idx < heads * quads; idx += THREADS) {
-        const int h = idx / quads, d = (idx - h * quads) * 4;
-        float mm = lds_m[0][h];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, lds_m[w][h]);
-        const float base = mm == -INFINITY ? 0.0f : mm;
-        float ll = 0.0f;
-        f32x4 o = {};
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const float f = __builtin_amdgcn_exp2f(lds_m[w][h] - base);
-            ll += lds_l[w][h] * f;
-            o += *reinterpret_cast<const f32x4*>(&lds_o[w][h][d]) * f;
+                for (int j = 0; j < EPL; j += 4) {
+                    const int d = (EPL < 8 ? EPL : 8) * (4 * g + i) + (j / 8) * 128 + j % 8;
+                    *reinterpret_cast<f32x4*>(&lds_o[wave][n][d]) = f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+                }
         }
-        const int head = kvh * G + h0 + h;
-        if (it.chunks == 1) {
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-            const float v[4] = {ll == 0.0f ? 0.0f : o[0] * inv, ll == 0.0f ? 0.0f : o[1] * inv, ll == 0.0f ? 0.0f : o[2] * inv,
-                                ll == 0.0f ? 0.0f : o[3] * inv};
-            store4_rt(a.out.p, DT, it.b * a.out.st + head * a.out.sh + d, v, 4, true);
-        } else {
-            const int64_t at = ((int64_t)(it.place + it.chunk) * hg + hgi) * p.hpg + h;
-            *reinterpret_cast<f32x4*>(p.part_o + at * a.D + d) = o;
-            if (d == 0) {
-                p.part_ml[2 * at] = mm;
-                p.part_ml[2 * at + 1] = ll;
+        __syncthreads();
+        const int quads = a.D / 4;
+        for (int idx = threadIdx.x; idx < heads * quads; idx += THREADS) {
+            const int h = idx / quads, d = (idx - h * quads) * 4;
+            float mm = lds_m[0][h];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, lds_m[w][h]);
+            const float base = mm == -INFINITY ? 0.0f : mm;
+            float ll = 0.0f;
+            f32x4 o = {};
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float f = __builtin_amdgcn_exp2f(lds_m[w][h] - base);
+                ll += lds_l[w][h] * f;
+                o += *reinterpret_cast<const f32x4*>(&lds_o[w][h][d]) * f;
+            }
+            const int head = kvh * G + h0 + h;
+            if (shares == 1) {
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+                const float v[4] = {ll == 0.0f ? 0.0f : o[0] * inv, ll == 0.0f ? 0.0f : o[1] * inv, ll == 0.0f ? 0.0f : o[2] * inv,
+                                    ll == 0.0f ? 0.0f : o[3] * inv};
+                store4_rt(a.out.p, DT, sh.b * a.out.st + head * a.out.sh + d, v, 4, true);
+            } else {
+                // of one share only the first and the last row can be split
+                const int place = 2 * share + (sh.unit != share * sh.per);
+                const int64_t at = ((int64_t)place * hg + hgi) * p.hpg + h;
+                *reinterpret_cast<f32x4*>(p.part_o + at * a.D + d) = o;
+                if (d == 0) {
+                    p.part_ml[2 * at] = mm;
+                    p.part_ml[2 * at + 1] = ll;
+                }
             }
         }
+        __syncthreads();
+        sh.unit = last;
+        sh.first += units;
     }
 }
 
-// out of a split row from its chunks' (O, m, l): a workgroup takes `each` heads of one row, its groups of D / 4 threads
-// the chunks in turn.
+// out of a split row from its parts' (O, m, l).  A workgroup takes `each` heads of one row in turn: the parts'
+// weights first, a thread a part, then the parts' O over groups of D / 4 threads, JOIN of them in flight.
+constexpr int JOIN = 4;
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(Launch p, int each) {
     __shared__ f32x4 lds_o[THREADS];
-    __shared__ float lds_m[THREADS], lds_l[THREADS];
+    __shared__ float lds_w[MOST_GROUPS], lds_m[WAVES], lds_l[WAVES];
     const PagedAttentionArgs& a = p.a;
-    const int2 meta = p.meta[blockIdx.x];
-    if (meta.x <= 1) return;
-    const int quads = a.D / 4, groups = THREADS / quads, grp = threadIdx.x / quads, dq = threadIdx.x % quads;
+    const int4 meta = p.meta[blockIdx.x];
+    if (meta.y <= 1) return;
+    const int tid = threadIdx.x, wave = tid >> 6, parts = meta.y;
+    const int quads = a.D / 4, groups = THREADS / quads, grp = tid / quads, dq = tid % quads;
     const int G = a.H / a.Hk, hg = a.Hk * p.ng;
     for (int head = blockIdx.y * each; head < min(a.H, (int)(blockIdx.y + 1) * each); ++head) {
-        const int kvh = head / G, in = head - kvh * G, hgi = kvh * p.ng + in / p.hpg, h = in % p.hpg;
-        float m = -INFINITY, l = 0.0f;
-        f32x4 o = {};
-        if (grp < groups)
-            for (int i = grp; i < meta.x; i += groups) {
-                const int64_t at = ((int64_t)(meta.y + i) * hg + hgi) * p.hpg + h;
-                const float mi = p.part_ml[2 * at], li = p.part_ml[2 * at + 1];
-                const f32x4 oi = *reinterpret_cast<const f32x4*>(p.part_o + at * a.D + 4 * dq);
-                const float mn = fmaxf(m, mi), base = mn == -INFINITY ? 0.0f : mn;
-                const float f = __builtin_amdgcn_exp2f(m - base), fi = __builtin_amdgcn_exp2f(mi - base);
-                l = l * f + li * fi;
-                o = o * f + oi * fi;
-                m = mn;
-            }
-        lds_o[threadIdx.x] = o;
-        lds_m[threadIdx.x] = m;
-        lds_l[threadIdx.x] = l;
+        const int kvh = head / G, in = head - kvh * G, hgi = kvh * p.ng + in / p.hpg;
+        // the row's part in share i: the share's first, but for the row that starts within its first share
+        const int64_t one = (int64_t)hg * p.hpg, from = (int64_t)hgi * p.hpg + in % p.hpg;
+        const auto place = [&](int i) { return (2 * (meta.x + i) + (i == 0 ? meta.z : 0)) * one + from; };
+        float m = -INFINITY;
+        for (int i = tid; i < parts; i += THREADS) m = fmaxf(m, p.part_ml[2 * place(i)]);
+        m = wave_max(m);
+        if ((tid & 63) == 0) lds_m[wave] = m;
         __syncthreads();
-        if (threadIdx.x < quads) {
-            float mm = -INFINITY;
-            for (int i = 0; i < groups; ++i) mm = fmaxf(mm, lds_m[i * quads + dq]);
-            const float base = mm == -INFINITY ? 0.0f : mm;
-            float ll = 0.0f;
-            f32x4 s = {};
-            for (int i = 0; i < groups; ++i) {
-                const float f = __builtin_amdgcn_exp2f(lds_m[i * quads + dq] - base);
-                ll += lds_l[i * quads + dq] * f;
-                s += lds_o[i * quads + dq] * f;
+        m = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
+        const float base = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+        for (int i = tid; i < parts; i += THREADS) {
+            const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * place(i)] - base);
+            lds_w[i] = w;
+            l += w * p.part_ml[2 * place(i) + 1];
+        }
+        l = wave_sum(l);
+        if ((tid & 63) == 0) lds_l[wave] = l;
+        __syncthreads();
+        l = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
+        f32x4 o = {};
+        if (grp < groups) {
+            const float* part = p.part_o + 4 * dq;
+            int i = grp;
+            for (; i + (JOIN - 1) * groups < parts; i += JOIN * groups) {
+                f32x4 x[JOIN];
+#pragma unroll
+                for (int u = 0; u < JOIN; ++u) x[u] = *reinterpret_cast<const f32x4*>(part + place(i + u * groups) * a.D);
+#pragma unroll
+                for (int u = 0; u < JOIN; ++u) o += x[u] * lds_w[i + u * groups];
             }
-            const float inv = 1.0f / ll;
-            const float v[4] = {ll == 0.0f ? 0.0f : s[0] * inv, ll == 0.0f ? 0.0f : s[1] * inv, ll == 0.0f ? 0.0f : s[2] * inv,
-                                ll == 0.0f ? 0.0f : s[3] * inv};
-            store4_rt(a.out.p, a.dtype, blockIdx.x * a.out.st + head * a.out.sh + 4 * dq, v, 4, true);
+            for (; i < parts; i += groups) o += *reinterpret_cast<const f32x4*>(part + place(i) * a.D) * lds_w[i];
+        }
+        lds_o[tid] = o;
+        __syncthreads();
+        if (tid < quads) {
+            for (int i = 1; i < groups; ++i) o += lds_o[i * quads + tid];
+            const float inv = 1.0f / l;
+            const float v[4] = {l == 0.0f ? 0.0f : o[0] * inv, l == 0.0f ? 0.0f : o[1] * inv, l == 0.0f ? 0.0f : o[2] * inv,
+                                l == 0.0f ? 0.0f : o[3] * inv};
+            store4_rt(a.out.p, a.dtype, blockIdx.x * a.out.st + head * a.out.sh + 4 * tid, v, 4, true);
         }
         __syncthreads();
     }
@@ -517,7 +553,7 @@ void head_groups(int64_t G, int& ng, int& hpg) {
     ng = (int)((G + 15) / 16);
     hpg = (int)((G + ng - 1) / ng);
 }
-int64_t chunks_per_group(int64_t hg) { return std::max<int64_t>(1, TARGET / hg); }
+int64_t shares_of(int64_t hg, int64_t D) { return std::max<int64_t>(1, held(D) / hg); }
 
 template <int DT, int DP>
 hipError_t launch(const Launch& p, bool p16, unsigned grid, hipStream_t st) {
@@ -537,7 +573,7 @@ hipError_t launch_dim(const Launch& p, bool p16, unsigned grid, hipStream_t st) 
     return launch<DT, 256>(p, p16, grid, st);
 }
 
-constexpr size_t META_BYTES = MAX_ROWS * sizeof(int2);
+constexpr size_t META_BYTES = MAX_ROWS * sizeof(int4);
 
 }  // namespace
 
@@ -545,7 +581,7 @@ size_t ws_paged_attention(int64_t, int64_t H, int64_t Hk, int64_t D) {
     if (Hk < 1 || H < Hk) return 0;
     int ng, hpg;
     head_groups(H / Hk, ng, hpg);
-    const size_t heads = (size_t)(2 * chunks_per_group(Hk * ng) * Hk * ng) * hpg;
+    const size_t heads = (size_t)(2 * shares_of(Hk * ng, D) * Hk * ng) * hpg;
     return META_BYTES + heads * 8 + heads * D * 4 + 256;
 }
 
@@ -553,34 +589,33 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
     Launch p;
     head_groups(a.H / a.Hk, p.ng, p.hpg);
     const int64_t hg = (int64_t)a.Hk * p.ng;
-    p.per_group = (int)chunks_per_group(hg);
+    p.shares = (int)shares_of(hg, a.D);
     // 16-token tiles whose places are reached by 32-bit offsets from a uniform address
     const auto near = [](int64_t sp) { return sp >= 0 && sp < (1 << 24); };
     const bool p16 = a.page % 16 == 0 && near(a.kc.sp) && near(a.vc.sp);
     const uint64_t d = (uint64_t)(p16 ? a.page / 16 : a.page);
     p.page_magic = d == 1 ? 0 : ~0ull / d + 1;
-    const size_t heads = (size_t)(2 * p.per_group * hg) * p.hpg;
+    const size_t heads = (size_t)(2 * p.shares * hg) * p.hpg;
     uint8_t* ws = (uint8_t*)a.ws;
-    p.meta = (int2*)ws;
+    p.meta = (int4*)ws;
     p.part_ml = (float*)(ws + META_BYTES);
     p.part_o = (float*)(ws + META_BYTES + (heads * 8 + 255) / 256 * 256);
-    const int64_t rows = std::min<int64_t>(MAX_ROWS, (1 << 23) / hg);  // a grid holds 2^32 threads
+    int64_t W = a.blocks == 0 ? 0 : std::min<int64_t>(a.W, 0x7FFFFF00 / a.page);  // positions stay 32-bit
+    // units a row can have at most: rows that cannot be split need no second kernel
+    int64_t most = (W * a.page + UNIT - 1) / UNIT;
+    if (a.window) most = std::min<int64_t>(most, a.window / UNIT + 2);
+    most = std::max<int64_t>(most, 1);
+    const int64_t rows = std::min<int64_t>(MAX_ROWS, (1 << 30) / most);  // sums of units stay 32-bit
     for (int64_t b0 = 0; b0 < a.B; b0 += rows) {
         p.a = a;
+        p.a.W = W;
         p.a.B = std::min<int64_t>(rows, a.B - b0);
         p.a.q.p = (uint16_t*)a.q.p + b0 * a.q.st;
         p.a.out.p = (uint16_t*)a.out.p + b0 * a.out.st;
         p.a.table = a.table + b0 * a.ldt;
         p.a.lengths = a.lengths + b0;
-        if (a.blocks == 0) p.a.W = 0;
-        p.a.W = std::min<int64_t>(p.a.W, 0x7FFFFF00 / a.page);  // positions stay 32-bit
-        // units a row can have at most: a row that cannot be split needs no second kernel
-        int64_t most = (p.a.W * a.page + UNIT - 1) / UNIT;
-        if (a.window) most = std::min<int64_t>(most, (a.window + TILE - 1 + UNIT - 1) / UNIT);
-        most = std::max<int64_t>(most, 1);
         p.join = most > 1;
-        const int64_t items = std::min<int64_t>(p.per_group + p.a.B, most * p.a.B);
-        const unsigned grid = (unsigned)(items * hg);
+        const unsigned grid = (unsigned)(std::min<int64_t>(p.shares, most * p.a.B) * hg);
         hipError_t e = a.dtype == DT_F16 ? launch_dim<DT_F16>(p, p16, grid, st) : launch_dim<DT_BF16>(p, p16, grid, st);
         if (e != hipSuccess) return e;
         if (p.join) {
