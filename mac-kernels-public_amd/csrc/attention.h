@@ -74,9 +74,9 @@ struct HeadGradArgs {
     void* dwq = nullptr;               // [D] or nullptr (not formed)
     void* dwk = nullptr;
     int dwq_dt = DT_F32, dwk_dt = DT_F32;
-    float* part = nullptr;             // head_grad_parts() x [2][D] partial sums
+    float* part = nullptr;             // head_grad_parts() x [D] partial sums, q's then k's
 };
-// Workgroups of the gradient kernel, each of which leaves one partial [2][D].
+// Workgroups of the gradient kernel, each of which leaves one partial [D].
 int head_grad_parts(int64_t T, int64_t heads);
 hipError_t run_head_grad(const HeadGradArgs& a, hipStream_t st);
 size_t ws_head_grad(int64_t T, int64_t heads, int64_t D);

@@ -15,9 +15,9 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int MAX_TOKENS = 8;         // tokens of one workgroup
-constexpr int WORKGROUPS = 2048;      // that a large call is cut into at least (8 on a compute unit)
-constexpr int GRAD_WORKGROUPS = 1024;
-constexpr int MOST_ROUNDS = 12;       // rows of one lane group, at most
+constexpr int WORKGROUPS = 2048;      // of one round each: a call of more rows takes several rounds a workgroup
+constexpr int GRAD_WORKGROUPS = 1152; // 4 on a compute unit are held, and what is left over of an eighth
+constexpr int MOST_ROUNDS = 8;        // rows of one lane group, at most
 
 template <int DT> struct HeadType;
 template <> struct HeadType<DT_F32> { using T = float; };
@@ -41,39 +41,64 @@ __device__ __forceinline__ void turn_at(const RopeTurn& r, int pair, int64_t t, 
     if (r.inverse) s = -s;
 }
 
+// row / heads for the rows of a few tokens (row * heads < 2^32), by ceil(2^32 / heads).
+struct Divisor {
+    int heads = 1;
+    uint32_t magic = 0;
+    Divisor() = default;
+    explicit Divisor(int h) : heads(h), magic(h > 1 ? (uint32_t)((0x100000000ull + h - 1) / h) : 0) {}
+    // the magic number of one head would be 2^32
+    __device__ __forceinline__ int operator()(int r) const { return heads <= 1 ? r : (int)__umulhi((uint32_t)r, magic); }
+};
+
 // How a call is cut: `lanes` a row, `heads` rows a token (store: v's too), `tokens` tokens and `span` rows of
 // them a workgroup (span < heads: one token over several workgroups).
 struct Cut {
     int lanes = 1, heads = 0, tokens = 1, span = 0;
-    uint32_t magic = 0;   // ceil(2^32 / heads), for row / heads of two and more
+    Divisor by_heads;
 };
 
 // The values a lane holds of a row: x[e] and x[VW + e] are a pair, or x[2 e] and x[2 e + 1] of interleaved ones.
-// VEC: two vectors; else value by value (any D and P).  A lane past the row's end holds zeros.
+// VEC: two vectors, which neighbouring lanes continue; else value by value (any D and P).  A lane past the row's
+// end holds zeros.
 template <typename T, int VW, bool VEC, bool INTER>
 struct Piece {
     static constexpr int N = 2 * VW;
     struct alignas(sizeof(T) * VW < 16 ? sizeof(T) * VW : 16) Vector { T v[VW]; };
     int first, second;    // VEC: where the vectors start
-    int pair;             // the first pair's number
+    int pair;             // the first pair's number; VEC INTER: the second vector's first pair is pair2
+    int pair2;
     int D, P;
     bool inside;
-    __device__ __forceinline__ Piece(int unit, int D_, int P_) : pair(VW * unit), D(D_), P(P_) {
-        if (INTER || pair >= P) {
+    __device__ __forceinline__ Piece(int unit, int D_, int P_) : pair(VW * unit), pair2(VW * unit + VW / 2), D(D_), P(P_) {
+        inside = 2 * pair < D;
+        if (INTER) {
+            first = VW * unit;
+            second = D / 2 + first;
+            if (VEC) {
+                pair = first / 2;
+                pair2 = second / 2;
+            }
+        } else if (pair >= P) {
             first = N * unit;
             second = first + VW;
         } else {
             first = VW * unit;
             second = P + first;
         }
-        inside = 2 * pair < D;
     }
     // Where value j is in the row; -1 for none.
     __device__ __forceinline__ int at(int j) const {
-        if (VEC && !INTER && pair >= P) return inside ? first + j : -1;
+        if (VEC) return inside ? (j < VW ? first + j : second + j - VW) : -1;
         const int i = pair + (INTER ? j / 2 : j % VW), half = INTER ? j % 2 : j / VW;
         const int d = i < P && !INTER ? i + half * P : 2 * i + half;
         return d < D ? d : -1;
+    }
+    // The VW pairs' entries of a table of all pairs.
+    __device__ __forceinline__ void turns(const float* table, float* x) const {
+        typedef float V __attribute__((ext_vector_type(VW / 2)));
+        *reinterpret_cast<V*>(x) = *reinterpret_cast<const V*>(table + pair);
+        *reinterpret_cast<V*>(x + VW / 2) = *reinterpret_cast<const V*>(table + (VEC && INTER ? pair2 : pair + VW / 2));
     }
     struct Raw { Vector a, b; };
     __device__ __forceinline__ Raw load(const T* row, bool wanted) const {
@@ -198,8 +223,7 @@ __global__ __launch_bounds__(THREADS) void head_rope_kernel(HeadRopeArgs a, Cut 
     };
     const auto row_of = [&](int r) {
         Row x;
-        // the magic number of one head would be 2^32
-        x.token = cut.tokens == 1 ? 0 : cut.heads == 1 ? r : (int)__umulhi((uint32_t)r, cut.magic);
+        x.token = cut.tokens == 1 ? 0 : cut.by_heads(r);
         x.h = r - x.token * cut.heads;
         x.kind = x.h < a.Hq ? 0 : x.h < a.Hq + a.Hk ? 1 : 2;
         x.h -= x.kind == 0 ? 0 : x.kind == 1 ? a.Hq : a.Hq + a.Hk;
@@ -260,8 +284,8 @@ __global__ __launch_bounds__(THREADS) void head_rope_kernel(HeadRopeArgs a, Cut 
             }
             if (piece.inside) {
                 float c[VW], s[VW];
-                read_row<VW>(h.c + row.token * h.stride + piece.pair, c);
-                read_row<VW>(h.s + row.token * h.stride + piece.pair, s);
+                piece.turns(h.c + row.token * h.stride, c);
+                piece.turns(h.s + row.token * h.stride, s);
 #pragma unroll
                 for (int e = 0; e < VW; ++e) {
                     const float u = PC::u(x, e), v = PC::v(x, e);
@@ -276,117 +300,100 @@ __global__ __launch_bounds__(THREADS) void head_rope_kernel(HeadRopeArgs a, Cut 
     }
 }
 
-// Sums of the weights' gradients stay in a lane over all its rows and are added up over the workgroup at
-// the end, in a fixed order; every workgroup leaves one partial [2][D].
+// A workgroup takes q's rows (workgroups below parts_q) or k's.  Sums of the weight's gradient stay in a lane over all
+// its rows and are added up over the workgroup at the end, in a fixed order; every workgroup leaves one partial [D].
 template <int DT, int VW, bool VEC, bool INTER>
-__global__ __launch_bounds__(THREADS) void head_grad_kernel(HeadGradArgs a, Cut cut) {
+__global__ __launch_bounds__(THREADS, VEC ? 4 : 1) void head_grad_kernel(HeadGradArgs a, Cut cut, Divisor by_q, Divisor by_k, int parts_q) {
     using T = typename HeadType<DT>::T;
     using PC = Piece<T, VW, VEC, INTER>;
-    const int units = (a.D + 2 * VW - 1) / (2 * VW);
+    const bool of_k = (int)blockIdx.x >= parts_q;
+    const int units = (a.D + 2 * VW - 1) / (2 * VW), heads = of_k ? a.Hk : a.Hq;
+    const Divisor by_heads = of_k ? by_k : by_q;
     const int unit = threadIdx.x & (cut.lanes - 1), group = threadIdx.x / cut.lanes, groups = THREADS / cut.lanes;
+    const int part = of_k ? blockIdx.x - parts_q : blockIdx.x, parts = of_k ? gridDim.x - parts_q : parts_q;
+    const HeadView in = of_k ? a.k : a.q, gin = of_k ? a.gk : a.gq, out = of_k ? a.dk : a.dq;
     const PC piece(unit, a.D, a.turn.P);
     const Shared h = shared_part<PC, VW>(lds, units, cut.tokens);
-    fill_weights<PC, VW>(h, units, a.D, a.turn.P, a.wq, a.wq_dt, a.wk, a.wk_dt);
-    float dw[2][PC::N] = {};
-    for (int64_t t0 = (int64_t)blockIdx.x * cut.tokens; t0 < a.T; t0 += (int64_t)gridDim.x * cut.tokens) {
-        const int tokens = (int)min<int64_t>(cut.tokens, a.T - t0);
+    fill_weights<PC, VW>(h, units, a.D, a.turn.P, of_k ? a.wk : a.wq, of_k ? a.wk_dt : a.wq_dt, nullptr, 0);
+    float dw[PC::N] = {};
+    for (int64_t t0 = (int64_t)part * cut.tokens; t0 < a.T; t0 += (int64_t)parts * cut.tokens) {
+        const int tokens = (int)min<int64_t>(cut.tokens, a.T - t0), end = tokens * heads;
         __syncthreads();
         fill_turns(h, a.turn, t0, tokens);
         __syncthreads();
+        for (int r = group; r < end; r += groups) {
+            const int token = cut.tokens == 1 ? 0 : by_heads(r), head = r - token * heads;
+            const typename PC::Raw rx = piece.load((const T*)in.p + (t0 + token) * in.st + head * in.sh, true);
+            const typename PC::Raw rg = piece.load((const T*)gin.p + (t0 + token) * gin.st + head * gin.sh, true);
+            float x[PC::N], g[PC::N];
+            PC::values(rx, x);
+            PC::values(rg, g);
+            float sum = 0.0f;
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            const HeadView &in = kind ? a.k : a.q, &gin = kind ? a.gk : a.gq, &out = kind ? a.dk : a.dq;
-            const int heads = kind ? a.Hk : a.Hq, end = tokens * heads;
-            struct Two {
-                typename PC::Raw x, g;
-                int token, h;
-            };
-            const auto load = [&](int r) {
-                Two w;
-                w.token = heads > 0 ? r / heads : 0;
-                w.h = r - w.token * heads;
-                w.x = piece.load((const T*)in.p + (t0 + w.token) * in.st + w.h * in.sh, r < end);
-                w.g = piece.load((const T*)gin.p + (t0 + w.token) * gin.st + w.h * gin.sh, r < end);
-                return w;
-            };
-            int r = group;
-            Two two = load(r);
-            for (; r < end; r += groups) {
-                const Two ahead = load(r + groups);
-                float x[PC::N], g[PC::N];
-                PC::values(two.x, x);
-                PC::values(two.g, g);
-                float sum = 0.0f;
+            for (int j = 0; j < PC::N; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
+            const float rstd = 1.0f / sqrtf(row_sum(sum, cut.lanes) / (float)a.D + a.eps);
+            float w[PC::N] = {};
+            if (piece.inside) {
+                float c[VW], s[VW];
+                piece.turns(h.c + token * h.stride, c);
+                piece.turns(h.s + token * h.stride, s);
 #pragma unroll
-                for (int j = 0; j < PC::N; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
-                const float rstd = 1.0f / sqrtf(row_sum(sum, cut.lanes) / (float)a.D + a.eps);
-                float w[PC::N] = {};
-                if (piece.inside) {
-                    float c[VW], s[VW];
-                    read_row<PC::N>(h.w + (kind * units + unit) * PC::N, w);
-                    read_row<VW>(h.c + two.token * h.stride + piece.pair, c);
-                    read_row<VW>(h.s + two.token * h.stride + piece.pair, s);
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) {
-                        const float u = PC::u(g, e), v = PC::v(g, e);
-                        PC::u(g, e) = u * c[e] + v * s[e];
-                        PC::v(g, e) = v * c[e] - u * s[e];
-                    }
+                for (int e = 0; e < VW; ++e) {
+                    const float u = PC::u(g, e), v = PC::v(g, e);
+                    PC::u(g, e) = u * c[e] + v * s[e];
+                    PC::v(g, e) = v * c[e] - u * s[e];
                 }
-                float dot = 0.0f;
-#pragma unroll
-                for (int j = 0; j < PC::N; ++j) {
-                    x[j] *= rstd;
-                    dw[kind][j] = __builtin_fmaf(g[j], x[j], dw[kind][j]);
-                    g[j] *= w[j];
-                    dot = __builtin_fmaf(g[j], x[j], dot);
-                }
-                dot = row_sum(dot, cut.lanes) / (float)a.D;
-#pragma unroll
-                for (int j = 0; j < PC::N; ++j) g[j] = rstd * (g[j] - x[j] * dot);
-                piece.store((T*)out.p + (t0 + two.token) * out.st + two.h * out.sh, g);
-                two = ahead;
+                read_row<PC::N>(h.w + unit * PC::N, w);
             }
+            float dot = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PC::N; ++j) {
+                x[j] *= rstd;
+                dw[j] = __builtin_fmaf(g[j], x[j], dw[j]);
+                g[j] *= w[j];
+                dot = __builtin_fmaf(g[j], x[j], dot);
+            }
+            dot = row_sum(dot, cut.lanes) / (float)a.D;
+#pragma unroll
+            for (int j = 0; j < PC::N; ++j) g[j] = rstd * (g[j] - x[j] * dot);
+            piece.store((T*)out.p + (t0 + token) * out.st + head * out.sh, g);
         }
     }
     if (!a.part) return;
     // the wave's rows, then the workgroup's waves
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, all = units * PC::N;
     __syncthreads();
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind)
-#pragma unroll
-        for (int j = 0; j < PC::N; ++j) {
-            float v = dw[kind][j];
-            for (int m = cut.lanes; m < 64; m <<= 1) v += __shfl_xor(v, m);
-            if (lane < cut.lanes && unit < units) lds[((wave * 2 + kind) * units + unit) * PC::N + j] = v;
-        }
+    for (int j = 0; j < PC::N; ++j) {
+        for (int m = cut.lanes; m < 64; m <<= 1) dw[j] += __shfl_xor(dw[j], m);
+        if (lane < cut.lanes && unit < units) lds[wave * all + unit * PC::N + j] = dw[j];
+    }
     __syncthreads();
-    const int all = 2 * units * PC::N;
     for (int i = threadIdx.x; i < all; i += THREADS) {
-        const int kind = i / (units * PC::N), j = i % (units * PC::N), d = PC(j / PC::N, a.D, a.turn.P).at(j % PC::N);
+        const int d = PC(i / PC::N, a.D, a.turn.P).at(i % PC::N);
         const float v = (lds[i] + lds[all + i]) + (lds[2 * all + i] + lds[3 * all + i]);
-        if (d >= 0) a.part[((int64_t)blockIdx.x * 2 + kind) * a.D + d] = v;
+        if (d >= 0) a.part[(int64_t)blockIdx.x * a.D + d] = v;
     }
 }
 
-// Weight gradients from the partials: a workgroup takes 16 values of q's or k's weight, 16 partials at a time.
-__global__ __launch_bounds__(THREADS) void head_grad_sum_kernel(HeadGradArgs a, int parts) {
+// Weight gradients from the partials: a workgroup takes 16 values of q's weight or of k's, 16 partials at a time.
+__global__ __launch_bounds__(THREADS) void head_grad_sum_kernel(HeadGradArgs a, int parts_q, int parts) {
     __shared__ float s[16][17];
-    const int col = threadIdx.x & 15, row = threadIdx.x >> 4, i = blockIdx.x * 16 + col;
+    const int col = threadIdx.x & 15, row = threadIdx.x >> 4, d = blockIdx.x * 16 + col;
+    const bool of_k = blockIdx.y;
+    void* dw = of_k ? a.dwk : a.dwq;
+    if (!dw) return;
     float sum = 0.0f;
-    if (i < 2 * a.D) {
+    if (d < a.D) {
 #pragma unroll 8
-        for (int p = row; p < parts; p += 16) sum += a.part[(int64_t)p * 2 * a.D + i];
+        for (int p = (of_k ? parts_q : 0) + row; p < (of_k ? parts : parts_q); p += 16) sum += a.part[(int64_t)p * a.D + d];
     }
     s[row][col] = sum;
     __syncthreads();
-    if (row == 0 && i < 2 * a.D) {
+    if (row == 0 && d < a.D) {
 #pragma unroll
         for (int p = 1; p < 16; ++p) sum += s[p][col];
-        const int kind = i / a.D, d = i - kind * a.D;
-        if (kind == 0 && a.dwq) store_rt(a.dwq, a.dwq_dt, d, sum);
-        if (kind == 1 && a.dwk) store_rt(a.dwk, a.dwk_dt, d, sum);
+        store_rt(dw, of_k ? a.dwk_dt : a.dwq_dt, d, sum);
     }
 }
 
@@ -399,14 +406,14 @@ bool aligned(const void* p, std::initializer_list<int64_t> strides, int es, int 
 }
 
 // The pieces of a call: 8 pairs a lane where both sizes allow 8-value vectors and all rows are aligned to them, else 4,
-// else 8 value by value.
+// else 8 value by value.  Vectors of interleaved pairs hold whole pairs whatever P is.
 struct Kind {
     int VW;
     bool vec;
 };
 template <typename ALIGNED>
-Kind kind_of(int D, int P, int dtype, const ALIGNED& all_aligned) {
-    const int es = dtype == DT_F32 ? 4 : 2;
+Kind kind_of(int D, const RopeTurn& turn, int dtype, const ALIGNED& all_aligned) {
+    const int es = dtype == DT_F32 ? 4 : 2, P = turn.interleaved ? 0 : turn.P;
     if (D % 16 == 0 && P % 8 == 0 && all_aligned(es, 16)) return {8, true};
     if (D % 8 == 0 && P % 4 == 0 && all_aligned(es, 4 * es)) return {4, true};
     return {8, false};
@@ -417,19 +424,29 @@ Cut cut_of(const Kind& k, int D, int heads) {
     const int units = (D + 2 * k.VW - 1) / (2 * k.VW);
     while (c.lanes < units) c.lanes *= 2;
     c.heads = heads;
+    c.by_heads = Divisor(heads);
     return c;
 }
 
-// Rounds of a workgroup's lane groups: few where the call is small, so that it spreads over the chip; more where it
-// is large, so that cosines and the launch are shared by more rows.
-int rounds_of(const Cut& c, int64_t T, int workgroups) {
-    const int64_t groups = THREADS / c.lanes, rounds = T * c.heads / (groups * workgroups);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(rounds, MOST_ROUNDS));
+// Tokens of a workgroup, at most `most`: the fewest whose rows leave the least of the lane groups' last round idle
+// (to a twentieth).
+int tokens_of(int heads, int groups, int most) {
+    int best = 1;
+    double held = 0.0;
+    for (int t = 1; t <= most; ++t) {
+        const int64_t rows = (int64_t)t * heads, rounds = (rows + groups - 1) / groups;
+        const double share = (double)rows / (double)(rounds * groups);
+        if (share > held + 0.05) {
+            held = share;
+            best = t;
+        }
+    }
+    return best;
 }
 
 size_t lds_bytes(const Kind& k, int D, int tokens, bool grad) {
     const size_t units = (D + 2 * k.VW - 1) / (2 * k.VW), w = 2 * units * 2 * k.VW, turns = 2 * (size_t)tokens * units * k.VW;
-    return 4 * (grad ? std::max(w + turns, 4 * w) : w + turns);
+    return 4 * (grad ? std::max(w + turns, 2 * w) : w + turns);
 }
 
 template <int DT, bool INTER>
@@ -442,18 +459,18 @@ hipError_t launch_rope(const HeadRopeArgs& a, const Kind& k, const Cut& c, dim3 
 }
 
 template <int DT, bool INTER>
-hipError_t launch_grad(const HeadGradArgs& a, const Kind& k, const Cut& c, dim3 grid, hipStream_t st) {
+hipError_t launch_grad(const HeadGradArgs& a, const Kind& k, const Cut& c, dim3 grid, int parts_q, hipStream_t st) {
     const size_t bytes = lds_bytes(k, a.D, c.tokens, true);
-    if (!k.vec) hipLaunchKernelGGL((head_grad_kernel<DT, 8, false, INTER>), grid, dim3(THREADS), bytes, st, a, c);
-    else if (k.VW == 8) hipLaunchKernelGGL((head_grad_kernel<DT, 8, true, INTER>), grid, dim3(THREADS), bytes, st, a, c);
-    else hipLaunchKernelGGL((head_grad_kernel<DT, 4, true, INTER>), grid, dim3(THREADS), bytes, st, a, c);
+    if (!k.vec) hipLaunchKernelGGL((head_grad_kernel<DT, 8, false, INTER>), grid, dim3(THREADS), bytes, st, a, c, Divisor(a.Hq), Divisor(a.Hk), parts_q);
+    else if (k.VW == 8) hipLaunchKernelGGL((head_grad_kernel<DT, 8, true, INTER>), grid, dim3(THREADS), bytes, st, a, c, Divisor(a.Hq), Divisor(a.Hk), parts_q);
+    else hipLaunchKernelGGL((head_grad_kernel<DT, 4, true, INTER>), grid, dim3(THREADS), bytes, st, a, c, Divisor(a.Hq), Divisor(a.Hk), parts_q);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
-    const Kind k = kind_of(a.D, a.turn.P, a.dtype, [&](int es, int bytes) {
+    const Kind k = kind_of(a.D, a.turn, a.dtype, [&](int es, int bytes) {
         if (!aligned(a.q.p, {a.q.st, a.q.sh}, es, bytes) || !aligned(a.qo.p, {a.qo.st, a.qo.sh}, es, bytes)) return false;
         if (a.Hk == 0) return true;
         if (!aligned(a.k.p, {a.k.st, a.k.sh}, es, bytes)) return false;
@@ -462,10 +479,17 @@ hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
                aligned(a.vc.p, {a.vc.sb, a.vc.sp, a.vc.sh}, es, bytes);
     });
     Cut c = cut_of(k, a.D, a.Hq + a.Hk + (a.store ? a.Hk : 0));
-    const int rows = rounds_of(c, a.T, WORKGROUPS) * (THREADS / c.lanes);
-    c.tokens = std::max(1, std::min(MAX_TOKENS, rows / c.heads));
-    c.span = c.tokens > 1 ? c.tokens * c.heads : std::min(rows, c.heads);
-    c.magic = (uint32_t)((0x100000000ull + c.heads - 1) / c.heads);
+    // A small call is spread over the chip, a row a lane group; a large one takes whole tokens, so that cosines and the
+    // launch are shared by more rows.
+    const int groups = THREADS / c.lanes;
+    const int64_t rounds = a.T * c.heads / ((int64_t)groups * WORKGROUPS);
+    if (rounds < 1) {
+        c.span = std::min(groups, c.heads);
+    } else {
+        c.tokens = tokens_of(c.heads, groups, MAX_TOKENS);
+        while (c.tokens > 1 && (int64_t)c.tokens * c.heads > (int64_t)MOST_ROUNDS * groups) --c.tokens;
+        c.span = c.tokens > 1 ? c.tokens * c.heads : std::min(c.heads, MOST_ROUNDS * groups);
+    }
     const dim3 grid((unsigned)((a.T + c.tokens - 1) / c.tokens), (unsigned)((c.tokens * c.heads + c.span - 1) / c.span));
     const bool i = a.turn.interleaved;
     if (a.dtype == DT_F32) return i ? launch_rope<DT_F32, true>(a, k, c, grid, st) : launch_rope<DT_F32, false>(a, k, c, grid, st);
@@ -473,13 +497,12 @@ hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
     return i ? launch_rope<DT_BF16, true>(a, k, c, grid, st) : launch_rope<DT_BF16, false>(a, k, c, grid, st);
 }
 
-// At most one token a workgroup less than there are, GRAD_WORKGROUPS of them at most.
-int head_grad_parts(int64_t T, int64_t) { return (int)std::max<int64_t>(1, std::min<int64_t>(T, GRAD_WORKGROUPS)); }
+int head_grad_parts(int64_t T, int64_t) { return (int)std::max<int64_t>(2, std::min<int64_t>(2 * T, GRAD_WORKGROUPS)); }
 
-size_t ws_head_grad(int64_t T, int64_t heads, int64_t D) { return (size_t)head_grad_parts(T, heads) * 2 * D * 4; }
+size_t ws_head_grad(int64_t T, int64_t heads, int64_t D) { return (size_t)head_grad_parts(T, heads) * D * 4; }
 
 hipError_t run_head_grad(const HeadGradArgs& a, hipStream_t st) {
-    const Kind k = kind_of(a.D, a.turn.P, a.dtype, [&](int es, int bytes) {
+    const Kind k = kind_of(a.D, a.turn, a.dtype, [&](int es, int bytes) {
         for (const HeadView* v : {&a.q, &a.gq, &a.dq})
             if (!aligned(v->p, {v->st, v->sh}, es, bytes)) return false;
         if (a.Hk > 0)
@@ -488,18 +511,21 @@ hipError_t run_head_grad(const HeadGradArgs& a, hipStream_t st) {
         return true;
     });
     Cut c = cut_of(k, a.D, a.Hq + a.Hk);
-    // several tokens where one has fewer heads than a workgroup lane groups
-    const int groups = THREADS / c.lanes, least = std::max(1, std::min(a.Hq, a.Hk > 0 ? a.Hk : a.Hq));
-    const int parts = head_grad_parts(a.T, a.Hq + a.Hk);
-    c.tokens = (int)std::max<int64_t>(1, std::min<int64_t>({MAX_TOKENS, groups / least, a.T / parts}));
+    // workgroups for q's rows and for k's as their heads are, each with the same number of token blocks or one less
+    const int groups = THREADS / c.lanes, most = head_grad_parts(a.T, c.heads);
+    const int most_k = std::max(1, std::min<int>(most - 1, (int)((int64_t)most * a.Hk / std::max(c.heads, 1)))), most_q = most - most_k;
+    c.tokens = tokens_of(std::max(1, std::min(a.Hq, a.Hk > 0 ? a.Hk : a.Hq)), groups, (int)std::min<int64_t>(MAX_TOKENS, std::max<int64_t>(1, 2 * a.T / most)));
+    const int64_t blocks = std::max<int64_t>(1, (a.T + c.tokens - 1) / c.tokens);
+    const auto even = [&](int n) { const int64_t each = (blocks + n - 1) / n; return (int)((blocks + each - 1) / each); };
+    const int parts_q = even(most_q), parts = parts_q + even(most_k);
     const dim3 grid((unsigned)parts);
     const bool i = a.turn.interleaved;
     hipError_t e;
-    if (a.dtype == DT_F32) e = i ? launch_grad<DT_F32, true>(a, k, c, grid, st) : launch_grad<DT_F32, false>(a, k, c, grid, st);
-    else if (a.dtype == DT_F16) e = i ? launch_grad<DT_F16, true>(a, k, c, grid, st) : launch_grad<DT_F16, false>(a, k, c, grid, st);
-    else e = i ? launch_grad<DT_BF16, true>(a, k, c, grid, st) : launch_grad<DT_BF16, false>(a, k, c, grid, st);
+    if (a.dtype == DT_F32) e = i ? launch_grad<DT_F32, true>(a, k, c, grid, parts_q, st) : launch_grad<DT_F32, false>(a, k, c, grid, parts_q, st);
+    else if (a.dtype == DT_F16) e = i ? launch_grad<DT_F16, true>(a, k, c, grid, parts_q, st) : launch_grad<DT_F16, false>(a, k, c, grid, parts_q, st);
+    else e = i ? launch_grad<DT_BF16, true>(a, k, c, grid, parts_q, st) : launch_grad<DT_BF16, false>(a, k, c, grid, parts_q, st);
     if (e != hipSuccess || (!a.dwq && !a.dwk)) return e;
-    hipLaunchKernelGGL(head_grad_sum_kernel, dim3((unsigned)((2 * a.D + 15) / 16)), dim3(THREADS), 0, st, a, parts);
+    hipLaunchKernelGGL(head_grad_sum_kernel, dim3((unsigned)((a.D + 15) / 16), 2), dim3(THREADS), 0, st, a, parts_q, parts);
     return hipGetLastError();
 }
 
