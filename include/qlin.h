@@ -305,7 +305,7 @@ qlin_status qlin_quantize_act_int8(const qlin_tensor* x, qlin_tensor* q, qlin_te
  * The attention side of a block, between its packed QKV projection and its output projection.
  *
  * Head tensors are [tokens, heads, D], f32/f16/bf16, any strides with unit stride along D (the slices
- * of a fused projection's output go in as they are), D <= 512.  16-byte aligned rows whose D and rotated size
+ * of a fused projection's output go in as they are), D <= 512, at most 16384 heads.  16-byte aligned rows whose D and rotated size
  * are multiples of 16 move in 16-byte pieces, of 8 in 8-byte ones; any other size is taken too, value
  * by value.
  *

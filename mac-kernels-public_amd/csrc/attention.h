@@ -40,6 +40,7 @@ struct RopeTurn {
 
 // ---- rotation and head norms (qk_rope.hip) ----
 constexpr int ROPE_MAX_DIM = 512;
+constexpr int ROPE_MAX_HEADS = 16384;  // of q, of k; the kernels' division of rows by heads is exact up to 3 x that
 struct HeadRopeArgs {
     int dtype = DT_F16;
     int64_t T = 0;

@@ -123,7 +123,7 @@ qlin_status head_sizes(const qlin_tensor* q, const char* name, int64_t& T, int64
     H = q->shape[1];
     D = q->shape[2];
     if (D > ROPE_MAX_DIM) return fail(QLIN_EUNSUPPORTED, "heads of %lld values, more than %d", (long long)D, ROPE_MAX_DIM);
-    if (H > 65535) return fail(QLIN_EUNSUPPORTED, "more than 65535 heads");
+    if (H > ROPE_MAX_HEADS) return fail(QLIN_EUNSUPPORTED, "more than %d heads", ROPE_MAX_HEADS);
     if (T > INT_MOST / 2) return fail(QLIN_EUNSUPPORTED, "more than %lld tokens", (long long)(INT_MOST / 2));
     return QLIN_OK;
 }
@@ -149,7 +149,7 @@ qlin_status forward_operands(const qlin_tensor* q, const qlin_tensor* k, const q
     if (qlin_status s = head_view(q, "q", a.dtype, a.T, H, D, a.q)) return s;
     if (k) {
         Hk = k->ndim == 3 ? k->shape[1] : 0;
-        if (Hk > 65535) return fail(QLIN_EUNSUPPORTED, "more than 65535 heads");
+        if (Hk > ROPE_MAX_HEADS) return fail(QLIN_EUNSUPPORTED, "more than %d heads", ROPE_MAX_HEADS);
         if (qlin_status s = head_view(k, "k", a.dtype, a.T, Hk, D, a.k)) return s;
         a.Hk = (int)Hk;
     } else if (wk) {

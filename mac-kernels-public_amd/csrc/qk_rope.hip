@@ -14,10 +14,11 @@ namespace qlin {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int MAX_TOKENS = 8;         // tokens of one workgroup
-constexpr int WORKGROUPS = 2048;      // of one round each: a call of more rows takes several rounds a workgroup
-constexpr int GRAD_WORKGROUPS = 1152; // 4 on a compute unit are held, and what is left over of an eighth
-constexpr int MOST_ROUNDS = 8;        // rows of one lane group, at most
+constexpr int MAX_TOKENS = 64;        // tokens that a workgroup's rows belong to, at most
+constexpr int WORKGROUPS = 2048;      // that a call is spread over, once or several times
+constexpr int GRAD_WORKGROUPS = 1024; // of head_grad_kernel that the chip holds at once
+constexpr int MOST_ROUNDS = 5;        // rows of one lane group, at most
+constexpr int GRAD_TOKENS = 8;        // tokens of one block of the gradient
 
 template <int DT> struct HeadType;
 template <> struct HeadType<DT_F32> { using T = float; };
@@ -51,8 +52,8 @@ struct Divisor {
     __device__ __forceinline__ int operator()(int r) const { return heads <= 1 ? r : (int)__umulhi((uint32_t)r, magic); }
 };
 
-// How a call is cut: `lanes` a row, `heads` rows a token (store: v's too), `tokens` tokens and `span` rows of
-// them a workgroup (span < heads: one token over several workgroups).
+// How a call is cut: `lanes` a row, `heads` rows a token (store: v's too).  Forward: all rows laid end to end, `span` of
+// them a workgroup, of `tokens` tokens at most.  Gradient: blocks of `tokens` tokens.
 struct Cut {
     int lanes = 1, heads = 0, tokens = 1, span = 0;
     Divisor by_heads;
@@ -212,9 +213,9 @@ __global__ __launch_bounds__(THREADS) void head_rope_kernel(HeadRopeArgs a, Cut 
     __shared__ bool stored[MAX_TOKENS];
     const int units = (a.D + 2 * VW - 1) / (2 * VW);
     const int unit = threadIdx.x & (cut.lanes - 1), group = threadIdx.x / cut.lanes, groups = THREADS / cut.lanes;
-    const int64_t t0 = (int64_t)blockIdx.x * cut.tokens;
-    const int tokens = (int)min<int64_t>(cut.tokens, a.T - t0);
-    const int begin = blockIdx.y * cut.span, end = min(begin + cut.span, tokens * cut.heads);
+    const int64_t from = (int64_t)blockIdx.x * cut.span, t0 = from / cut.heads;
+    const int begin = (int)(from - t0 * cut.heads);  // rows count from the first head of token t0
+    const int end = begin + (int)min<int64_t>(cut.span, a.T * cut.heads - from), tokens = cut.by_heads(end - 1) + 1;
     const PC piece(unit, a.D, a.turn.P);
 
     // the place of a row of this workgroup's
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(THREADS) void head_rope_kernel(HeadRopeArgs a, Cut 
     };
     const auto row_of = [&](int r) {
         Row x;
-        x.token = cut.tokens == 1 ? 0 : cut.by_heads(r);
+        x.token = cut.by_heads(r);
         x.h = r - x.token * cut.heads;
         x.kind = x.h < a.Hq ? 0 : x.h < a.Hq + a.Hk ? 1 : 2;
         x.h -= x.kind == 0 ? 0 : x.kind == 1 ? a.Hq : a.Hq + a.Hk;
@@ -376,9 +377,10 @@ __global__ __launch_bounds__(THREADS, VEC ? 4 : 1) void head_grad_kernel(HeadGra
     }
 }
 
-// Weight gradients from the partials: a workgroup takes 16 values of q's weight or of k's, 16 partials at a time.
-__global__ __launch_bounds__(THREADS) void head_grad_sum_kernel(HeadGradArgs a, int parts_q, int parts) {
-    __shared__ float s[16][17];
+// Weight gradients from the partials: a workgroup takes 16 values of q's weight or of k's, SUM_ROWS partials at a time.
+constexpr int SUM_ROWS = 64;
+__global__ __launch_bounds__(16 * SUM_ROWS) void head_grad_sum_kernel(HeadGradArgs a, int parts_q, int parts) {
+    __shared__ float s[SUM_ROWS][17];
     const int col = threadIdx.x & 15, row = threadIdx.x >> 4, d = blockIdx.x * 16 + col;
     const bool of_k = blockIdx.y;
     void* dw = of_k ? a.dwk : a.dwq;
@@ -386,15 +388,15 @@ __global__ __launch_bounds__(THREADS) void head_grad_sum_kernel(HeadGradArgs a, 
     float sum = 0.0f;
     if (d < a.D) {
 #pragma unroll 8
-        for (int p = (of_k ? parts_q : 0) + row; p < (of_k ? parts : parts_q); p += 16) sum += a.part[(int64_t)p * a.D + d];
+        for (int p = (of_k ? parts_q : 0) + row; p < (of_k ? parts : parts_q); p += SUM_ROWS) sum += a.part[(int64_t)p * a.D + d];
     }
     s[row][col] = sum;
     __syncthreads();
-    if (row == 0 && d < a.D) {
-#pragma unroll
-        for (int p = 1; p < 16; ++p) sum += s[p][col];
-        store_rt(dw, of_k ? a.dwk_dt : a.dwq_dt, d, sum);
+    for (int n = SUM_ROWS / 2; n >= 1; n >>= 1) {
+        if (row < n) s[row][col] += s[row + n][col];
+        __syncthreads();
     }
+    if (row == 0 && d < a.D) store_rt(dw, of_k ? a.dwk_dt : a.dwq_dt, d, s[0][col]);
 }
 
 // Whether rows of these views move in pieces of `bytes` (8 or 16).
@@ -479,18 +481,17 @@ hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
                aligned(a.vc.p, {a.vc.sb, a.vc.sp, a.vc.sh}, es, bytes);
     });
     Cut c = cut_of(k, a.D, a.Hq + a.Hk + (a.store ? a.Hk : 0));
-    // A small call is spread over the chip, a row a lane group; a large one takes whole tokens, so that cosines and the
-    // launch are shared by more rows.
-    const int groups = THREADS / c.lanes;
-    const int64_t rounds = a.T * c.heads / ((int64_t)groups * WORKGROUPS);
-    if (rounds < 1) {
-        c.span = std::min(groups, c.heads);
-    } else {
-        c.tokens = tokens_of(c.heads, groups, MAX_TOKENS);
-        while (c.tokens > 1 && (int64_t)c.tokens * c.heads > (int64_t)MOST_ROUNDS * groups) --c.tokens;
-        c.span = c.tokens > 1 ? c.tokens * c.heads : std::min(c.heads, MOST_ROUNDS * groups);
-    }
-    const dim3 grid((unsigned)((a.T + c.tokens - 1) / c.tokens), (unsigned)((c.tokens * c.heads + c.span - 1) / c.span));
+    // Equal runs of rows, in whole rounds of the lane groups: a small call is spread over the chip, a row a lane group; a
+    // large one over WORKGROUPS at a time, which share a token's cosines among up to 5 rounds.  Measured (us, at
+    // most 3 / 5 / 8 / 16 rounds): 4095 tokens x 56 rows into a cache 28.2 / 26.3 / 26.0 / 26.7, 4608 x 96 42.3 /
+    // 41.7 / 47.1 / 47.0, 9504 x 80 78.5 / 79.6 / 82.0 / 93.1.
+    const int64_t groups = THREADS / c.lanes, rows = a.T * c.heads, round = groups * WORKGROUPS;
+    const int64_t times = std::max<int64_t>(1, (rows + MOST_ROUNDS * round - 1) / (MOST_ROUNDS * round));
+    int64_t span = std::max<int64_t>(1, (rows + times * round - 1) / (times * round)) * groups;
+    if (span > (int64_t)(MAX_TOKENS - 1) * c.heads) span = (int64_t)(MAX_TOKENS - 1) * c.heads;
+    c.span = (int)std::min(span, rows);
+    c.tokens = (int)std::min<int64_t>(a.T, (c.span - 1) / c.heads + 2);
+    const dim3 grid((unsigned)((rows + c.span - 1) / c.span));
     const bool i = a.turn.interleaved;
     if (a.dtype == DT_F32) return i ? launch_rope<DT_F32, true>(a, k, c, grid, st) : launch_rope<DT_F32, false>(a, k, c, grid, st);
     if (a.dtype == DT_F16) return i ? launch_rope<DT_F16, true>(a, k, c, grid, st) : launch_rope<DT_F16, false>(a, k, c, grid, st);
@@ -514,7 +515,7 @@ hipError_t run_head_grad(const HeadGradArgs& a, hipStream_t st) {
     // workgroups for q's rows and for k's as their heads are, each with the same number of token blocks or one less
     const int groups = THREADS / c.lanes, most = head_grad_parts(a.T, c.heads);
     const int most_k = std::max(1, std::min<int>(most - 1, (int)((int64_t)most * a.Hk / std::max(c.heads, 1)))), most_q = most - most_k;
-    c.tokens = tokens_of(std::max(1, std::min(a.Hq, a.Hk > 0 ? a.Hk : a.Hq)), groups, (int)std::min<int64_t>(MAX_TOKENS, std::max<int64_t>(1, 2 * a.T / most)));
+    c.tokens = tokens_of(std::max(1, std::min(a.Hq, a.Hk > 0 ? a.Hk : a.Hq)), groups, (int)std::min<int64_t>(GRAD_TOKENS, std::max<int64_t>(1, 4 * a.T / most)));
     const int64_t blocks = std::max<int64_t>(1, (a.T + c.tokens - 1) / c.tokens);
     const auto even = [&](int n) { const int64_t each = (blocks + n - 1) / n; return (int)((blocks + each - 1) / each); };
     const int parts_q = even(most_q), parts = parts_q + even(most_k);
@@ -525,7 +526,7 @@ hipError_t run_head_grad(const HeadGradArgs& a, hipStream_t st) {
     else if (a.dtype == DT_F16) e = i ? launch_grad<DT_F16, true>(a, k, c, grid, parts_q, st) : launch_grad<DT_F16, false>(a, k, c, grid, parts_q, st);
     else e = i ? launch_grad<DT_BF16, true>(a, k, c, grid, parts_q, st) : launch_grad<DT_BF16, false>(a, k, c, grid, parts_q, st);
     if (e != hipSuccess || (!a.dwq && !a.dwk)) return e;
-    hipLaunchKernelGGL(head_grad_sum_kernel, dim3((unsigned)((a.D + 15) / 16), 2), dim3(THREADS), 0, st, a, parts_q, parts);
+    hipLaunchKernelGGL(head_grad_sum_kernel, dim3((unsigned)((a.D + 15) / 16), 2), dim3(16 * SUM_ROWS), 0, st, a, parts_q, parts);
     return hipGetLastError();
 }
 
