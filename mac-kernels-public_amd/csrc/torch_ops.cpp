@@ -382,6 +382,15 @@ pybind11::tuple qk_norm_rope_grad(const at::Tensor& gq, const OptTensor& gk, con
     return pybind11::make_tuple(as(dq, qt), as(dk, k), weight(da), weight(db));
 }
 
+// n values of type dt over `base`'s memory, from the `first` on (in values of dt).
+at::Tensor part_of(const at::Tensor& base, at::ScalarType dt, int64_t first, int64_t n) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(),
+                                                            c10::scalarTypeToTypeMeta(dt));
+    t.unsafeGetTensorImpl()->set_storage_offset(first);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+}
+
 pybind11::tuple paged_plan(const at::Tensor& context, const at::Tensor& added, const at::Tensor& table,
                            const at::Tensor& free_blocks, int64_t page, int64_t tokens) {
     const char* op = "paged_plan";
@@ -389,12 +398,11 @@ pybind11::tuple paged_plan(const at::Tensor& context, const at::Tensor& added, c
     all_on_device(op, {&ct, &at_, &tt, &ft});
     if (tokens < 0) fail(QLIN_EINVAL, std::string(op) + ": tokens must not be negative");
     const int64_t B = context.dim() == 1 ? context.size(0) : 0;
-    const auto i32 = context.options().dtype(at::kInt);
-    // the int32 results share one allocation
-    const at::Tensor all = at::empty({2 * tokens + 2 * B + 2}, i32), slots = at::empty({tokens}, i32.dtype(at::kLong));
-    const at::Tensor positions = all.narrow(0, 0, tokens), rows = all.narrow(0, tokens, tokens),
-                     starts = all.narrow(0, 2 * tokens, B + 1), lengths = all.narrow(0, 2 * tokens + B + 1, B),
-                     used = all.narrow(0, 2 * tokens + 2 * B + 1, 1);
+    // one allocation for all results, each a tensor of its own over a part of it: slots, then the int32 ones
+    const at::Tensor all = at::empty({tokens + (2 * tokens + 2 * B + 3) / 2}, context.options().dtype(at::kLong));
+    const auto i32 = [&](int64_t first, int64_t n) { return part_of(all, at::kInt, 2 * tokens + first, n); };
+    const at::Tensor slots = part_of(all, at::kLong, 0, tokens), positions = i32(0, tokens), rows = i32(tokens, tokens),
+                     starts = i32(2 * tokens, B + 1), lengths = i32(2 * tokens + B + 1, B), used = i32(2 * tokens + 2 * B + 1, 1);
     qlin_tensor dc = desc(context), da = desc(added), df = desc(free_blocks), dt = desc(table), ds = desc(slots),
                 dp = desc(positions), dr = desc(rows), dst = desc(starts), dl = desc(lengths), du = desc(used);
     check(qlin_paged_plan(&dc, &da, &df, page, &dt, &ds, &dp, &dr, &dst, &dl, &du, current_stream(context)));

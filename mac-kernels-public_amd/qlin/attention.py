@@ -79,14 +79,6 @@ def _flags(interleaved, inverse=False):
     return (_lib.ROPE_INTERLEAVED if interleaved else 0) | (_lib.ROPE_INVERSE if inverse else 0)
 
 
-def _fast(op, name, *args):
-    """The call through the C++ module; None when it is not built."""
-    try:
-        return getattr(ops._FAST, name)(*args)
-    except ops._FastError as e:
-        raise _fast_error(op, e) from None
-
-
 def _run(op, name, device, *args):
     """The C ABI entry point `name`; tensors (and None) become descriptors, valid for this call."""
     args = [a if isinstance(a, (int, float)) else _desc(op, a) for a in args]
@@ -100,7 +92,10 @@ def axis_rope(q, k, positions, inv_freq, axis=None, *, interleaved=False, invers
     op = "axis_rope"
     _disabled(op)
     if ops._FAST is not None:
-        return _fast(op, "axis_rope", q, k, positions, inv_freq, axis, _flags(interleaved, inverse))
+        try:
+            return ops._FAST.axis_rope(q, k, positions, inv_freq, axis, _flags(interleaved, inverse))
+        except ops._FastError as e:
+            raise _fast_error(op, e) from None
     _check_device(op, q, k, positions, inv_freq, axis)
     q3, k3 = _heads(op, q, "q"), None if k is None else _heads(op, k, "k")
     qo = torch.empty(q3.shape, dtype=q.dtype, device=q.device)
@@ -116,7 +111,10 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, axis=None, *, ep
     op = "qk_norm_rope"
     _disabled(op)
     if ops._FAST is not None:
-        return _fast(op, "qk_norm_rope", q, k, q_weight, k_weight, float(eps), positions, inv_freq, axis, _flags(interleaved))
+        try:
+            return ops._FAST.qk_norm_rope(q, k, q_weight, k_weight, float(eps), positions, inv_freq, axis, _flags(interleaved))
+        except ops._FastError as e:
+            raise _fast_error(op, e) from None
     _check_device(op, q, k, q_weight, k_weight, positions, inv_freq, axis)
     q3, k3 = _heads(op, q, "q"), None if k is None else _heads(op, k, "k")
     qo = torch.empty(q3.shape, dtype=q.dtype, device=q.device)
@@ -137,8 +135,11 @@ def qk_norm_rope_store(q, k, v, q_weight, k_weight, positions, inv_freq, slots, 
     if eps is not None and not e >= 0.0:
         raise ValueError(f"{op}: eps must not be negative")
     if ops._FAST is not None:
-        return _fast(op, "qk_norm_rope_store", q, k, v, q_weight, k_weight, e, positions, inv_freq, axis,
-                     _flags(interleaved), slots, k_cache, v_cache)
+        try:
+            return ops._FAST.qk_norm_rope_store(q, k, v, q_weight, k_weight, e, positions, inv_freq, axis, _flags(interleaved),
+                                                slots, k_cache, v_cache)
+        except ops._FastError as err:
+            raise _fast_error(op, err) from None
     _check_device(op, q, k, v, q_weight, k_weight, positions, inv_freq, axis, slots, k_cache, v_cache)
     q3 = _heads(op, q, "q")
     qo = torch.empty(q3.shape, dtype=q.dtype, device=q.device)
@@ -156,8 +157,11 @@ def qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_f
     op = "qk_norm_rope_grad"
     _disabled(op)
     if ops._FAST is not None:
-        return _fast(op, "qk_norm_rope_grad", dq_out, dk_out, q, k, q_weight, k_weight, float(eps), positions, inv_freq, axis,
-                     _flags(interleaved), bool(weight_grads))
+        try:
+            return ops._FAST.qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, float(eps), positions, inv_freq, axis,
+                                               _flags(interleaved), bool(weight_grads))
+        except ops._FastError as e:
+            raise _fast_error(op, e) from None
     _check_device(op, dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, axis)
     q3, k3 = _heads(op, q, "q"), None if k is None else _heads(op, k, "k")
     dq = torch.empty(q3.shape, dtype=q.dtype, device=q.device)
@@ -185,7 +189,10 @@ def paged_plan(context, added, block_table, free_blocks, page, tokens):
     op = "paged_plan"
     _disabled(op)
     if ops._FAST is not None:
-        return PagedPlan(*_fast(op, "paged_plan", context, added, block_table, free_blocks, int(page), int(tokens)))
+        try:
+            return PagedPlan._make(ops._FAST.paged_plan(context, added, block_table, free_blocks, int(page), int(tokens)))
+        except ops._FastError as e:
+            raise _fast_error(op, e) from None
     _check_device(op, context, added, block_table, free_blocks)
     if int(tokens) < 0:
         raise ValueError(f"{op}: tokens must not be negative")
@@ -208,7 +215,10 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, wi
     _disabled(op)
     scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
     if ops._FAST is not None:
-        return _fast(op, "paged_attention", q, k_cache, v_cache, block_table, lengths, scale, int(window), out)
+        try:
+            return ops._FAST.paged_attention(q, k_cache, v_cache, block_table, lengths, scale, int(window), out)
+        except ops._FastError as e:
+            raise _fast_error(op, e) from None
     _check_device(op, q, k_cache, v_cache, block_table, lengths, out)
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError(f"{op}: q must be [rows, heads, D] and the caches [blocks, page, kv heads, D]")
