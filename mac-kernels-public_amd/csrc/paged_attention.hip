@@ -96,6 +96,7 @@ __device__ __forceinline__ int units_of(const PagedAttentionArgs& a, int length)
 // A workgroup's run of units, [unit, end) in the running sum; the row of its first one, which starts at `first`.
 struct Share {
     int b, first, unit, end, per;
+    int length;   // up to 64 rows: lane b has row b's length
 };
 
 // Running sum over a wave, this lane's own value included.
@@ -119,7 +120,8 @@ __device__ __forceinline__ bool set_share(const Launch& p, int w, int total, Sha
 // without a barrier.
 __device__ __forceinline__ bool find_share_wave(const Launch& p, int w, Share& s) {
     const int lane = threadIdx.x & 63;
-    const int units = lane < p.a.B ? units_of(p.a, p.a.lengths[lane]) : 0;
+    s.length = lane < p.a.B ? p.a.lengths[lane] : 0;
+    const int units = lane < p.a.B ? units_of(p.a, s.length) : 0;
     const int sum = scan(units, lane);
     if (!set_share(p, w, __builtin_amdgcn_readlane(sum, 63), s)) return false;
     const uint64_t here = __ballot(s.unit < sum && s.unit >= sum - units);
@@ -325,7 +327,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
 
     const float c = a.scale * 1.4426950408889634f;  // weights are powers of two
     for (; sh.unit < sh.end; ++sh.b) {
-        const int length = ((ScalarInts)a.lengths)[sh.b];
+        const int length = a.B <= 64 ? __builtin_amdgcn_readlane(sh.length, sh.b) : ((ScalarInts)a.lengths)[sh.b];
         range_of(a, length, lo, hi);
         row = sh.b * a.ldt;
         const int units = units_of(a, length), last = min(sh.end, sh.first + units);
@@ -488,63 +490,61 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
     }
 }
 
-// out of a split row from its parts' (O, m, l).  A workgroup takes `each` heads of one row in turn: the parts'
-// weights first, a thread a part, then the parts' O over groups of D / 4 threads, JOIN of them in flight.
-constexpr int JOIN = 4;
-__global__ __launch_bounds__(THREADS) void paged_join_kernel(Launch p, int each) {
-    __shared__ f32x4 lds_o[THREADS];
-    __shared__ float lds_w[MOST_GROUPS], lds_m[WAVES], lds_l[WAVES];
+// out of a split row from its parts' (O, m, l): a workgroup a (row, head), groups of D / 4 threads over the parts, JOIN
+// parts a group in flight; the first of them are on their way while the weights are formed.  One wave where there
+// are many (row, head)s, which have few parts each, else four: the call of 64 rows x 32 heads 158 us with four waves,
+// 155 with one, that of 1 x 40 with 64 parts each 99.4 and 102.2.
+constexpr int JOIN = 8;
+template <int N>
+__global__ __launch_bounds__(N) void paged_join_kernel(Launch p) {
+    __shared__ f32x4 lds_o[N];
+    __shared__ float lds_w[MOST_GROUPS];
     const PagedAttentionArgs& a = p.a;
-    const int4 meta = p.meta[blockIdx.x];
-    if (meta.y <= 1) return;
-    const int tid = threadIdx.x, wave = tid >> 6, parts = meta.y;
-    const int quads = a.D / 4, groups = THREADS / quads, grp = tid / quads, dq = tid % quads;
-    const int G = a.H / a.Hk, hg = a.Hk * p.ng;
-    for (int head = blockIdx.y * each; head < min(a.H, (int)(blockIdx.y + 1) * each); ++head) {
-        const int kvh = head / G, in = head - kvh * G, hgi = kvh * p.ng + in / p.hpg;
-        // the row's part in share i: the share's first, but for the row that starts within its first share
-        const int64_t one = (int64_t)hg * p.hpg, from = (int64_t)hgi * p.hpg + in % p.hpg;
-        const auto place = [&](int i) { return (2 * (meta.x + i) + (i == 0 ? meta.z : 0)) * one + from; };
-        float m = -INFINITY;
-        for (int i = tid; i < parts; i += THREADS) m = fmaxf(m, p.part_ml[2 * place(i)]);
-        m = wave_max(m);
-        if ((tid & 63) == 0) lds_m[wave] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
-        const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
-        for (int i = tid; i < parts; i += THREADS) {
-            const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * place(i)] - base);
-            lds_w[i] = w;
-            l += w * p.part_ml[2 * place(i) + 1];
-        }
-        l = wave_sum(l);
-        if ((tid & 63) == 0) lds_l[wave] = l;
-        __syncthreads();
-        l = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
-        f32x4 o = {};
-        if (grp < groups) {
-            const float* part = p.part_o + 4 * dq;
-            int i = grp;
-            for (; i + (JOIN - 1) * groups < parts; i += JOIN * groups) {
-                f32x4 x[JOIN];
+    const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const int4 meta = p.meta[b];
+    const int parts = meta.y;
+    if (parts <= 1) return;
+    const int quads = a.D / 4, groups = N / quads, grp = tid / quads, dq = tid % quads;
+    const int G = a.H / a.Hk, hg = a.Hk * p.ng, kvh = head / G, in = head - kvh * G, hgi = kvh * p.ng + in / p.hpg;
+    // the row's part in share i: the share's first, but for the row that starts within its first share
+    const int64_t one = (int64_t)hg * p.hpg, from = (int64_t)hgi * p.hpg + in % p.hpg;
+    const auto place = [&](int i) { return (2 * (meta.x + i) + (i == 0 ? meta.z : 0)) * one + from; };
+    const float* part = p.part_o + 4 * dq;
+    f32x4 x[JOIN];
+    const auto fetch = [&](int i) {
 #pragma unroll
-                for (int u = 0; u < JOIN; ++u) x[u] = *reinterpret_cast<const f32x4*>(part + place(i + u * groups) * a.D);
+        for (int u = 0; u < JOIN; ++u) {
+            x[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (grp < groups && i + u * groups < parts) x[u] = *reinterpret_cast<const f32x4*>(part + place(i + u * groups) * a.D);
+        }
+    };
+    fetch(grp);
+    float m = -INFINITY, l = 0.0f;  // every wave forms them for itself
+    for (int i = lane; i < parts; i += 64) m = fmaxf(m, p.part_ml[2 * place(i)]);
+    m = wave_max(m);
+    const float base = m == -INFINITY ? 0.0f : m;
+    for (int i = lane; i < parts; i += 64) {
+        const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * place(i)] - base);
+        if (tid < 64) lds_w[i] = w;
+        l += w * p.part_ml[2 * place(i) + 1];
+    }
+    l = wave_sum(l);
+    __syncthreads();
+    f32x4 o = {};
+    for (int i = grp; i < parts; i += JOIN * groups) {
+        if (i != grp) fetch(i);
 #pragma unroll
-                for (int u = 0; u < JOIN; ++u) o += x[u] * lds_w[i + u * groups];
-            }
-            for (; i < parts; i += groups) o += *reinterpret_cast<const f32x4*>(part + place(i) * a.D) * lds_w[i];
-        }
-        lds_o[tid] = o;
-        __syncthreads();
-        if (tid < quads) {
-            for (int i = 1; i < groups; ++i) o += lds_o[i * quads + tid];
-            const float inv = 1.0f / l;
-            const float v[4] = {l == 0.0f ? 0.0f : o[0] * inv, l == 0.0f ? 0.0f : o[1] * inv, l == 0.0f ? 0.0f : o[2] * inv,
-                                l == 0.0f ? 0.0f : o[3] * inv};
-            store4_rt(a.out.p, a.dtype, blockIdx.x * a.out.st + head * a.out.sh + 4 * tid, v, 4, true);
-        }
-        __syncthreads();
+        for (int u = 0; u < JOIN; ++u)
+            if (i + u * groups < parts) o += x[u] * lds_w[i + u * groups];
+    }
+    lds_o[tid] = o;
+    __syncthreads();
+    if (tid < quads) {
+        for (int i = 1; i < groups; ++i) o += lds_o[i * quads + tid];
+        const float inv = 1.0f / l;
+        const float v[4] = {l == 0.0f ? 0.0f : o[0] * inv, l == 0.0f ? 0.0f : o[1] * inv, l == 0.0f ? 0.0f : o[2] * inv,
+                            l == 0.0f ? 0.0f : o[3] * inv};
+        store4_rt(a.out.p, a.dtype, b * a.out.st + head * a.out.sh + 4 * tid, v, 4, true);
     }
 }
 
@@ -619,9 +619,9 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
         hipError_t e = a.dtype == DT_F16 ? launch_dim<DT_F16>(p, p16, grid, st) : launch_dim<DT_BF16>(p, p16, grid, st);
         if (e != hipSuccess) return e;
         if (p.join) {
-            const int each = (int)std::max<int64_t>(1, std::min<int64_t>(a.H, p.a.B * a.H / 1024));
-            hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)p.a.B, (unsigned)((a.H + each - 1) / each)), dim3(THREADS), 0, st,
-                               p, each);
+            const dim3 each((unsigned)p.a.B, (unsigned)a.H);
+            if (p.a.B * a.H > 2 * CUS) hipLaunchKernelGGL(paged_join_kernel<64>, each, dim3(64), 0, st, p);
+            else hipLaunchKernelGGL(paged_join_kernel<256>, each, dim3(256), 0, st, p);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
     }
