@@ -14,7 +14,7 @@ namespace qlin {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int MAX_TOKENS = 64;        // tokens that a workgroup's rows belong to, at most
+constexpr int MAX_TOKENS = 64;        // tokens that a workgroup's rows belong to, at most: see most_tokens()
 constexpr int WORKGROUPS = 2048;      // that a call is spread over, once or several times
 constexpr int GRAD_WORKGROUPS = 1024; // of head_grad_kernel that the chip holds at once
 constexpr int MOST_ROUNDS = 5;        // rows of one lane group, at most
@@ -421,6 +421,9 @@ Kind kind_of(int D, const RopeTurn& turn, int dtype, const ALIGNED& all_aligned)
     return {8, false};
 }
 
+// Tokens whose cosines and sines a workgroup holds in LDS, at most: 32 KB of them, or two tokens.
+int64_t most_tokens(int64_t D) { return std::max<int64_t>(2, std::min<int64_t>(MAX_TOKENS, 8192 / (D + 15))); }
+
 Cut cut_of(const Kind& k, int D, int heads) {
     Cut c;
     const int units = (D + 2 * k.VW - 1) / (2 * k.VW);
@@ -488,7 +491,7 @@ hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
     const int64_t groups = THREADS / c.lanes, rows = a.T * c.heads, round = groups * WORKGROUPS;
     const int64_t times = std::max<int64_t>(1, (rows + MOST_ROUNDS * round - 1) / (MOST_ROUNDS * round));
     int64_t span = std::max<int64_t>(1, (rows + times * round - 1) / (times * round)) * groups;
-    if (span > (int64_t)(MAX_TOKENS - 1) * c.heads) span = (int64_t)(MAX_TOKENS - 1) * c.heads;
+    span = std::min(span, (most_tokens(a.D) - 1) * c.heads);
     c.span = (int)std::min(span, rows);
     c.tokens = (int)std::min<int64_t>(a.T, (c.span - 1) / c.heads + 2);
     const dim3 grid((unsigned)((rows + c.span - 1) / c.span));

@@ -100,6 +100,7 @@ SHAPES = [
     (3, 1, 2, 510, (254, 256), True),
     (301, 20, 4, 64, (64,), False),
     (2, 24, 24, 128, (0, 128), True),     # an axis that turns nothing
+    (9000, 1, 2, 16, (16,), True),        # many tokens of few short heads
 ]
 
 
@@ -147,6 +148,27 @@ def test_positions(pdtype, start):
     y2, _ = Q.axis_rope(q.to(DEV), None, wide.to(DEV)[:, ::3], freq.to(DEV), axis.to(DEV))
     y1, _ = Q.axis_rope(q.to(DEV), None, pos.to(DEV), freq.to(DEV), axis.to(DEV))
     assert torch.equal(y1, y2)
+
+
+@pytest.mark.parametrize("t,d", [(70000, 512), (200000, 128)])
+def test_many_tokens_of_one_head(t, d):
+    """A workgroup's rows are of as many tokens as its LDS holds cosines of (the bounds of test_rotation_and_norms, in float64
+    on the GPU)."""
+    Q = qlin()
+    freq, _ = Q.rope_frequencies(d, device=DEV)
+    pos = torch.arange(t, device=DEV)
+    q = torch.randn(t, 1, d, generator=torch.Generator(DEV).manual_seed(1), device=DEV, dtype=F32).half()
+    y, _ = Q.axis_rope(q, None, pos, freq)
+    dq, _, _, _ = Q.qk_norm_rope_grad(q, None, q, None, None, None, pos, freq)
+    ang = (pos.double()[:, None] * freq.double())[:, None]
+    x = q.double()
+    assert bool(((y.double() - rotate(x, ang, False)).abs() <= 2.0 ** -11 * rotate(x, ang, False).abs()
+                 + 2.0 ** -18 * lengths_of_pairs(x, d // 2, False) + TINY[F16]).all())
+    rstd = (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    g, unit, size = rotate(x, -ang, False), x * rstd, lengths_of_pairs(x, d // 2, False)
+    want = rstd * (g - unit * (g * unit).mean(-1, keepdim=True))
+    tol = 2.0 ** -11 * want.abs() + 2.0 ** -17 * rstd * (size + unit.abs() * (size * unit.abs()).mean(-1, keepdim=True)) + TINY[F16]
+    assert bool(((dq.double() - want).abs() <= tol).all())
 
 
 def test_axis_entries_outside_count_as_the_nearest():
