@@ -18,7 +18,13 @@
 // workgroup takes an equal run of them, as many workgroups as the chip holds at once.  So one long row among short ones
 // is spread like the rest, and the host need not know the lengths: every workgroup forms the running sum from them.
 // A row that crosses from one workgroup's run into the next leaves its parts as (O, m, l) in fp32, and a second
-// kernel joins them.
+// kernel joins them.  Where the table has no room for long rows, a workgroup takes one row (whole_rows()).
+//
+// Measured on one MI355X (calls back to back, bytes of the cache over the whole call): 1 row of 131071 tokens, 40 heads
+// over 8 of 128 values 99 us, 5.4 TB/s; 64 rows of 100 to 16384, 32 over 8 155 us, 5.5 TB/s; 8 rows of 3000 to 4096 31.5 us,
+// 3.7 TB/s, of which the first loads take some 5 us and the second kernel with its launch 6; 1 row of 77 6.9 us.  Tried
+// and slower: more workgroups than the chip holds, a join by the last workgroup (its agent fences write back and drop
+// the L2: 105 us for the 8 rows), 3 waves a SIMD (spills), the next row's loads before this row's join.
 #include "attention.h"
 
 namespace qlin {
@@ -35,6 +41,15 @@ constexpr int MOST_GROUPS = 4 * CUS;  // of any head size: see held()
 // Workgroups of the kernel for this head size that the chip holds at once (registers: 4, 2 and 1 on a compute unit).
 int64_t held(int64_t D) { return CUS * (D <= 64 ? 4 : D <= 128 ? 2 : 1); }
 
+// Units up to which rows are not split: a workgroup takes one whole row, without the running sum and the second kernel.
+// Where that fills the chip rows may be longer.  Measured, not split / split (us, 8 kv heads; 1 unit = 128 tokens):
+// D = 128, 1 row of 4 units 10.3 / 11.4, of 8 15.4 / 11.5; 64 rows of 4 21.5 / 28.7, of 8 41.7 / 47.6, of 16 77.9 / 80.5;
+// D = 64, 8 rows of 4 8.1 / 12.0, of 8 13.8 / 13.3; 64 rows of 16 45.2 / 52.4; D = 256, 8 rows of 2 11.6 / 14.8, of 4
+// 16.8 / 15.6; 64 rows of 8 73.5 / 75.5, of 16 135 / 131.
+int64_t whole_rows(int64_t D, int64_t workgroups) {
+    return workgroups >= 2 * CUS ? std::min<int64_t>(16, 2048 / D) : D <= 128 ? 4 : 2;
+}
+
 struct Launch {
     PagedAttentionArgs a;
     int ng;                 // head groups of a kv head
@@ -44,7 +59,7 @@ struct Launch {
     float* part_o;          // [share, first or last row][kv head, group][head][D]
     float* part_ml;         // [share, first or last row][kv head, group][head][2]
     int4* meta;             // [rows]: the first share, shares, whether the row is not the first of its first share
-    bool join;
+    bool split;             // shares of equal runs, joined; else a workgroup takes one row
 };
 
 // What no kernel writes while this one runs is read through the scalar cache: its loads do not queue with
@@ -207,7 +222,11 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
     const int n = lane & 15, g = lane >> 4;  // column (a head) and row group
     const int hg = a.Hk * p.ng, hgi = blockIdx.x % hg, share = blockIdx.x / hg;
     Share sh;
-    if (a.B <= 64 ? !find_share_wave(p, share, sh) : !find_share(p, share, sh)) return;
+    if (!p.split) {
+        sh = Share{share, 0, 0, 1, 1, 0};
+    } else if (a.B <= 64 ? !find_share_wave(p, share, sh) : !find_share(p, share, sh)) {
+        return;
+    }
     const int kvh = hgi / p.ng, G = a.H / a.Hk, h0 = (hgi % p.ng) * p.hpg, heads = min(p.hpg, G - h0);
     const uint16_t* kbase = (const uint16_t*)a.kc.p + kvh * a.kc.sh;
     const uint16_t* vbase = (const uint16_t*)a.vc.p + kvh * a.vc.sh;
@@ -327,14 +346,14 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
 
     const float c = a.scale * 1.4426950408889634f;  // weights are powers of two
     for (; sh.unit < sh.end; ++sh.b) {
-        const int length = a.B <= 64 ? __builtin_amdgcn_readlane(sh.length, sh.b) : ((ScalarInts)a.lengths)[sh.b];
+        const int length = p.split && a.B <= 64 ? __builtin_amdgcn_readlane(sh.length, sh.b) : ((ScalarInts)a.lengths)[sh.b];
         range_of(a, length, lo, hi);
         row = sh.b * a.ldt;
-        const int units = units_of(a, length), last = min(sh.end, sh.first + units);
+        const int units = p.split ? units_of(a, length) : 1, last = min(sh.end, sh.first + units);
         const int start = (lo & ~(TILE - 1)) + (sh.unit - sh.first) * UNIT;
-        const int end = (int)min((int64_t)start + (int64_t)(last - sh.unit) * UNIT, (int64_t)hi);
+        const int end = p.split ? (int)min((int64_t)start + (int64_t)(last - sh.unit) * UNIT, (int64_t)hi) : hi;
         const int share0 = sh.first / sh.per, shares = (sh.first + units - 1) / sh.per - share0 + 1;
-        if (p.join && hgi == 0 && sh.unit == sh.first && threadIdx.x == 0)
+        if (p.split && hgi == 0 && sh.unit == sh.first && threadIdx.x == 0)
             p.meta[sh.b] = make_int4(share0, shares, sh.first != share0 * sh.per, 0);
 
         // Q^T: column n is a head; up to 8 heads the columns 8 .. 15 repeat them for the weights' second part
@@ -601,7 +620,7 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
     p.part_ml = (float*)(ws + META_BYTES);
     p.part_o = (float*)(ws + META_BYTES + (heads * 8 + 255) / 256 * 256);
     int64_t W = a.blocks == 0 ? 0 : std::min<int64_t>(a.W, 0x7FFFFF00 / a.page);  // positions stay 32-bit
-    // units a row can have at most: rows that cannot be split need no second kernel
+    // units a row can have at most
     int64_t most = (W * a.page + UNIT - 1) / UNIT;
     if (a.window) most = std::min<int64_t>(most, a.window / UNIT + 2);
     most = std::max<int64_t>(most, 1);
@@ -614,11 +633,11 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
         p.a.out.p = (uint16_t*)a.out.p + b0 * a.out.st;
         p.a.table = a.table + b0 * a.ldt;
         p.a.lengths = a.lengths + b0;
-        p.join = most > 1;
-        const unsigned grid = (unsigned)(std::min<int64_t>(p.shares, most * p.a.B) * hg);
+        p.split = most > whole_rows(a.D, p.a.B * hg);
+        const unsigned grid = (unsigned)((p.split ? std::min<int64_t>(p.shares, most * p.a.B) : p.a.B) * hg);
         hipError_t e = a.dtype == DT_F16 ? launch_dim<DT_F16>(p, p16, grid, st) : launch_dim<DT_BF16>(p, p16, grid, st);
         if (e != hipSuccess) return e;
-        if (p.join) {
+        if (p.split) {
             const dim3 each((unsigned)p.a.B, (unsigned)a.H);
             if (p.a.B * a.H > 2 * CUS) hipLaunchKernelGGL(paged_join_kernel<64>, each, dim3(64), 0, st, p);
             else hipLaunchKernelGGL(paged_join_kernel<256>, each, dim3(256), 0, st, p);

@@ -119,6 +119,16 @@ def test_pages_before_the_window_are_not_used():
     assert torch.equal(want, qlin().paged_attention(q, k, v, table, lengths, window=100))
 
 
+@pytest.mark.parametrize("width", [16, 17, 32, 33, 70, 128, 129, 300])
+@pytest.mark.parametrize("rows", [1, 5, 70, 300])
+def test_whole_rows_and_split_ones(rows, width):
+    """Tables with room for rows that one workgroup takes and for rows that are split, whatever the lengths are."""
+    lengths = [(i * 137) % (width * 16) for i in range(rows)]
+    lengths[0] = width * 16 - 3
+    s = make(lengths, 4, 2, 64, 16, F16, width=width)
+    check(qlin().paged_attention(*s), *s)
+
+
 @pytest.mark.parametrize("rows", [1, 65, 1030])
 def test_many_rows(rows):
     lengths = [(i * 37) % 90 for i in range(rows)]
