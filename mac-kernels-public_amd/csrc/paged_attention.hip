@@ -50,6 +50,14 @@ int64_t whole_rows(int64_t D, int64_t workgroups) {
     return workgroups >= 2 * CUS ? std::min<int64_t>(16, 2048 / D) : D <= 128 ? 4 : 2;
 }
 
+// Whether whole rows of at most `longest` tokens take a wave each instead of a workgroup of four: many rows that leave some
+// of four waves without a tile.  Measured, one wave / four (us, 8 kv heads of 128 values): 200 rows of 30 tokens 8.8 / 18.8,
+// of 60 11.7 / 19.5, of 120 16.9 / 22.6, of 250 34.4 / 41.4, of 500 63.8 / 64.8; 64 rows of 60 7.8 / 8.2, of 120 10.3 / 9.8,
+// of 250 15.4 / 13.0; of 256 values, 64 rows of 120 16.3 / 18.2, of 250 27.2 / 26.6.
+bool one_wave_rows(int64_t D, int64_t longest, int64_t workgroups) {
+    return longest <= 512 && 2 * workgroups >= held(D) * (longest <= 64 ? 2 : longest <= 128 ? 3 : 6);
+}
+
 struct Launch {
     PagedAttentionArgs a;
     int ng;                 // head groups of a kv head
@@ -207,25 +215,29 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
 
 // DP: the head size's room (64, 128, 256).  P16: pages of whole 16-token tiles, so that a tile's base address is
 // uniform; else every token's address is looked up by itself.  WIDE: 9 to 16 heads.
-template <int DT, int DP, bool P16, bool WIDE>
-__global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_kernel(Launch p) {
+// W: waves of a workgroup, 4, or 1 for many short rows (not split).
+template <int DT, int DP, bool P16, bool WIDE, int W>
+__global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_kernel(Launch p) {
+    static_assert(W == WAVES || W == 1, "rows are split in units of 4 waves' tiles");
+    constexpr int STEP = W * TILE;
+    const bool split = W == WAVES && p.split;
     constexpr int KS = DP / 32;              // 32-value steps of a score
     constexpr int EPL = DP / 16;             // values of a V row that a lane holds
     constexpr int VL = EPL > 8 ? 2 : 1;      // loads they take
     using VT = typename std::conditional<EPL == 4, u32x2, u32x4>::type;
     constexpr int OS = DP + 4;               // row stride of the join in LDS
     constexpr int OH = WIDE ? 16 : 8;
-    __shared__ float lds_o[WAVES][OH][OS];
-    __shared__ float lds_m[WAVES][16], lds_l[WAVES][16];
+    __shared__ float lds_o[W][OH][OS];
+    __shared__ float lds_m[W][16], lds_l[W][16];
     const PagedAttentionArgs& a = p.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;  // column (a head) and row group
     const int hg = a.Hk * p.ng, hgi = blockIdx.x % hg, share = blockIdx.x / hg;
     Share sh;
-    if (!p.split) {
+    if (!split) {
         sh = Share{share, 0, 0, 1, 1, 0};
-    } else if (a.B <= 64 ? !find_share_wave(p, share, sh) : !find_share(p, share, sh)) {
-        return;
+    } else if constexpr (W == WAVES) {
+        if (a.B <= 64 ? !find_share_wave(p, share, sh) : !find_share(p, share, sh)) return;
     }
     const int kvh = hgi / p.ng, G = a.H / a.Hk, h0 = (hgi % p.ng) * p.hpg, heads = min(p.hpg, G - h0);
     const uint16_t* kbase = (const uint16_t*)a.kc.p + kvh * a.kc.sh;
@@ -346,14 +358,14 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
 
     const float c = a.scale * 1.4426950408889634f;  // weights are powers of two
     for (; sh.unit < sh.end; ++sh.b) {
-        const int length = p.split && a.B <= 64 ? __builtin_amdgcn_readlane(sh.length, sh.b) : ((ScalarInts)a.lengths)[sh.b];
+        const int length = split && a.B <= 64 ? __builtin_amdgcn_readlane(sh.length, sh.b) : ((ScalarInts)a.lengths)[sh.b];
         range_of(a, length, lo, hi);
         row = sh.b * a.ldt;
-        const int units = p.split ? units_of(a, length) : 1, last = min(sh.end, sh.first + units);
+        const int units = split ? units_of(a, length) : 1, last = min(sh.end, sh.first + units);
         const int start = (lo & ~(TILE - 1)) + (sh.unit - sh.first) * UNIT;
-        const int end = p.split ? (int)min((int64_t)start + (int64_t)(last - sh.unit) * UNIT, (int64_t)hi) : hi;
+        const int end = split ? (int)min((int64_t)start + (int64_t)(last - sh.unit) * UNIT, (int64_t)hi) : hi;
         const int share0 = sh.first / sh.per, shares = (sh.first + units - 1) / sh.per - share0 + 1;
-        if (p.split && hgi == 0 && sh.unit == sh.first && threadIdx.x == 0)
+        if (split && hgi == 0 && sh.unit == sh.first && threadIdx.x == 0)
             p.meta[sh.b] = make_int4(share0, shares, sh.first != share0 * sh.per, 0);
 
         // Q^T: column n is a head; up to 8 heads the columns 8 .. 15 repeat them for the weights' second part
@@ -371,7 +383,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
         int t = start + wave * TILE;
         if (t < end) {
             Tile x = locate(t, entries(t));
-            Entries ahead = entries(t + UNIT);
+            Entries ahead = entries(t + STEP);
             load_k(x);
             load_v(x);
             while (true) {
@@ -381,12 +393,12 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
                     s0 = Mma<DT>::mul(kr[0][j], q[j], s0);
                     s1 = Mma<DT>::mul(kr[1][j], q[j], s1);
                 }
-                const int tn = t + UNIT;
+                const int tn = t + STEP;
                 const bool more = tn < end;
                 Tile y = x;
                 if (more) {
                     y = locate(tn, ahead);
-                    ahead = entries(tn + UNIT);
+                    ahead = entries(tn + STEP);
                     load_k(y);
                 }
                 float s[8];
@@ -472,16 +484,16 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void paged_attention_ke
         }
         __syncthreads();
         const int quads = a.D / 4;
-        for (int idx = threadIdx.x; idx < heads * quads; idx += THREADS) {
+        for (int idx = threadIdx.x; idx < heads * quads; idx += 64 * W) {
             const int h = idx / quads, d = (idx - h * quads) * 4;
             float mm = lds_m[0][h];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, lds_m[w][h]);
+            for (int w = 1; w < W; ++w) mm = fmaxf(mm, lds_m[w][h]);
             const float base = mm == -INFINITY ? 0.0f : mm;
             float ll = 0.0f;
             f32x4 o = {};
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float f = __builtin_amdgcn_exp2f(lds_m[w][h] - base);
                 ll += lds_l[w][h] * f;
                 o += *reinterpret_cast<const f32x4*>(&lds_o[w][h][d]) * f;
@@ -575,21 +587,23 @@ void head_groups(int64_t G, int& ng, int& hpg) {
 int64_t shares_of(int64_t hg, int64_t D) { return std::max<int64_t>(1, held(D) / hg); }
 
 template <int DT, int DP>
-hipError_t launch(const Launch& p, bool p16, unsigned grid, hipStream_t st) {
+hipError_t launch(const Launch& p, bool p16, bool one_wave, unsigned grid, hipStream_t st) {
     const bool wide = p.hpg > 8;
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(THREADS), 0, st, p); };
-    if (p16 && wide) go(paged_attention_kernel<DT, DP, true, true>);
-    else if (p16) go(paged_attention_kernel<DT, DP, true, false>);
-    else if (wide) go(paged_attention_kernel<DT, DP, false, true>);
-    else go(paged_attention_kernel<DT, DP, false, false>);
+    auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, p); };
+    if (one_wave && wide) go(paged_attention_kernel<DT, DP, true, true, 1>, 64);
+    else if (one_wave) go(paged_attention_kernel<DT, DP, true, false, 1>, 64);
+    else if (p16 && wide) go(paged_attention_kernel<DT, DP, true, true, WAVES>, THREADS);
+    else if (p16) go(paged_attention_kernel<DT, DP, true, false, WAVES>, THREADS);
+    else if (wide) go(paged_attention_kernel<DT, DP, false, true, WAVES>, THREADS);
+    else go(paged_attention_kernel<DT, DP, false, false, WAVES>, THREADS);
     return hipGetLastError();
 }
 
 template <int DT>
-hipError_t launch_dim(const Launch& p, bool p16, unsigned grid, hipStream_t st) {
-    if (p.a.D <= 64) return launch<DT, 64>(p, p16, grid, st);
-    if (p.a.D <= 128) return launch<DT, 128>(p, p16, grid, st);
-    return launch<DT, 256>(p, p16, grid, st);
+hipError_t launch_dim(const Launch& p, bool p16, bool one_wave, unsigned grid, hipStream_t st) {
+    if (p.a.D <= 64) return launch<DT, 64>(p, p16, one_wave, grid, st);
+    if (p.a.D <= 128) return launch<DT, 128>(p, p16, one_wave, grid, st);
+    return launch<DT, 256>(p, p16, one_wave, grid, st);
 }
 
 constexpr size_t META_BYTES = MAX_ROWS * sizeof(int4);
@@ -624,6 +638,7 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
     int64_t most = (W * a.page + UNIT - 1) / UNIT;
     if (a.window) most = std::min<int64_t>(most, a.window / UNIT + 2);
     most = std::max<int64_t>(most, 1);
+    const int64_t longest = a.window ? std::min<int64_t>(W * a.page, a.window + TILE) : W * a.page;
     const int64_t rows = std::min<int64_t>(MAX_ROWS, (1 << 30) / most);  // sums of units stay 32-bit
     for (int64_t b0 = 0; b0 < a.B; b0 += rows) {
         p.a = a;
@@ -635,7 +650,8 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
         p.a.lengths = a.lengths + b0;
         p.split = most > whole_rows(a.D, p.a.B * hg);
         const unsigned grid = (unsigned)((p.split ? std::min<int64_t>(p.shares, most * p.a.B) : p.a.B) * hg);
-        hipError_t e = a.dtype == DT_F16 ? launch_dim<DT_F16>(p, p16, grid, st) : launch_dim<DT_BF16>(p, p16, grid, st);
+        const bool one_wave = p16 && !p.split && one_wave_rows(a.D, longest, p.a.B * hg);
+        hipError_t e = a.dtype == DT_F16 ? launch_dim<DT_F16>(p, p16, one_wave, grid, st) : launch_dim<DT_BF16>(p, p16, one_wave, grid, st);
         if (e != hipSuccess) return e;
         if (p.split) {
             const dim3 each((unsigned)p.a.B, (unsigned)a.H);

@@ -129,6 +129,19 @@ def test_whole_rows_and_split_ones(rows, width):
     check(qlin().paged_attention(*s), *s)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,longest", [
+    (300, 8, 8, 128, 20), (150, 32, 8, 128, 100), (400, 8, 8, 64, 130), (220, 48, 4, 96, 64), (200, 8, 4, 256, 33),
+    (230, 16, 8, 72, 500),
+])
+def test_many_short_rows(rows, heads, kv_heads, dim, longest, dtype):
+    """So many that a wave takes each, empty ones among them; the last in a window too."""
+    lengths = [(i * 53) % (longest + 1) for i in range(rows)]
+    s = make(lengths, heads, kv_heads, dim, 16, dtype)
+    check(qlin().paged_attention(*s), *s)
+    check(qlin().paged_attention(*s, window=19), *s, window=19)
+
+
 @pytest.mark.parametrize("rows", [1, 65, 1030])
 def test_many_rows(rows):
     lengths = [(i * 37) % 90 for i in range(rows)]
