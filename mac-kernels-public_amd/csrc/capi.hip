@@ -417,6 +417,16 @@ qlin_status qlin_query(int op, int64_t M, int64_t N, int64_t K, int param, int x
             if (K > QLIN_MAX_K_WO) return fail(QLIN_EUNSUPPORTED, "K > %d", QLIN_MAX_K_WO);
             return QLIN_OK;
         }
+        case QLIN_OP_QK_NORM_ROPE_GRAD:  // N: the heads of q and of k together
+            if (x_dtype != out_dtype) return fail(QLIN_EUNSUPPORTED, "the gradients have the inputs' dtype");
+            if (K > ROPE_MAX_DIM) return fail(QLIN_EUNSUPPORTED, "heads of %lld values, more than %d", (long long)K, ROPE_MAX_DIM);
+            if (N > 2 * ROPE_MAX_HEADS) return fail(QLIN_EUNSUPPORTED, "more than %d heads", ROPE_MAX_HEADS);
+            return QLIN_OK;
+        case QLIN_OP_PAGED_ATTENTION:
+            if (x_dtype != out_dtype || x_dtype == QLIN_DT_F32) return fail(QLIN_EUNSUPPORTED, "f16 or bf16, in and out");
+            if (K < 8 || K > PAGED_MAX_DIM || K % 8) return fail(QLIN_EUNSUPPORTED, "heads of %lld values", (long long)K);
+            if (param < 1 || N % param || N > 65535) return fail(QLIN_EUNSUPPORTED, "%lld heads over %d", (long long)N, param);
+            return QLIN_OK;
     }
     return fail(QLIN_EUNSUPPORTED, "unknown op %d", op);
 }

@@ -195,6 +195,20 @@ def test_python_entry_points_refuse():
         ops._FAST = fast
 
 
+def test_query_and_workspace():
+    L, lb = lib()
+    query = lambda op, n, k, param, a=L.DT_F16, b=L.DT_F16: lb.qlin_query(op, 4, n, k, param, a, b)
+    assert query(L.OP_PAGED_ATTENTION, 32, 128, 8) == 0 and query(L.OP_PAGED_ATTENTION, 32, 128, 8, L.DT_BF16, L.DT_BF16) == 0
+    for bad in ((32, 132, 8), (32, 264, 8), (32, 128, 5), (32, 128, 0), (32, 128, 8, L.DT_F32, L.DT_F32), (32, 128, 8, L.DT_F16, L.DT_BF16)):
+        assert query(L.OP_PAGED_ATTENTION, *bad) == 1
+    assert query(L.OP_QK_NORM_ROPE_GRAD, 96, 128, 0) == 0 and query(L.OP_QK_NORM_ROPE_GRAD, 96, 513, 0) == 1
+    size = lambda op, m, n, k, param: lb.qlin_workspace_size(op, m, n, k, param, L.DT_F16)
+    # two parts of a split row a workgroup: 2 x 512 workgroups x 4 heads x (128 values, maximum and sum)
+    assert size(L.OP_PAGED_ATTENTION, 8, 32, 128, 8) >= 2 * 512 * 4 * 130 * 4
+    assert size(L.OP_PAGED_ATTENTION, 8, 32, 128, 0) == 0
+    assert size(L.OP_QK_NORM_ROPE_GRAD, 1056, 96, 128, 0) <= 1024 * 128 * 4
+
+
 def test_frequencies():
     import qlin
     f, a = qlin.rope_frequencies((16, 56, 56), 1e4)
