@@ -101,13 +101,28 @@ struct Piece {
         *reinterpret_cast<V*>(x) = *reinterpret_cast<const V*>(table + pair);
         *reinterpret_cast<V*>(x + VW / 2) = *reinterpret_cast<const V*>(table + (VEC && INTER ? pair2 : pair + VW / 2));
     }
+    // Nontemporal: a row is read once, and what it would take of the caches is left to the outputs, which the next kernel
+    // reads.  Measured with a kernel that writes the rows before and one that reads the outputs after (us, all three): 4608
+    // tokens x 96 heads 137 against 150, 9504 x 80 234 against 245, 4095 x 48 58 against 58; the gradient 145 against
+    // 159 and 244 against 264.  Nontemporal stores: 139, 245, 63; 156 and 264.
+    static __device__ __forceinline__ Vector vector_at(const T* p) {
+        typedef uint32_t Words __attribute__((ext_vector_type(sizeof(Vector) % 16 ? 2 : 4)));
+        if constexpr (sizeof(Vector) == sizeof(Words)) {
+            return __builtin_bit_cast(Vector, __builtin_nontemporal_load(reinterpret_cast<const Words*>(p)));
+        } else {
+            struct Two { Words a, b; };
+            static_assert(sizeof(Vector) == sizeof(Two), "8 fp32 values");
+            const Words* q = reinterpret_cast<const Words*>(p);
+            return __builtin_bit_cast(Vector, Two{__builtin_nontemporal_load(q), __builtin_nontemporal_load(q + 1)});
+        }
+    }
     struct Raw { Vector a, b; };
     __device__ __forceinline__ Raw load(const T* row, bool wanted) const {
         Raw r = {};
         if constexpr (VEC) {
             if (wanted && inside) {
-                r.a = *reinterpret_cast<const Vector*>(row + first);
-                r.b = *reinterpret_cast<const Vector*>(row + second);
+                r.a = vector_at(row + first);
+                r.b = vector_at(row + second);
             }
         } else {
 #pragma unroll
