@@ -21,10 +21,11 @@
 // kernel joins them.  Where the table has no room for long rows, a workgroup takes one row (whole_rows()).
 //
 // Measured on one MI355X (calls back to back, bytes of the cache over the whole call): 1 row of 131071 tokens, 40 heads
-// over 8 of 128 values 99 us, 5.4 TB/s; 64 rows of 100 to 16384, 32 over 8 155 us, 5.5 TB/s; 8 rows of 3000 to 4096 31.5 us,
-// 3.7 TB/s, of which the first loads take some 5 us and the second kernel with its launch 6; 1 row of 77 6.9 us.  Tried
+// over 8 of 128 values 90 us, 6.0 TB/s; 64 rows of 100 to 16384, 32 over 8 142 us, 6.1 TB/s; 8 rows of 3000 to 4096 28.7 us,
+// 4.0 TB/s, of which the first loads take some 5 us and the second kernel with its launch 6; 1 row of 77 6.3 us.  Tried
 // and slower: more workgroups than the chip holds, a join by the last workgroup (its agent fences write back and drop
-// the L2: 105 us for the 8 rows), 3 waves a SIMD (spills), the next row's loads before this row's join.
+// the L2: 105 us for the 8 rows), 3 waves a SIMD (spills), the next row's loads before this row's join, loads without
+// branches around them (the waits are exact then; 3% faster for 64 values, 2 to 5% slower for 128).
 #include "attention.h"
 
 namespace qlin {
@@ -43,17 +44,17 @@ int64_t held(int64_t D) { return CUS * (D <= 64 ? 4 : D <= 128 ? 2 : 1); }
 
 // Units up to which rows are not split: a workgroup takes one whole row, without the running sum and the second kernel.
 // Where that fills the chip rows may be longer.  Measured, not split / split (us, 8 kv heads; 1 unit = 128 tokens):
-// D = 128, 1 row of 4 units 10.3 / 11.4, of 8 15.4 / 11.5; 64 rows of 4 21.5 / 28.7, of 8 41.7 / 47.6, of 16 77.9 / 80.5;
-// D = 64, 8 rows of 4 8.1 / 12.0, of 8 13.8 / 13.3; 64 rows of 16 45.2 / 52.4; D = 256, 8 rows of 2 11.6 / 14.8, of 4
-// 16.8 / 15.6; 64 rows of 8 73.5 / 75.5, of 16 135 / 131.
+// D = 128, 1 row of 4 units 10.5 / 12.9, of 8 15.5 / 12.4; 64 rows of 4 21.4 / 27.0, of 8 39.5 / 44.7, of 16 73.6 / 75.0;
+// D = 64, 8 rows of 4 10.1 / 12.4, of 8 15.8 / 13.2; 64 rows of 16 43.3 / 48.7; D = 256, 8 rows of 2 11.9 / 15.1, of 4
+// 18.2 / 16.3; 64 rows of 8 71.0 / 72.2, of 16 128 / 123.
 int64_t whole_rows(int64_t D, int64_t workgroups) {
     return workgroups >= 2 * CUS ? std::min<int64_t>(16, 2048 / D) : D <= 128 ? 4 : 2;
 }
 
 // Whether whole rows of at most `longest` tokens take a wave each instead of a workgroup of four: many rows that leave some
-// of four waves without a tile.  Measured, one wave / four (us, 8 kv heads of 128 values): 200 rows of 30 tokens 8.8 / 18.8,
-// of 60 11.7 / 19.5, of 120 16.9 / 22.6, of 250 34.4 / 41.4, of 500 63.8 / 64.8; 64 rows of 60 7.8 / 8.2, of 120 10.3 / 9.8,
-// of 250 15.4 / 13.0; of 256 values, 64 rows of 120 16.3 / 18.2, of 250 27.2 / 26.6.
+// of four waves without a tile.  Measured, one wave / four (us, 8 kv heads of 128 values): 200 rows of 30 tokens 8.9 / 19.1,
+// of 60 12.1 / 19.8, of 120 17.7 / 23.1, of 250 31.2 / 38.2, of 500 59.5 / 61.8; 64 rows of 60 8.0 / 8.1, of 120 11.1 / 10.2,
+// of 250 17.1 / 13.7; of 256 values, 64 rows of 120 17.5 / 18.9, of 250 25.7 / 26.0.
 bool one_wave_rows(int64_t D, int64_t longest, int64_t workgroups) {
     return longest <= 512 && 2 * workgroups >= held(D) * (longest <= 64 ? 2 : longest <= 128 ? 3 : 6);
 }
@@ -529,8 +530,8 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
 
 // out of a split row from its parts' (O, m, l): a workgroup a (row, head), groups of D / 4 threads over the parts, JOIN
 // parts a group in flight; the first of them are on their way while the weights are formed.  One wave where there
-// are many (row, head)s, which have few parts each, else four: the call of 64 rows x 32 heads 158 us with four waves,
-// 155 with one, that of 1 x 40 with 64 parts each 99.4 and 102.2.
+// are many (row, head)s, which have few parts each, else four: 64 rows x 32 heads 8.1 us with four waves, 4.9 with one;
+// 1 x 40 with 64 parts each 5.3 with four, some 3 us more with one.
 constexpr int JOIN = 8;
 template <int N>
 __global__ __launch_bounds__(N) void paged_join_kernel(Launch p) {

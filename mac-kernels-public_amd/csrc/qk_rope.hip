@@ -60,9 +60,10 @@ struct Cut {
 };
 
 // The values a lane holds of a row: x[e] and x[VW + e] are a pair, or x[2 e] and x[2 e + 1] of interleaved ones.
-// VEC: two vectors, which neighbouring lanes continue; else value by value (any D and P).  A lane past the row's
-// end holds zeros.
-template <typename T, int VW, bool VEC, bool INTER>
+// VEC: two vectors, which neighbouring lanes continue (ONCE: read nontemporally); else value by value (any D and P).  A
+// lane past the row's end holds zeros.
+enum { SCALAR = 0, VECTORS = 1, ONCE = 2 };
+template <typename T, int VW, int VEC, bool INTER>
 struct Piece {
     static constexpr int N = 2 * VW;
     struct alignas(sizeof(T) * VW < 16 ? sizeof(T) * VW : 16) Vector { T v[VW]; };
@@ -101,13 +102,11 @@ struct Piece {
         *reinterpret_cast<V*>(x) = *reinterpret_cast<const V*>(table + pair);
         *reinterpret_cast<V*>(x + VW / 2) = *reinterpret_cast<const V*>(table + (VEC && INTER ? pair2 : pair + VW / 2));
     }
-    // Nontemporal: a row is read once, and what it would take of the caches is left to the outputs, which the next kernel
-    // reads.  Measured with a kernel that writes the rows before and one that reads the outputs after (us, all three): 4608
-    // tokens x 96 heads 137 against 150, 9504 x 80 234 against 245, 4095 x 48 58 against 58; the gradient 145 against
-    // 159 and 244 against 264.  Nontemporal stores: 139, 245, 63; 156 and 264.
     static __device__ __forceinline__ Vector vector_at(const T* p) {
         typedef uint32_t Words __attribute__((ext_vector_type(sizeof(Vector) % 16 ? 2 : 4)));
-        if constexpr (sizeof(Vector) == sizeof(Words)) {
+        if constexpr (VEC != ONCE) {
+            return *reinterpret_cast<const Vector*>(p);
+        } else if constexpr (sizeof(Vector) == sizeof(Words)) {
             return __builtin_bit_cast(Vector, __builtin_nontemporal_load(reinterpret_cast<const Words*>(p)));
         } else {
             struct Two { Words a, b; };
@@ -220,7 +219,7 @@ __device__ __forceinline__ void read_row(const float* p, float* x) {
 
 extern __shared__ __align__(16) float lds[];
 
-template <int DT, int VW, bool VEC, bool INTER>
+template <int DT, int VW, int VEC, bool INTER>
 __global__ __launch_bounds__(THREADS) void head_rope_kernel(HeadRopeArgs a, Cut cut) {
     using T = typename HeadType<DT>::T;
     using PC = Piece<T, VW, VEC, INTER>;
@@ -318,7 +317,7 @@ __global__ __launch_bounds__(THREADS) void head_rope_kernel(HeadRopeArgs a, Cut 
 
 // A workgroup takes q's rows (workgroups below parts_q) or k's.  Sums of the weight's gradient stay in a lane over all
 // its rows and are added up over the workgroup at the end, in a fixed order; every workgroup leaves one partial [D].
-template <int DT, int VW, bool VEC, bool INTER>
+template <int DT, int VW, int VEC, bool INTER>
 __global__ __launch_bounds__(THREADS, VEC ? 4 : 1) void head_grad_kernel(HeadGradArgs a, Cut cut, Divisor by_q, Divisor by_k, int parts_q) {
     using T = typename HeadType<DT>::T;
     using PC = Piece<T, VW, VEC, INTER>;
@@ -424,16 +423,26 @@ bool aligned(const void* p, std::initializer_list<int64_t> strides, int es, int 
 
 // The pieces of a call: 8 pairs a lane where both sizes allow 8-value vectors and all rows are aligned to them, else 4,
 // else 8 value by value.  Vectors of interleaved pairs hold whole pairs whatever P is.
+//
+// Rows of more than MUCH bytes in all are read nontemporally: what they would take of the caches is left to the outputs,
+// which the next kernel reads.  Measured with a kernel that writes the rows before and one that reads the outputs after
+// (us, all three; nontemporal / not): 9504 tokens x 80 heads of 128 (195 MB) 234 / 245, 4608 x 96 (113) 137 / 150, 4095 x 48
+// (50) 58.0 / 58.4, 1056 x 96 (26) 36.8 / 36.8; the gradient 244 / 264, 145 / 159, -, 50.5 / 49.6; a forward
+// call and its gradient on 1056 x 96 at once, which read the same rows, 44.8 / 41.3.  Nontemporal stores gain nothing there:
+// 245, 139, 63.
+constexpr int64_t MUCH = 32 << 20;
+
 struct Kind {
     int VW;
-    bool vec;
+    int vec;
 };
 template <typename ALIGNED>
-Kind kind_of(int D, const RopeTurn& turn, int dtype, const ALIGNED& all_aligned) {
+Kind kind_of(int64_t rows, int D, const RopeTurn& turn, int dtype, const ALIGNED& all_aligned) {
     const int es = dtype == DT_F32 ? 4 : 2, P = turn.interleaved ? 0 : turn.P;
-    if (D % 16 == 0 && P % 8 == 0 && all_aligned(es, 16)) return {8, true};
-    if (D % 8 == 0 && P % 4 == 0 && all_aligned(es, 4 * es)) return {4, true};
-    return {8, false};
+    const int vec = rows * D * es > MUCH ? ONCE : VECTORS;
+    if (D % 16 == 0 && P % 8 == 0 && all_aligned(es, 16)) return {8, vec};
+    if (D % 8 == 0 && P % 4 == 0 && all_aligned(es, 4 * es)) return {4, vec};
+    return {8, SCALAR};
 }
 
 // Tokens whose cosines and sines a workgroup holds in LDS, at most: 32 KB of them, or two tokens.
@@ -472,25 +481,31 @@ size_t lds_bytes(const Kind& k, int D, int tokens, bool grad) {
 template <int DT, bool INTER>
 hipError_t launch_rope(const HeadRopeArgs& a, const Kind& k, const Cut& c, dim3 grid, hipStream_t st) {
     const size_t bytes = lds_bytes(k, a.D, c.tokens, false);
-    if (!k.vec) hipLaunchKernelGGL((head_rope_kernel<DT, 8, false, INTER>), grid, dim3(THREADS), bytes, st, a, c);
-    else if (k.VW == 8) hipLaunchKernelGGL((head_rope_kernel<DT, 8, true, INTER>), grid, dim3(THREADS), bytes, st, a, c);
-    else hipLaunchKernelGGL((head_rope_kernel<DT, 4, true, INTER>), grid, dim3(THREADS), bytes, st, a, c);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(THREADS), bytes, st, a, c); };
+    if (k.vec == SCALAR) go(head_rope_kernel<DT, 8, SCALAR, INTER>);
+    else if (k.VW == 8 && k.vec == ONCE) go(head_rope_kernel<DT, 8, ONCE, INTER>);
+    else if (k.VW == 8) go(head_rope_kernel<DT, 8, VECTORS, INTER>);
+    else if (k.vec == ONCE) go(head_rope_kernel<DT, 4, ONCE, INTER>);
+    else go(head_rope_kernel<DT, 4, VECTORS, INTER>);
     return hipGetLastError();
 }
 
 template <int DT, bool INTER>
 hipError_t launch_grad(const HeadGradArgs& a, const Kind& k, const Cut& c, dim3 grid, int parts_q, hipStream_t st) {
     const size_t bytes = lds_bytes(k, a.D, c.tokens, true);
-    if (!k.vec) hipLaunchKernelGGL((head_grad_kernel<DT, 8, false, INTER>), grid, dim3(THREADS), bytes, st, a, c, Divisor(a.Hq), Divisor(a.Hk), parts_q);
-    else if (k.VW == 8) hipLaunchKernelGGL((head_grad_kernel<DT, 8, true, INTER>), grid, dim3(THREADS), bytes, st, a, c, Divisor(a.Hq), Divisor(a.Hk), parts_q);
-    else hipLaunchKernelGGL((head_grad_kernel<DT, 4, true, INTER>), grid, dim3(THREADS), bytes, st, a, c, Divisor(a.Hq), Divisor(a.Hk), parts_q);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(THREADS), bytes, st, a, c, Divisor(a.Hq), Divisor(a.Hk), parts_q); };
+    if (k.vec == SCALAR) go(head_grad_kernel<DT, 8, SCALAR, INTER>);
+    else if (k.VW == 8 && k.vec == ONCE) go(head_grad_kernel<DT, 8, ONCE, INTER>);
+    else if (k.VW == 8) go(head_grad_kernel<DT, 8, VECTORS, INTER>);
+    else if (k.vec == ONCE) go(head_grad_kernel<DT, 4, ONCE, INTER>);
+    else go(head_grad_kernel<DT, 4, VECTORS, INTER>);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
-    const Kind k = kind_of(a.D, a.turn, a.dtype, [&](int es, int bytes) {
+    const Kind k = kind_of(a.T * (a.Hq + a.Hk), a.D, a.turn, a.dtype, [&](int es, int bytes) {
         if (!aligned(a.q.p, {a.q.st, a.q.sh}, es, bytes) || !aligned(a.qo.p, {a.qo.st, a.qo.sh}, es, bytes)) return false;
         if (a.Hk == 0) return true;
         if (!aligned(a.k.p, {a.k.st, a.k.sh}, es, bytes)) return false;
@@ -501,8 +516,8 @@ hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
     Cut c = cut_of(k, a.D, a.Hq + a.Hk + (a.store ? a.Hk : 0));
     // Equal runs of rows, in whole rounds of the lane groups: a small call is spread over the chip, a row a lane group; a
     // large one over WORKGROUPS at a time, which share a token's cosines among up to 5 rounds.  Measured (us, at
-    // most 3 / 5 / 8 / 16 rounds): 4095 tokens x 56 rows into a cache 28.2 / 26.3 / 26.0 / 26.7, 4608 x 96 42.3 /
-    // 41.7 / 47.1 / 47.0, 9504 x 80 78.5 / 79.6 / 82.0 / 93.1.
+    // most 3 / 5 / 8 / 16 rounds): 4095 tokens x 56 rows into a cache 29.7 / 26.4 / 26.8 / 26.1, 4608 x 96 41.5 /
+    // 41.1 / 46.4 / 46.4, 9504 x 80 75.1 / 76.9 / 80.5 / 91.5.
     const int64_t groups = THREADS / c.lanes, rows = a.T * c.heads, round = groups * WORKGROUPS;
     const int64_t times = std::max<int64_t>(1, (rows + MOST_ROUNDS * round - 1) / (MOST_ROUNDS * round));
     int64_t span = std::max<int64_t>(1, (rows + times * round - 1) / (times * round)) * groups;
@@ -521,7 +536,7 @@ int head_grad_parts(int64_t T, int64_t) { return (int)std::max<int64_t>(2, std::
 size_t ws_head_grad(int64_t T, int64_t heads, int64_t D) { return (size_t)head_grad_parts(T, heads) * D * 4; }
 
 hipError_t run_head_grad(const HeadGradArgs& a, hipStream_t st) {
-    const Kind k = kind_of(a.D, a.turn, a.dtype, [&](int es, int bytes) {
+    const Kind k = kind_of(a.T * (a.Hq + a.Hk), a.D, a.turn, a.dtype, [&](int es, int bytes) {
         for (const HeadView* v : {&a.q, &a.gq, &a.dq})
             if (!aligned(v->p, {v->st, v->sh}, es, bytes)) return false;
         if (a.Hk > 0)

@@ -171,6 +171,27 @@ def test_many_tokens_of_one_head(t, d):
     assert bool(((dq.double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("d,sizes,inter", [(128, (64, 64), True), (128, (128,), False), (72, (24, 48), True), (72, (72,), False)])
+def test_large_calls_are_their_parts(d, sizes, inter, dtype):
+    """Rows of more than 32 MB are read in another way than small ones: the same bits as token by token slices."""
+    Q = qlin()
+    h, hk = 12, 4
+    t = (40 << 20) // ((h + hk) * d * (4 if dtype == F32 else 2))
+    freq, axis = (x.to(DEV) for x in Q.rope_frequencies(sizes))
+    pos = grid_positions(len(sizes), t).to(DEV)
+    gen = torch.Generator(DEV).manual_seed(1)
+    qkv, g = (torch.randn(t, h + hk, d, generator=gen, device=DEV).to(dtype) for _ in range(2))
+    w = (1 + 0.2 * rand(d, seed=3)).to(DEV)
+    run = lambda a, b: Q.qk_norm_rope(qkv[a:b, :h], qkv[a:b, h:], w, w, pos[:, a:b], freq, axis, interleaved=inter)
+    grad = lambda a, b: Q.qk_norm_rope_grad(g[a:b, :h], g[a:b, h:], qkv[a:b, :h], qkv[a:b, h:], w, w, pos[:, a:b], freq, axis,
+                                            interleaved=inter)[:2]
+    for call in (run, grad):
+        whole, parts = call(0, t), [call(a, min(a + 501, t)) for a in range(0, t, 501)]
+        for i in range(2):
+            assert torch.equal(whole[i], torch.cat([p[i] for p in parts]))
+
+
 def test_axis_entries_outside_count_as_the_nearest():
     Q = qlin()
     freq, axis = Q.rope_frequencies((32, 32))
