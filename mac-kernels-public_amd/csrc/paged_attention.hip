@@ -12,7 +12,10 @@
 //
 // The weights p enter the second product as two 16-bit parts (p rounded, and what is left of it), or a row's
 // output would carry their rounding on top of its own.  Up to 8 heads the second part rides in the 8 columns that the
-// heads leave free; 9 to 16 heads take a second instruction.
+// heads leave free; 9 to 16 heads take a second instruction.  fp16 has no exponents below 2^-24, and weights that far below a
+// row's largest add up over a long row: there p is 2^15 exp(s - m), the second part 2^11 times what is left, and the parts'
+// sums are kept apart until the end, so that a weight keeps 16 bits down to 2^-35 of the largest and counts down to 2^-51.
+// O and l have the factor alike.
 //
 // Work split: a row's tokens count in units of 128 (4 waves x 32), all rows' units are laid end to end and every
 // workgroup takes an equal run of them, as many workgroups as the chip holds at once.  So one long row among short ones
@@ -39,8 +42,9 @@ constexpr int MAX_ROWS = 1024;       // rows of one launch (their lengths are su
 constexpr int CUS = 256;
 constexpr int MOST_GROUPS = 4 * CUS;  // of any head size: see held()
 
-// Workgroups of the kernel for this head size that the chip holds at once (registers: 4, 2 and 1 on a compute unit).
-int64_t held(int64_t D) { return CUS * (D <= 64 ? 4 : D <= 128 ? 2 : 1); }
+// Workgroups of the kernel for this head size that the chip holds at once (registers: 4, 2 and 1 on a compute unit; 3 of
+// small heads in groups of 9 to 16, `wide`: 8 rows of 8000 to 16384 tokens, 64 over 4 heads of 64 values 26.8 us so, 29.8 with 4).
+int64_t held(int64_t D, bool wide) { return CUS * (D <= 64 ? wide ? 3 : 4 : D <= 128 ? 2 : 1); }
 
 // Units up to which rows are not split: a workgroup takes one whole row, without the running sum and the second kernel.
 // Where that fills the chip rows may be longer.  Measured, not split / split (us, 8 kv heads; 1 unit = 128 tokens):
@@ -56,7 +60,7 @@ int64_t whole_rows(int64_t D, int64_t workgroups) {
 // of 60 12.1 / 19.8, of 120 17.7 / 23.1, of 250 31.2 / 38.2, of 500 59.5 / 61.8; 64 rows of 60 8.0 / 8.1, of 120 11.1 / 10.2,
 // of 250 17.1 / 13.7; of 256 values, 64 rows of 120 17.5 / 18.9, of 250 25.7 / 26.0.
 bool one_wave_rows(int64_t D, int64_t longest, int64_t workgroups) {
-    return longest <= 512 && 2 * workgroups >= held(D) * (longest <= 64 ? 2 : longest <= 128 ? 3 : 6);
+    return longest <= 512 && 2 * workgroups >= held(D, false) * (longest <= 64 ? 2 : longest <= 128 ? 3 : 6);
 }
 
 struct Launch {
@@ -75,8 +79,10 @@ struct Launch {
 // those of keys and values.
 typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
 
+// RAISE: the largest weight is 2^RAISE.  LOW: factor of a weight's second part.
 template <int DT> struct Mma;
 template <> struct Mma<DT_F16> {
+    static constexpr float RAISE = 15.0f, LOW = 2048.0f;
     static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
@@ -87,6 +93,7 @@ template <> struct Mma<DT_F16> {
     }
 };
 template <> struct Mma<DT_BF16> {
+    static constexpr float RAISE = 0.0f, LOW = 1.0f;
     static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
                 q[j] = *reinterpret_cast<const u32x4*>((const uint16_t*)a.q.p + sh.b * a.q.st +
                                                        (int64_t)(kvh * G + h0 + col) * a.q.sh + 32 * j + 8 * g);
         }
-        f32x4 acc[EPL] = {};
+        f32x4 acc[EPL] = {}, low[WIDE ? EPL : 1] = {};  // up to 8 heads: of the second parts in the columns 8 .. 15
         float m = -INFINITY, l = 0.0f;
         int t = start + wave * TILE;
         if (t < end) {
@@ -428,7 +435,9 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
                 float w[8], sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(s[i] - base);
+                    w[i] = s[i] - base;
+                    if constexpr (Mma<DT>::RAISE != 0.0f) w[i] += Mma<DT>::RAISE;
+                    w[i] = __builtin_amdgcn_exp2f(w[i]);
                     sum += w[i];
                 }
                 l = l * keep + sum;
@@ -437,18 +446,22 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
-                        pl[i] = Mma<DT>::pack(w[2 * i] - Mma<DT>::rounded(w[2 * i]), w[2 * i + 1] - Mma<DT>::rounded(w[2 * i + 1]));
+                        pl[i] = Mma<DT>::pack((w[2 * i] - Mma<DT>::rounded(w[2 * i])) * Mma<DT>::LOW,
+                                              (w[2 * i + 1] - Mma<DT>::rounded(w[2 * i + 1])) * Mma<DT>::LOW);
                     }
                 } else {
                     const bool second = n & 8;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] -= second ? Mma<DT>::rounded(w[i]) : 0.0f;
+                    for (int i = 0; i < 8; ++i) w[i] = second ? (w[i] - Mma<DT>::rounded(w[i])) * Mma<DT>::LOW : w[i];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
                 }
                 if (__ballot(keep != 1.0f)) {
 #pragma unroll
-                    for (int j = 0; j < EPL; ++j) acc[j] *= keep;
+                    for (int j = 0; j < EPL; ++j) {
+                        acc[j] *= keep;
+                        if constexpr (WIDE) low[j] *= keep;
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < EPL; ++j) {
@@ -458,7 +471,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
 #pragma unroll
                     for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vr[2 * i + 1][ld][word], vr[2 * i][ld][word], sel);
                     acc[j] = Mma<DT>::mul(vt, ph, acc[j]);
-                    if constexpr (WIDE) acc[j] = Mma<DT>::mul(vt, pl, acc[j]);
+                    if constexpr (WIDE) low[j] = Mma<DT>::mul(vt, pl, low[j]);
                 }
                 if (!more) break;
                 load_v(y);
@@ -470,12 +483,15 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
         // join of the four waves: lane (n, g) has dims of rows 4 g + i of its head: EPL (or 8 + 8) consecutive ones each
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        if constexpr (!WIDE) {
 #pragma unroll
-            for (int j = 0; j < EPL; ++j)
+        for (int j = 0; j < EPL; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] += __shfl_xor(acc[j][i], 8);
-        }
+            for (int i = 0; i < 4; ++i) {
+                float second;
+                if constexpr (WIDE) second = low[j][i];
+                else second = __shfl_xor(acc[j][i], 8);
+                acc[j][i] = __builtin_fmaf(second, 1.0f / Mma<DT>::LOW, acc[j][i]);
+            }
         if (n < OH) {
             if (g == 0) {
                 lds_m[wave][n] = m;
@@ -591,7 +607,7 @@ void head_groups(int64_t G, int& ng, int& hpg) {
     ng = (int)((G + 15) / 16);
     hpg = (int)((G + ng - 1) / ng);
 }
-int64_t shares_of(int64_t hg, int64_t D) { return std::max<int64_t>(1, held(D) / hg); }
+int64_t shares_of(int64_t hg, int64_t hpg, int64_t D) { return std::max<int64_t>(1, held(D, hpg > 8) / hg); }
 
 template <int DT, int DP>
 hipError_t launch(const Launch& p, bool p16, bool one_wave, unsigned grid, hipStream_t st) {
@@ -621,7 +637,7 @@ size_t ws_paged_attention(int64_t, int64_t H, int64_t Hk, int64_t D) {
     if (Hk < 1 || H < Hk) return 0;
     int ng, hpg;
     head_groups(H / Hk, ng, hpg);
-    const size_t heads = (size_t)(2 * shares_of(Hk * ng, D) * Hk * ng) * hpg;
+    const size_t heads = (size_t)(2 * shares_of(Hk * ng, hpg, D) * Hk * ng) * hpg;
     return META_BYTES + heads * 8 + heads * D * 4 + 256;
 }
 
@@ -629,7 +645,7 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
     Launch p;
     head_groups(a.H / a.Hk, p.ng, p.hpg);
     const int64_t hg = (int64_t)a.Hk * p.ng;
-    p.shares = (int)shares_of(hg, a.D);
+    p.shares = (int)shares_of(hg, p.hpg, a.D);
     // 16-token tiles whose places are reached by 32-bit offsets from a uniform address
     const auto near = [](int64_t sp) { return sp >= 0 && sp < (1 << 24); };
     const bool p16 = a.page % 16 == 0 && near(a.kc.sp) && near(a.vc.sp);
