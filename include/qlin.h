@@ -376,7 +376,8 @@ qlin_status qlin_paged_plan(const qlin_tensor* context, const qlin_tensor* added
  * shares one row: the tokens of one prompt are rows with lengths 1, 2, ...); lengths i32 [rows], at most W * page
  * counts.  D a multiple of 8 up to 256, 16-byte aligned rows (QLIN_EUNSUPPORTED otherwise).  A row with no token gives
  * zeros; a token whose table entry is outside the cache counts as absent.  What the cache holds behind a row's last
- * token is never used, whatever it is.  Scores, their running maximum and sum and the output are fp32.
+ * token is never used, whatever it is.  Scores, their running maximum and sum and the output are fp32.  An infinite value
+ * gives its infinity (opposite ones NaN) where its weight is above 2^-39 (f16) or 2^-126 (bf16) of the row's largest, else NaN.
  * Workspace: qlin_workspace_size(QLIN_OP_PAGED_ATTENTION, rows, heads, D, kv heads, q's dtype). */
 qlin_status qlin_paged_attention(const qlin_tensor* q, const qlin_tensor* k_cache, const qlin_tensor* v_cache,
                                  const qlin_tensor* block_table, const qlin_tensor* lengths, float scale, int64_t window,

@@ -10,12 +10,13 @@
 // The order of tokens in the second product is free, so it is the order in which a lane holds S^T: the weights
 // go from one to the other in their lane, and m, l and the rescaling are per lane (its column is a head).
 //
-// The weights p enter the second product as two 16-bit parts (p rounded, and what is left of it), or a row's
+// The weights p enter the second product as two 16-bit parts (p cut off, and what is left of it), or a row's
 // output would carry their rounding on top of its own.  Up to 8 heads the second part rides in the 8 columns that the
-// heads leave free; 9 to 16 heads take a second instruction.  fp16 has no exponents below 2^-24, and weights that far below a
-// row's largest add up over a long row: there p is 2^15 exp(s - m), the second part 2^11 times what is left, and the parts'
-// sums are kept apart until the end, so that a weight keeps 16 bits down to 2^-35 of the largest and counts down to 2^-51.
-// O and l have the factor alike.
+// heads leave free; 9 to 16 heads take a second instruction.  The second part is never negative, and at least the type's
+// least: an infinite value gives its infinity with both parts (0 times it would be a NaN).  fp16 has no exponents below
+// 2^-24, and weights that far below a row's largest add up over a long row: there p is 2^15 exp(s - m), the second part 2^11
+// times what is left, and the parts' sums are kept apart until the end, so that a weight keeps 16 bits down to 2^-35 of the
+// largest and counts down to 2^-50.  O and l have the factor alike.
 //
 // Work split: a row's tokens count in units of 128 (4 waves x 32), all rows' units are laid end to end and every
 // workgroup takes an equal run of them, as many workgroups as the chip holds at once.  So one long row among short ones
@@ -79,27 +80,31 @@ struct Launch {
 // those of keys and values.
 typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
 
-// RAISE: the largest weight is 2^RAISE.  LOW: factor of a weight's second part.
+// The weights' parts, in pairs.  RAISE: the largest weight is 2^RAISE.  LOW: factor of a weight's second part.
 template <int DT> struct Mma;
 template <> struct Mma<DT_F16> {
-    static constexpr float RAISE = 15.0f, LOW = 2048.0f;
+    static constexpr float RAISE = 15.0f, LOW = 2048.0f, LEAST = 0x1p-24f;
     static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ float rounded(float v) { return (float)(f16)v; }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        const f16x2 h = {(f16)a, (f16)b};
-        return __builtin_bit_cast(uint32_t, h);
+    static __device__ __forceinline__ uint32_t first(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    }
+    static __device__ __forceinline__ uint32_t second(float a, float b, uint32_t of) {
+        const f16x2 h = __builtin_bit_cast(f16x2, of);
+        return first(__builtin_fmaf(a - (float)h[0], LOW, LEAST), __builtin_fmaf(b - (float)h[1], LOW, LEAST));
     }
 };
 template <> struct Mma<DT_BF16> {
-    static constexpr float RAISE = 0.0f, LOW = 1.0f;
+    static constexpr float RAISE = 0.0f, LOW = 1.0f, LEAST = 0x1p-126f;
     static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ float rounded(float v) { return (float)(__bf16)v; }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        const bf16x2 h = {(__bf16)a, (__bf16)b};
+    static __device__ __forceinline__ uint32_t first(float a, float b) {
+        return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+    static __device__ __forceinline__ uint32_t second(float a, float b, uint32_t of) {
+        const bf16x2 h = {(__bf16)(a - __uint_as_float(of << 16) + LEAST), (__bf16)(b - __uint_as_float(of & 0xFFFF0000u) + LEAST)};
         return __builtin_bit_cast(uint32_t, h);
     }
 };
@@ -241,6 +246,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
     using VT = typename std::conditional<EPL == 4, u32x2, u32x4>::type;
     constexpr int OS = DP + 4;               // row stride of the join in LDS
     constexpr int OH = WIDE ? 16 : 8;
+    constexpr bool APART = WIDE && Mma<DT>::LOW != 1.0f;  // the second parts have sums of their own
     __shared__ float lds_o[W][OH][OS];
     __shared__ float lds_m[W][16], lds_l[W][16];
     const PagedAttentionArgs& a = p.a;
@@ -392,7 +398,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
                 q[j] = *reinterpret_cast<const u32x4*>((const uint16_t*)a.q.p + sh.b * a.q.st +
                                                        (int64_t)(kvh * G + h0 + col) * a.q.sh + 32 * j + 8 * g);
         }
-        f32x4 acc[EPL] = {}, low[WIDE ? EPL : 1] = {};  // up to 8 heads: of the second parts in the columns 8 .. 15
+        f32x4 acc[EPL] = {}, low[APART ? EPL : 1] = {};
         float m = -INFINITY, l = 0.0f;
         int t = start + wave * TILE;
         if (t < end) {
@@ -442,25 +448,17 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
                 }
                 l = l * keep + sum;
                 u32x4 ph, pl;
-                if constexpr (WIDE) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
-                        pl[i] = Mma<DT>::pack((w[2 * i] - Mma<DT>::rounded(w[2 * i])) * Mma<DT>::LOW,
-                                              (w[2 * i + 1] - Mma<DT>::rounded(w[2 * i + 1])) * Mma<DT>::LOW);
-                    }
-                } else {
-                    const bool second = n & 8;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = second ? (w[i] - Mma<DT>::rounded(w[i])) * Mma<DT>::LOW : w[i];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) ph[i] = Mma<DT>::pack(w[2 * i], w[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) {
+                    ph[i] = Mma<DT>::first(w[2 * i], w[2 * i + 1]);
+                    pl[i] = Mma<DT>::second(w[2 * i], w[2 * i + 1], ph[i]);
+                    if (!WIDE && (n & 8)) ph[i] = pl[i];
                 }
                 if (__ballot(keep != 1.0f)) {
 #pragma unroll
                     for (int j = 0; j < EPL; ++j) {
                         acc[j] *= keep;
-                        if constexpr (WIDE) low[j] *= keep;
+                        if constexpr (APART) low[j] *= keep;
                     }
                 }
 #pragma unroll
@@ -471,7 +469,8 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
 #pragma unroll
                     for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vr[2 * i + 1][ld][word], vr[2 * i][ld][word], sel);
                     acc[j] = Mma<DT>::mul(vt, ph, acc[j]);
-                    if constexpr (WIDE) low[j] = Mma<DT>::mul(vt, pl, low[j]);
+                    if constexpr (APART) low[j] = Mma<DT>::mul(vt, pl, low[j]);
+                    else if constexpr (WIDE) acc[j] = Mma<DT>::mul(vt, pl, acc[j]);
                 }
                 if (!more) break;
                 load_v(y);
@@ -483,15 +482,13 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 1 : 2) void paged_attention_ker
         // join of the four waves: lane (n, g) has dims of rows 4 g + i of its head: EPL (or 8 + 8) consecutive ones each
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
+        if constexpr (!WIDE || APART) {
 #pragma unroll
-        for (int j = 0; j < EPL; ++j)
+            for (int j = 0; j < EPL; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float second;
-                if constexpr (WIDE) second = low[j][i];
-                else second = __shfl_xor(acc[j][i], 8);
-                acc[j][i] = __builtin_fmaf(second, 1.0f / Mma<DT>::LOW, acc[j][i]);
-            }
+                for (int i = 0; i < 4; ++i)
+                    acc[j][i] = __builtin_fmaf(APART ? low[APART ? j : 0][i] : __shfl_xor(acc[j][i], 8), 1.0f / Mma<DT>::LOW, acc[j][i]);
+        }
         if (n < OH) {
             if (g == 0) {
                 lds_m[wave][n] = m;

@@ -3,7 +3,7 @@ plans that are kept and saved, second derivatives, sizes at the ends of their ra
 
 import pytest
 import torch
-from test_gpu_paged_attention import DEV, F16, check, make
+from test_gpu_paged_attention import BF16, DEV, F16, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,26 @@ def test_a_token_far_above_the_rest(lengths, heads, kv_heads, dim, page, width, 
     v[first, 0] = 0
     s = (q, k, v, table, n)
     check(qlin().paged_attention(*s, scale=1.0), *s, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page,width", PATHS + [([1], 8, 2, 128, 16, 4)])
+def test_infinities_in_values(lengths, heads, kv_heads, dim, page, width, dtype):
+    """An infinite value gives its infinity, opposite ones and a NaN give NaN, and no other value of the row changes."""
+    q, k, v, table, n = make(lengths, heads, kv_heads, dim, page, dtype, width=width)
+    inf, b, last = float("inf"), len(lengths) - 1, lengths[-1] - 1
+    first, end = int(table[b, 0]), int(table[b, last // page])
+    plain = v.clone()
+    plain[first, 0, 0, 3:8] = 0
+    plain[end, last % page, 0, 6] = 0
+    v[first, 0, 0, 3:8] = torch.tensor([inf, -inf, inf, inf, float("nan")], dtype=dtype, device=DEV)
+    v[end, last % page, 0, 6] = -inf
+    got, want = (qlin().paged_attention(q, k, x, table, n) for x in (v, plain))
+    check(want, q, k, plain, table, n)
+    heads_of_0 = heads // kv_heads
+    assert bool((got[b, :heads_of_0, 3] == inf).all()) and bool((got[b, :heads_of_0, 4] == -inf).all())
+    assert bool((got[b, :heads_of_0, 5] == inf).all()) and bool(got[b, :heads_of_0, 7].isnan().all())
+    sixth = got[b, :heads_of_0, 6]
+    assert bool((sixth == -inf).all() if last == 0 else sixth.isnan().all())
+    want[b, :heads_of_0, 3:8] = got[b, :heads_of_0, 3:8] = 0
+    assert torch.equal(got, want)
