@@ -4,6 +4,7 @@ plans that are kept and saved, second derivatives, sizes at the ends of their ra
 import pytest
 import torch
 from test_gpu_paged_attention import BF16, DEV, F16, check, make
+from test_gpu_qk_rope import rand
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,31 @@ def test_infinities_in_values(lengths, heads, kv_heads, dim, page, width, dtype)
     assert bool((sixth == -inf).all() if last == 0 else sixth.isnan().all())
     want[b, :heads_of_0, 3:8] = got[b, :heads_of_0, 3:8] = 0
     assert torch.equal(got, want)
+
+
+def same_values(a, b):
+    """Equal values, NaN where NaN is, zeros of the same sign."""
+    return a.shape == b.shape and bool((((a == b) & (a.signbit() == b.signbit())) | (a.isnan() & b.isnan())).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("d,rotated", [(128, 64), (128, 0), (72, 24), (20, 12), (7, 4)])
+def test_values_behind_the_rotation_pass_as_they_are(d, rotated, inter, dtype):
+    """Whatever they are, and without any effect on one another."""
+    Q = qlin()
+    t, h = 5, 3
+    freq, _ = Q.rope_frequencies(rotated, device=DEV)
+    pos = torch.arange(t, device=DEV)
+    q = rand(t, h, d, seed=1, dtype=dtype).to(DEV)
+    clean = Q.axis_rope(q, None, pos, freq, interleaved=inter)[0]
+    q[:, 0, rotated + 1], q[:, 1, d - 1], q[:, 2, rotated] = float("nan"), float("-inf"), -0.0
+    y = Q.axis_rope(q, None, pos, freq, interleaved=inter)[0]
+    assert same_values(y[..., rotated:], q[..., rotated:]) and torch.equal(y[..., :rotated], clean[..., :rotated])
+    # with the norms an infinite value makes its row's others zero; a NaN in a gradient stays in its own weight's sum
+    y = Q.qk_norm_rope(q, None, None, None, pos, freq, interleaved=inter)[0][:, 1]
+    assert bool(y[:, d - 1].isnan().all()) and bool((y[:, : d - 1] == 0).all())
+    x, g, w = rand(t, h, d, seed=2, dtype=dtype).to(DEV), rand(t, h, d, seed=3, dtype=dtype).to(DEV), torch.ones(d, device=DEV)
+    g[2, 1, rotated + 1] = float("nan")
+    dw = Q.qk_norm_rope_grad(g, None, x, None, w, None, pos, freq, interleaved=inter)[2]
+    assert dw.isnan().nonzero().flatten().tolist() == [rotated + 1]
