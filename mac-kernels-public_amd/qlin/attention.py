@@ -237,16 +237,17 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, wi
 
 class _AxisRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, axis, interleaved):
+    def forward(ctx, q, k, positions, inv_freq, axis, interleaved, inverse):
         ctx.save_for_backward(positions, inv_freq, axis)
-        ctx.interleaved = bool(interleaved)
-        return axis_rope(q, k, positions, inv_freq, axis, interleaved=interleaved)
+        ctx.conf = (bool(interleaved), bool(inverse))
+        return axis_rope(q, k, positions, inv_freq, axis, interleaved=interleaved, inverse=inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
-        positions, inv_freq, axis = ctx.saved_tensors
-        dq, dk = axis_rope(gq, gk, positions, inv_freq, axis, interleaved=ctx.interleaved, inverse=True)
-        return dq, dk, None, None, None, None
+        interleaved, inverse = ctx.conf
+        # itself a rotation with gradients: a second derivative goes on through it
+        dq, dk = _AxisRope.apply(gq, gk, *ctx.saved_tensors, interleaved, not inverse)
+        return dq, dk, None, None, None, None, None
 
 
 class _QkNormRope(torch.autograd.Function):
@@ -257,6 +258,7 @@ class _QkNormRope(torch.autograd.Function):
         return qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, axis, eps=eps, interleaved=interleaved)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, positions, inv_freq, axis = ctx.saved_tensors
         eps, interleaved = ctx.conf
@@ -268,10 +270,10 @@ class _QkNormRope(torch.autograd.Function):
 
 
 def axis_rope_trainable(q, k, positions, inv_freq, axis=None, interleaved=False):
-    """axis_rope with gradients for q and k."""
-    return _AxisRope.apply(q, k, positions, inv_freq, axis, interleaved)
+    """axis_rope with gradients for q and k, of any order."""
+    return _AxisRope.apply(q, k, positions, inv_freq, axis, interleaved, False)
 
 
 def qk_norm_rope_trainable(q, k, q_weight, k_weight, positions, inv_freq, axis=None, eps=1e-6, interleaved=False):
-    """qk_norm_rope with gradients for q, k and the weights (frozen ones cost nothing)."""
+    """qk_norm_rope with gradients for q, k and the weights (frozen ones cost nothing); first derivatives only."""
     return _QkNormRope.apply(q, k, q_weight, k_weight, positions, inv_freq, axis, eps, interleaved)

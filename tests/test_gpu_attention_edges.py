@@ -4,7 +4,7 @@ plans that are kept and saved, second derivatives, sizes at the ends of their ra
 import pytest
 import torch
 from test_gpu_paged_attention import BF16, DEV, F16, check, make
-from test_gpu_qk_rope import rand
+from test_gpu_qk_rope import angles, grid_positions, rand, rotate
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,25 @@ def test_values_behind_the_rotation_pass_as_they_are(d, rotated, inter, dtype):
     g[2, 1, rotated + 1] = float("nan")
     dw = Q.qk_norm_rope_grad(g, None, x, None, w, None, pos, freq, interleaved=inter)[2]
     assert dw.isnan().nonzero().flatten().tolist() == [rotated + 1]
+
+
+def test_second_derivatives():
+    """The rotation's gradient has a gradient (by the outputs' gradients; the rotation is linear); the norms' has none and says so."""
+    Q = qlin()
+    t, h, d = 6, 2, 32
+    freq, axis = Q.rope_frequencies((16, 16))
+    pos = grid_positions(2, t)
+    ang = angles(pos, freq, axis)
+    x, scale = rand(t, h, d, seed=1), rand(t, h, d, seed=2)
+
+    def penalty(rope, x, scale):
+        y = rope(x)
+        (g,) = torch.autograd.grad((y ** 3 * scale).sum(), x, create_graph=True)
+        return torch.autograd.grad((g ** 2).sum(), x)[0]
+
+    dev = [a.to(DEV) for a in (pos, freq, axis)]
+    got = penalty(lambda a: Q.axis_rope_trainable(a, None, *dev)[0], x.to(DEV).requires_grad_(True), scale.to(DEV))
+    want = penalty(lambda a: rotate(a, ang, False), x.double().requires_grad_(True), scale.double())
+    assert float((got.double().cpu() - want).norm() / want.norm()) < 1e-5  # five fp32 stages of 2^-22 at most each
+    with pytest.raises(RuntimeError):
+        penalty(lambda a: Q.qk_norm_rope_trainable(a, None, None, None, *dev)[0], x.to(DEV).requires_grad_(True), scale.to(DEV))
