@@ -356,7 +356,7 @@ at::Tensor qk_norm_rope_store(const at::Tensor& q, const at::Tensor& k, const at
 
 pybind11::tuple qk_norm_rope_grad(const at::Tensor& gq, const OptTensor& gk, const at::Tensor& q, const OptTensor& k,
                                   const OptTensor& wq, const OptTensor& wk, double eps, const at::Tensor& positions,
-                                  const at::Tensor& inv_freq, const OptTensor& axis, int64_t flags, bool weight_grads) {
+                                  const at::Tensor& inv_freq, const OptTensor& axis, int64_t flags, bool wq_grad, bool wk_grad) {
     const char* op = "qk_norm_rope_grad";
     const OptTensor gt = gq, qt = q, pt = positions, ft = inv_freq;
     all_on_device(op, {&gt, &gk, &qt, &k, &wq, &wk, &pt, &ft, &axis});
@@ -367,8 +367,8 @@ pybind11::tuple qk_norm_rope_grad(const at::Tensor& gq, const OptTensor& gk, con
         dk = Opt(like(k3.t));
     }
     if (gk) h3 = Opt(heads_of(op, *gk, "dk_out"));
-    if (weight_grads && wq) da = Opt(at::empty_like(a.t));
-    if (weight_grads && wk) db = Opt(at::empty_like(b.t));
+    if (wq_grad && wq) da = Opt(at::empty_like(a.t));
+    if (wk_grad && wk) db = Opt(at::empty_like(b.t));
     const hipStream_t st = current_stream(q);
     at::Tensor ws;
     if (da.there || db.there)

@@ -153,13 +153,14 @@ def qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_f
                       interleaved=False, weight_grads=True):
     """(dq, dk, dq_weight, dk_weight) of qk_norm_rope from the gradients of its outputs.  The weights' gradients are summed
     in fp32 in a fixed order and rounded to the weight's dtype; None where there is no weight, and with `weight_grads`
-    False (frozen norms)."""
+    False (frozen norms; a pair says it for q's and k's apart)."""
     op = "qk_norm_rope_grad"
     _disabled(op)
+    of_q, of_k = weight_grads if isinstance(weight_grads, (tuple, list)) else (weight_grads, weight_grads)
     if ops._FAST is not None:
         try:
             return ops._FAST.qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, float(eps), positions, inv_freq, axis,
-                                               _flags(interleaved), bool(weight_grads))
+                                               _flags(interleaved), bool(of_q), bool(of_k))
         except ops._FastError as e:
             raise _fast_error(op, e) from None
     _check_device(op, dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, axis)
@@ -167,8 +168,8 @@ def qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_f
     dq = torch.empty(q3.shape, dtype=q.dtype, device=q.device)
     dk = None if k is None else torch.empty(k3.shape, dtype=k.dtype, device=q.device)
     wq, wk = _vector(q_weight), _vector(k_weight)
-    dwq = torch.empty_like(wq) if weight_grads and wq is not None else None
-    dwk = torch.empty_like(wk) if weight_grads and wk is not None else None
+    dwq = torch.empty_like(wq) if of_q and wq is not None else None
+    dwk = torch.empty_like(wk) if of_k and wk is not None else None
     ws = None
     if dwq is not None or dwk is not None:
         ws = ops._workspace(_lib.OP_QK_NORM_ROPE_GRAD, q3.shape[0], q3.shape[1] + (0 if k is None else k3.shape[1]),
@@ -264,7 +265,7 @@ class _QkNormRope(torch.autograd.Function):
         eps, interleaved = ctx.conf
         need = ctx.needs_input_grad
         dq, dk, dwq, dwk = qk_norm_rope_grad(gq, gk, q, k, q_weight, k_weight, positions, inv_freq, axis, eps=eps,
-                                             interleaved=interleaved, weight_grads=need[2] or need[3])
+                                             interleaved=interleaved, weight_grads=(need[2], need[3]))
         return (dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None, dwk if need[3] else None,
                 None, None, None, None, None)
 
@@ -275,5 +276,6 @@ def axis_rope_trainable(q, k, positions, inv_freq, axis=None, interleaved=False)
 
 
 def qk_norm_rope_trainable(q, k, q_weight, k_weight, positions, inv_freq, axis=None, eps=1e-6, interleaved=False):
-    """qk_norm_rope with gradients for q, k and the weights (frozen ones cost nothing); first derivatives only."""
+    """qk_norm_rope with gradients for q, k and the weights (a frozen weight's is not formed); first derivatives
+    only."""
     return _QkNormRope.apply(q, k, q_weight, k_weight, positions, inv_freq, axis, eps, interleaved)

@@ -95,6 +95,14 @@ def test_values_behind_the_rotation_pass_as_they_are(d, rotated, inter, dtype):
     assert dw.isnan().nonzero().flatten().tolist() == [rotated + 1]
 
 
+def routes(monkeypatch):
+    from qlin import ops
+    assert ops._FAST is not None
+    yield "C++"
+    monkeypatch.setattr(ops, "_FAST", None)
+    yield "ctypes"
+
+
 def test_second_derivatives():
     """The rotation's gradient has a gradient (by the outputs' gradients; the rotation is linear); the norms' has none and says so."""
     Q = qlin()
@@ -115,3 +123,32 @@ def test_second_derivatives():
     assert float((got.double().cpu() - want).norm() / want.norm()) < 1e-5  # five fp32 stages of 2^-22 at most each
     with pytest.raises(RuntimeError):
         penalty(lambda a: Q.qk_norm_rope_trainable(a, None, None, None, *dev)[0], x.to(DEV).requires_grad_(True), scale.to(DEV))
+
+
+def test_frozen_weights_have_no_gradient_formed(monkeypatch):
+    from qlin import attention
+    Q = qlin()
+    t, d = 12, 64
+    freq, pos = Q.rope_frequencies(64, device=DEV)[0], torch.arange(t, device=DEV)
+    real, formed = attention.qk_norm_rope_grad, []
+
+    def grad(*a, **k):
+        out = real(*a, **k)
+        formed.append([x is not None for x in out[2:]])
+        return out
+
+    monkeypatch.setattr(attention, "qk_norm_rope_grad", grad)
+    q, k = (rand(t, h, d, seed=h).to(DEV).requires_grad_(True) for h in (4, 2))
+    for learn in ((True, False), (False, True), (False, False), (True, True)):
+        w = [torch.ones(d, device=DEV).requires_grad_(r) for r in learn]
+        yq, yk = Q.qk_norm_rope_trainable(q, k, *w, pos, freq)
+        (yq.square().sum() + yk.square().sum()).backward()
+        assert formed.pop() == list(learn) and [x.grad is not None for x in w] == list(learn)
+    for route in routes(monkeypatch):
+        w = torch.ones(d, device=DEV)
+        a = [x.detach() for x in (q, k, q, k)]
+        both = real(*a, w, w, pos, freq)
+        for flags in ((True, False), (False, True), (False, False)):
+            out = real(*a, w, w, pos, freq, weight_grads=flags)
+            for i in range(2):
+                assert torch.equal(out[2 + i], both[2 + i]) if flags[i] else out[2 + i] is None, (route, flags)
