@@ -90,7 +90,7 @@ def build_torch_ops():
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", os.path.join(HERE, "..", "include"), "-I", "/opt/rocm/include", "-I", sysconfig.get_paths()["include"],
            *[a for p in ce.include_paths() for a in ("-I", p)],
-           "-L", os.path.dirname(OUT), "-lqlin", "-L", tlib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+           "-L", os.path.dirname(OUT), "-lqlin", "-L", tlib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
            "-ltorch_python", "-L", "/opt/rocm/lib", "-lamdhip64",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}", "-Wl,-rpath,/opt/rocm/lib"]
     r = subprocess.run(cmd, capture_output=True, text=True)

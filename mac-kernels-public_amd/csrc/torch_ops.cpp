@@ -9,6 +9,7 @@
 // NoCapableBackendError (QLIN_EUNSUPPORTED), ValueError (QLIN_EINVAL, QLIN_EWORKSPACE) or
 // QlinError, exactly as for its ctypes calls.
 #include <torch/extension.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 
 #include <string>
@@ -382,10 +383,10 @@ pybind11::tuple qk_norm_rope_grad(const at::Tensor& gq, const OptTensor& gk, con
     return pybind11::make_tuple(as(dq, qt), as(dk, k), weight(da), weight(db));
 }
 
-// n values of type dt over `base`'s memory, from the `first` on (in values of dt).
-at::Tensor part_of(const at::Tensor& base, at::ScalarType dt, int64_t first, int64_t n) {
+// n values of `base` [..], from the `first` on.
+at::Tensor part_of(const at::Tensor& base, int64_t first, int64_t n) {
     at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(),
-                                                            c10::scalarTypeToTypeMeta(dt));
+                                                            base.dtype());
     t.unsafeGetTensorImpl()->set_storage_offset(first);
     t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
     return t;
@@ -398,11 +399,12 @@ pybind11::tuple paged_plan(const at::Tensor& context, const at::Tensor& added, c
     all_on_device(op, {&ct, &at_, &tt, &ft});
     if (tokens < 0) fail(QLIN_EINVAL, std::string(op) + ": tokens must not be negative");
     const int64_t B = context.dim() == 1 ? context.size(0) : 0;
-    // one allocation for all results, each a tensor of its own over a part of it: slots, then the int32 ones
-    const at::Tensor all = at::empty({tokens + (2 * tokens + 2 * B + 3) / 2}, context.options().dtype(at::kLong));
-    const auto i32 = [&](int64_t first, int64_t n) { return part_of(all, at::kInt, 2 * tokens + first, n); };
-    const at::Tensor slots = part_of(all, at::kLong, 0, tokens), positions = i32(0, tokens), rows = i32(tokens, tokens),
-                     starts = i32(2 * tokens, B + 1), lengths = i32(2 * tokens + B + 1, B), used = i32(2 * tokens + 2 * B + 1, 1);
+    // One allocation for the int32 results of the tokens and one for those of the requests, each a tensor of its own over a
+    // part of it: what a caller keeps of a step (lengths) holds no memory of its tokens, and no memory has two dtypes.
+    const auto fresh = [&](int64_t n, at::ScalarType dt) { return at::Tensor(at::detail::empty_cuda({n}, dt, context.device(), c10::nullopt)); };
+    const at::Tensor slots = fresh(tokens, at::kLong), t2 = fresh(2 * tokens, at::kInt), r2 = fresh(2 * B + 2, at::kInt);
+    const at::Tensor positions = part_of(t2, 0, tokens), rows = part_of(t2, tokens, tokens), starts = part_of(r2, 0, B + 1),
+                     lengths = part_of(r2, B + 1, B), used = part_of(r2, 2 * B + 1, 1);
     qlin_tensor dc = desc(context), da = desc(added), df = desc(free_blocks), dt = desc(table), ds = desc(slots),
                 dp = desc(positions), dr = desc(rows), dst = desc(starts), dl = desc(lengths), du = desc(used);
     check(qlin_paged_plan(&dc, &da, &df, page, &dt, &ds, &dp, &dr, &dst, &dl, &du, current_stream(context)));

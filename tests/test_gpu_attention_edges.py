@@ -1,5 +1,6 @@
 """Edges of the attention side: weights far below a row's largest, infinities, values that pass a rotation by, empty heads,
 plans that are kept and saved, second derivatives, sizes at the ends of their ranges."""
+import io
 
 import pytest
 import torch
@@ -101,6 +102,22 @@ def routes(monkeypatch):
     yield "C++"
     monkeypatch.setattr(ops, "_FAST", None)
     yield "ctypes"
+
+
+def test_a_plan_is_saved_and_its_lengths_kept(monkeypatch):
+    """A plan's fields can be saved together, and a field that is kept keeps nothing of the others but their request tables."""
+    Q = qlin()
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    for route in routes(monkeypatch):
+        table = torch.zeros(3, 400, dtype=torch.int32, device=DEV)
+        plan = Q.paged_plan(ints([5, 0, 31]), ints([2000, 300, 1]), table, ints(list(range(200))), 16, 2301)
+        f = io.BytesIO()
+        torch.save(plan._asdict(), f)
+        f.seek(0)
+        back = torch.load(f, weights_only=True)
+        assert all(torch.equal(back[n], getattr(plan, n)) for n in plan._fields), route
+        for n in ("starts", "lengths", "used"):
+            assert getattr(plan, n).untyped_storage().nbytes() <= 512, (route, n)
 
 
 def test_second_derivatives():
