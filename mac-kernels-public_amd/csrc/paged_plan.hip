@@ -14,7 +14,8 @@ constexpr int THREADS = 256;
 constexpr int64_t MOST = 0x7FFFFFFF;
 
 // Largest i with sum[i] <= x among sum[0] = 0 <= sum[1] <= ... <= sum[n - 1]; x >= 0.
-__device__ __forceinline__ int find(const int32_t* sum, int n, int x) {
+template <typename T>
+__device__ __forceinline__ int find(const T* sum, int n, T x) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -25,14 +26,14 @@ __device__ __forceinline__ int find(const int32_t* sum, int n, int x) {
 }
 
 __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PagedPlanArgs a) {
-    extern __shared__ int32_t lds[];
-    int32_t* starts = lds;            // [B + 1]: new tokens before request b
-    int32_t* first = lds + a.B + 1;   // [B + 1]: missing pages before request b
+    extern __shared__ int64_t lds[];
+    int64_t* first = lds;                                   // [B + 1]: missing pages before request b
+    int32_t* starts = reinterpret_cast<int32_t*>(lds + a.B + 1);  // [B + 1]: new tokens before request b
     __shared__ int64_t wave_tokens[THREADS / 64], wave_pages[THREADS / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (a.B + THREADS - 1) / THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
 
-    // running sums, in 64 bits; what does not fit 32 stays at the largest value
+    // running sums, in 64 bits; a start that does not fit 32 stays at the largest value, which no place reaches
     int64_t tokens = 0, pages = 0;
     for (int b = b0; b < b1; ++b) {
         const int64_t c = max(a.context[b], 0), n = max(a.added[b], 0);
@@ -62,13 +63,13 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PagedPlanArgs a) {
     for (int b = b0; b < b1; ++b) {
         const int64_t c = max(a.context[b], 0), n = max(a.added[b], 0);
         starts[b] = (int32_t)min(st, MOST);
-        first[b] = (int32_t)min(sp, MOST);
+        first[b] = sp;
         st += n;
         sp += (c + n + a.page - 1) / a.page - (c + a.page - 1) / a.page;
     }
     if (tid == THREADS - 1) {
         starts[a.B] = (int32_t)min(st, MOST);
-        first[a.B] = (int32_t)min(sp, MOST);
+        first[a.B] = sp;
     }
     __syncthreads();
 
@@ -77,12 +78,14 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PagedPlanArgs a) {
         a.starts[b] = starts[b];
         if (b < a.B) a.lengths[b] = (int32_t)min((int64_t)max(a.context[b], 0) + max(a.added[b], 0), MOST);
     }
-    if (me == 0) a.used[0] = first[a.B];
-    const int needed = first[a.B];
+    if (me == 0) a.used[0] = (int32_t)min(first[a.B], MOST);
+    const int64_t needed = first[a.B];
     for (int64_t e = me; e < needed; e += all) {  // the new entries of the table
-        const int b = find(first, a.B + 1, (int)e);
+        const int b = find(first, a.B + 1, e);
         const int64_t at = ((int64_t)max(a.context[b], 0) + a.page - 1) / a.page + (e - first[b]);
         if (at < a.W) a.table[b * a.ldt + at] = e < a.F ? a.free_blocks[e] : -1;
+        // the request's other pages have no entry either, and a length that is wrong by far must not take a step for each
+        else e += (first[b + 1] - e - 1) / all * all;
     }
     const int total = starts[a.B];
     for (int64_t i = me; i < a.N; i += all) {
@@ -110,7 +113,7 @@ __global__ __launch_bounds__(THREADS) void paged_plan_kernel(PagedPlanArgs a) {
 hipError_t run_paged_plan(const PagedPlanArgs& a, hipStream_t st) {
     const int64_t work = std::max<int64_t>(a.N, a.B + 1);
     const unsigned grid = (unsigned)std::min<int64_t>((work + THREADS - 1) / THREADS, 256);
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(grid), dim3(THREADS), (size_t)2 * (a.B + 1) * 4, st, a);
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(grid), dim3(THREADS), (size_t)12 * (a.B + 1), st, a);
     return hipGetLastError();
 }
 

@@ -5,6 +5,7 @@ import io
 import pytest
 import torch
 from test_gpu_paged_attention import BF16, DEV, F16, check, make
+from test_gpu_paged_plan import check as check_plan
 from test_gpu_qk_rope import angles, grid_positions, rand, rotate
 
 pytestmark = pytest.mark.gpu
@@ -118,6 +119,33 @@ def test_a_plan_is_saved_and_its_lengths_kept(monkeypatch):
         assert all(torch.equal(back[n], getattr(plan, n)) for n in plan._fields), route
         for n in ("starts", "lengths", "used"):
             assert getattr(plan, n).untyped_storage().nbytes() <= 512, (route, n)
+
+
+def test_a_wrong_length_over_pages_of_one_token():
+    """2^31 - 1 new tokens in a table that holds 3 of them a row: the rest has no entry and takes no time either."""
+    top = 2 ** 31 - 1
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    table = torch.full((3, 3), -7, dtype=torch.int32, device=DEV)
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    for _ in range(2):
+        begin.record()
+        plan = qlin().paged_plan(ints([1, 2, 0]), ints([1, top, 2]), table, ints([10, 11, 12, 13]), 1, 6)
+        end.record()
+    torch.cuda.synchronize()
+    assert table.tolist() == [[-7, 10, -7], [-7, -7, 11], [-1, -1, -7]]
+    assert plan.starts.tolist() == [0, 1, top, top] and plan.used.tolist() == [top] and plan.lengths.tolist() == [2, top, 2]
+    assert plan.slots.tolist() == [10, 11, -1, -1, -1, -1] and plan.rows.tolist() == [0, 1, 1, 1, 1, 1]
+    assert begin.elapsed_time(end) < 50.0
+
+
+@pytest.mark.parametrize("width", [0, 1, 5, 40])
+@pytest.mark.parametrize("page", [1, 3, 16])
+def test_plans_of_rows_that_are_too_short(page, width):
+    import random
+    r = random.Random(page * 100 + width)
+    context, added = [r.randrange(60) for _ in range(70)], [r.choice((0, 1, r.randrange(90))) for _ in range(70)]
+    for pages in (0, 17, 6000):
+        check_plan(context, added, page, width, list(range(1000, 1000 + pages)), sum(added) + 5)
 
 
 def test_second_derivatives():
