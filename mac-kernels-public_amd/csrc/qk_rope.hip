@@ -342,7 +342,8 @@ __global__ __launch_bounds__(THREADS, VEC ? 4 : 1) void head_grad_kernel(HeadGra
     const Shared h = shared_part<PC, VW>(lds, units, cut.tokens);
     fill_weights<PC, VW>(h, units, a.D, a.turn.P, of_k ? a.wk : a.wq, of_k ? a.wk_dt : a.wq_dt, nullptr, 0);
     float dw[PC::N] = {};
-    for (int64_t t0 = (int64_t)part * cut.tokens; t0 < a.T; t0 += (int64_t)parts * cut.tokens) {
+    const int64_t past = heads > 0 ? a.T : 0;  // the one workgroup of a side without heads leaves its sum of zeros at once
+    for (int64_t t0 = (int64_t)part * cut.tokens; t0 < past; t0 += (int64_t)parts * cut.tokens) {
         const int tokens = (int)min<int64_t>(cut.tokens, a.T - t0), end = tokens * heads;
         __syncthreads();
         fill_turns(h, a.turn, t0, tokens);

@@ -197,3 +197,25 @@ def test_frozen_weights_have_no_gradient_formed(monkeypatch):
             out = real(*a, w, w, pos, freq, weight_grads=flags)
             for i in range(2):
                 assert torch.equal(out[2 + i], both[2 + i]) if flags[i] else out[2 + i] is None, (route, flags)
+
+
+def test_the_gradient_of_q_alone_takes_no_longer_than_with_k():
+    Q = qlin()
+    t, h, d = 9504, 40, 128
+    freq, pos = Q.rope_frequencies(d, device=DEV)[0], torch.arange(t, device=DEV)
+    x, g = (torch.randn(t, h, d, device=DEV, dtype=BF16) for _ in range(2))
+    w = torch.ones(d, device=DEV)
+
+    def us(k):
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            Q.qk_norm_rope_grad(g, g if k else None, x, x if k else None, w, w if k else None, pos, freq)
+            b.record()
+            b.synchronize()
+            times.append(1000 * a.elapsed_time(b))
+        return min(times)
+
+    both, alone = us(True), us(False)
+    assert alone < both, (alone, both)
