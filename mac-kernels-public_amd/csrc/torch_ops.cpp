@@ -276,7 +276,10 @@ at::Tensor heads_of(const char* op, const at::Tensor& t, const char* name) {
     if (t.dim() < 3)
         fail(QLIN_EINVAL, std::string(op) + ": " + name + " must be [.., heads, D], it has " + std::to_string(t.dim()) +
                               " dimensions");
-    return dense(t.dim() == 3 ? t : t.reshape({-1, t.size(-2), t.size(-1)}));
+    if (t.dim() == 3) return dense(t);
+    int64_t tokens = 1;  // -1 has no meaning to reshape without values
+    for (int64_t i = 0; i < t.dim() - 2; ++i) tokens *= t.size(i);
+    return dense(t.reshape({tokens, t.size(-2), t.size(-1)}));
 }
 
 at::Tensor packed(const at::Tensor& t, c10::optional<at::ScalarType> dt = c10::nullopt) {

@@ -15,6 +15,7 @@ the kernels do not take raise NoCapableBackendError, malformed ones ValueError, 
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -59,7 +60,7 @@ def _heads(op, t, name):
     """[.., heads, D] as [tokens, heads, D]."""
     if t.dim() < 3:
         raise ValueError(f"{op}: {name} must be [.., heads, D], it has {t.dim()} dimensions")
-    return _dense(t if t.dim() == 3 else t.reshape(-1, *t.shape[-2:]))
+    return _dense(t if t.dim() == 3 else t.reshape(math.prod(t.shape[:-2]), *t.shape[-2:]))  # -1 has no meaning without values
 
 
 def _vector(t, dtype=None):

@@ -105,6 +105,21 @@ def routes(monkeypatch):
     yield "ctypes"
 
 
+def test_no_heads_in_more_dimensions(monkeypatch):
+    Q = qlin()
+    freq, pos, w = torch.ones(32, device=DEV), torch.zeros(6, dtype=torch.int64, device=DEV), torch.ones(64, device=DEV)
+    slots, cache = torch.arange(6, device=DEV), torch.zeros(1, 16, 0, 64, device=DEV)
+    for route in routes(monkeypatch):
+        for hq, hk, d in ((4, 0, 64), (0, 2, 64), (0, 0, 64), (4, 2, 0)):
+            q, k = torch.ones(2, 3, hq, d, device=DEV), torch.ones(2, 3, hk, d, device=DEV)
+            f, v = (freq, w) if d else (freq[:0], w[:0])
+            for got in (Q.axis_rope(q, k, pos, f), Q.qk_norm_rope(q, k, v, v, pos, f),
+                        Q.qk_norm_rope_grad(q, k, q, k, v, v, pos, f)[:2]):
+                assert got[0].shape == q.shape and got[1].shape == k.shape, route
+            if hk == 0:
+                assert Q.qk_norm_rope_store(q, k, k, v, v, pos, f, slots, cache, cache).shape == q.shape
+
+
 def test_a_plan_is_saved_and_its_lengths_kept(monkeypatch):
     """A plan's fields can be saved together, and a field that is kept keeps nothing of the others but their request tables."""
     Q = qlin()
