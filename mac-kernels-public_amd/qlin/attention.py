@@ -215,7 +215,9 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, wi
     like q.  A row without a token gives zeros."""
     op = "paged_attention"
     _disabled(op)
-    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0  # no head size: refused below
+    scale = float(scale)
     if ops._FAST is not None:
         try:
             return ops._FAST.paged_attention(q, k_cache, v_cache, block_table, lengths, scale, int(window), out)

@@ -120,6 +120,17 @@ def test_no_heads_in_more_dimensions(monkeypatch):
                 assert Q.qk_norm_rope_store(q, k, k, v, v, pos, f, slots, cache, cache).shape == q.shape
 
 
+def test_heads_of_no_values_are_refused(monkeypatch):
+    Q = qlin()
+    z = lambda *s: torch.zeros(s, dtype=F16, device=DEV)
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)
+    for _ in routes(monkeypatch):
+        with pytest.raises(Q.NoCapableBackendError):
+            Q.paged_attention(z(2, 8, 0), z(5, 16, 2, 0), z(5, 16, 2, 0), i(2, 4), i(2))
+        with pytest.raises(ValueError):
+            Q.paged_attention(z(), z(5, 16, 2, 64), z(5, 16, 2, 64), i(2, 4), i(2))
+
+
 def test_a_plan_is_saved_and_its_lengths_kept(monkeypatch):
     """A plan's fields can be saved together, and a field that is kept keeps nothing of the others but their request tables."""
     Q = qlin()
