@@ -374,7 +374,7 @@ qlin_status qlin_paged_plan(const qlin_tensor* context, const qlin_tensor* added
  * q, out [rows, heads, D] f16/bf16, any strides with unit stride along D; k_cache, v_cache [blocks, page, kv heads, D] in q's
  * dtype, any strides with unit stride along D; block_table i32 [rows, W], unit column stride, any row stride (0
  * shares one row: the tokens of one prompt are rows with lengths 1, 2, ...); lengths i32 [rows], at most W * page
- * counts.  D a multiple of 8 up to 256, 16-byte aligned rows (QLIN_EUNSUPPORTED otherwise).  A row with no token gives
+ * and 2^31 - 256 count.  D a multiple of 8 up to 256, 16-byte aligned rows (QLIN_EUNSUPPORTED otherwise).  A row with no token gives
  * zeros; a token whose table entry is outside the cache counts as absent.  What the cache holds behind a row's last
  * token is never used, whatever it is.  Scores, their running maximum and sum and the output are fp32.  An infinite value
  * gives its infinity (opposite ones NaN) where its weight is above 2^-39 (f16) or 2^-126 (bf16) of the row's largest, else NaN.

@@ -116,9 +116,10 @@ __device__ __forceinline__ uint32_t divided(uint32_t n, uint64_t magic) {
     return (uint32_t)((hi + (lo >> 32)) >> 32);
 }
 
-// The range of row b's tokens that count.
+// The range of row b's tokens that count, LAST at most: positions of a whole tile behind it stay 32-bit.
+constexpr int64_t LAST = 0x7FFFFF00;
 __device__ __forceinline__ void range_of(const PagedAttentionArgs& a, int length, int& lo, int& hi) {
-    const int64_t n = min((int64_t)max(length, 0), a.W * a.page);
+    const int64_t n = min((int64_t)max(length, 0), min(a.W * a.page, LAST));
     hi = (int)n;
     lo = a.window && n > a.window ? (int)(n - a.window) : 0;
 }
@@ -653,12 +654,12 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
     p.meta = (int4*)ws;
     p.part_ml = (float*)(ws + META_BYTES);
     p.part_o = (float*)(ws + META_BYTES + (heads * 8 + 255) / 256 * 256);
-    int64_t W = a.blocks == 0 ? 0 : std::min<int64_t>(a.W, 0x7FFFFF00 / a.page);  // positions stay 32-bit
+    const int64_t W = a.blocks == 0 ? 0 : std::min<int64_t>(a.W, (LAST + a.page - 1) / a.page), room = std::min(W * a.page, LAST);
     // units a row can have at most
-    int64_t most = (W * a.page + UNIT - 1) / UNIT;
+    int64_t most = (room + UNIT - 1) / UNIT;
     if (a.window) most = std::min<int64_t>(most, a.window / UNIT + 2);
     most = std::max<int64_t>(most, 1);
-    const int64_t longest = a.window ? std::min<int64_t>(W * a.page, a.window + TILE) : W * a.page;
+    const int64_t longest = a.window ? std::min<int64_t>(room, a.window + TILE) : room;
     const int64_t rows = std::min<int64_t>(MAX_ROWS, (1 << 30) / most);  // sums of units stay 32-bit
     for (int64_t b0 = 0; b0 < a.B; b0 += rows) {
         p.a = a;

@@ -245,3 +245,18 @@ def test_the_gradient_of_q_alone_takes_no_longer_than_with_k():
 
     both, alone = us(True), us(False)
     assert alone < both, (alone, both)
+
+
+@pytest.mark.parametrize("page,w", [(1 << 30, 2), (0x7FFFFF80, 1), (100, 0x7FFFFFFF // 100 + 1)])
+def test_positions_to_the_end_of_32_bits(page, w):
+    """A window at the end of a row of 2^30 tokens and more (every place of a block is the same memory)."""
+    d, blocks = 64, 2
+    k, v = (torch.randn(blocks, d, generator=torch.Generator().manual_seed(i)).half().to(DEV) for i in range(2))
+    q = torch.randn(1, 4, d, generator=torch.Generator().manual_seed(2)).half().to(DEV)
+    kc, vc = (x.as_strided((blocks, page, 1, d), (d, 0, d, 1)) for x in (k, v))
+    table = torch.zeros(1, w, dtype=torch.int32, device=DEV)
+    table[0, -1 if w < 8 else -4:] = 1
+    most = 0x7FFFFF00  # positions that a kernel's tiles can count
+    length = (1 << 30) + 5 if w == 2 else most - 3
+    out = qlin().paged_attention(q, kc, vc, table, torch.tensor([length], dtype=torch.int32, device=DEV), window=5)
+    assert torch.equal(out, v[1].expand(1, 4, d))
