@@ -260,3 +260,15 @@ def test_positions_to_the_end_of_32_bits(page, w):
     length = (1 << 30) + 5 if w == 2 else most - 3
     out = qlin().paged_attention(q, kc, vc, table, torch.tensor([length], dtype=torch.int32, device=DEV), window=5)
     assert torch.equal(out, v[1].expand(1, 4, d))
+
+
+def test_more_workgroups_than_a_launch_has_threads_for():
+    """1024 rows of 16640 kv heads are more than 2^24 workgroups of 256 threads."""
+    rows, h, d = 1024, 16640, 8
+    k, v = (torch.randn(1, 8, h, d, generator=torch.Generator(DEV).manual_seed(i), device=DEV).half() for i in range(2))
+    q = torch.randn(rows, h, d, generator=torch.Generator(DEV).manual_seed(2), device=DEV).half()
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(rows, 1)
+    lengths = torch.arange(rows, device=DEV, dtype=torch.int32) % 9
+    out = qlin().paged_attention(q, k, v, table, lengths)
+    some = [0, 1, 7, 8, 9, 500, 1007, 1008, 1023]
+    check(out[some], q[some], k, v, table[some], lengths[some])
