@@ -659,7 +659,7 @@ hipError_t run_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
     int64_t most = (room + UNIT - 1) / UNIT;
     if (a.window) most = std::min<int64_t>(most, a.window / UNIT + 2);
     most = std::max<int64_t>(most, 1);
-    const int64_t longest = a.window ? std::min<int64_t>(room, a.window + TILE) : room;
+    const int64_t longest = a.window ? std::min<int64_t>(room, std::min(a.window, room) + TILE) : room;
     // of one launch: sums of units stay 32-bit, and a workgroup a row and head group below the 2^32 threads of a launch
     const int64_t rows = std::min<int64_t>({MAX_ROWS, (1 << 30) / most, 0xFFFFFFFFll / THREADS / hg});
     for (int64_t b0 = 0; b0 < a.B; b0 += rows) {

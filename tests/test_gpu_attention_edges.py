@@ -272,3 +272,11 @@ def test_more_workgroups_than_a_launch_has_threads_for():
     out = qlin().paged_attention(q, k, v, table, lengths)
     some = [0, 1, 7, 8, 9, 500, 1007, 1008, 1023]
     check(out[some], q[some], k, v, table[some], lengths[some])
+
+
+def test_a_window_past_every_length_is_none():
+    """Up to the largest number there is: the same kernel, so the same bits."""
+    s = make([1000, 1024, 3, 777] * 16, 8, 8, 128, 16, BF16)
+    want = qlin().paged_attention(*s)
+    for window in (1024, 1 << 40, 2 ** 63 - 1):
+        assert torch.equal(qlin().paged_attention(*s, window=window), want), window
