@@ -364,7 +364,8 @@ qlin_status qlin_qk_norm_rope_grad(const qlin_tensor* dq_out, const qlin_tensor*
  * (i32, i32, i64 [N], N >= the new tokens; the places behind the last token get -1 in all three, new
  * tokens behind N get no place).  starts i32 [B + 1]: the running sum of added; lengths i32 [B]: context + added; used
  * i32 [1]: the pages that the step needs.  When used > F the free list was too short: pages past it are
- * -1 in the table and so are their tokens' slots; the same for pages past W, which have no entry. */
+ * -1 in the table and so are their tokens' slots; the same for pages past W, which have no entry.  What is
+ * written shares no memory with anything else of the call (QLIN_EINVAL): lengths is not context in place. */
 qlin_status qlin_paged_plan(const qlin_tensor* context, const qlin_tensor* added, const qlin_tensor* free_blocks,
                             int64_t page, qlin_tensor* block_table, qlin_tensor* slots, qlin_tensor* positions,
                             qlin_tensor* rows, qlin_tensor* starts, qlin_tensor* lengths, qlin_tensor* used, void* stream);

@@ -83,6 +83,27 @@ qlin_status vector_of(const qlin_tensor* t, const char* name, int64_t n, int dty
     return QLIN_OK;
 }
 
+// Memory of rows of `width` bytes, `step` apart; a vector is one row.
+struct Range {
+    const char* name;
+    uintptr_t p;
+    int64_t width, rows, step;
+};
+
+Range range_of(const qlin_tensor* t, const char* name, int es) {
+    if (t->ndim == 1) return {name, (uintptr_t)t->data, t->shape[0] * es, 1, 0};
+    return {name, (uintptr_t)t->data, t->shape[1] * es, t->shape[0], step(t, 0) * es};
+}
+
+// Whether the vector v and the rows r share a byte.
+bool share_memory(const Range& v, const Range& r) {
+    if (v.width == 0 || r.width == 0 || r.rows == 0) return false;
+    if (v.p + v.width <= r.p || v.p >= r.p + (r.rows - 1) * r.step + r.width) return false;
+    if (v.p < r.p || r.rows == 1) return true;
+    const int64_t at = (int64_t)(v.p - r.p), in = at % r.step;
+    return in < r.width || (in + v.width > r.step && at / r.step + 1 < r.rows);
+}
+
 qlin_status turn_of(const qlin_tensor* positions, const qlin_tensor* inv_freq, const qlin_tensor* axis, int flags, int64_t T,
                     int64_t D, RopeTurn& r) {
     if (flags & ~(QLIN_ROPE_INTERLEAVED | QLIN_ROPE_INVERSE)) return fail(QLIN_EINVAL, "unknown flags %d", flags);
@@ -286,6 +307,17 @@ qlin_status qlin_paged_plan(const qlin_tensor* context, const qlin_tensor* added
     if (qlin_status s = vector_of(starts, "starts", B + 1, QLIN_DT_I32)) return s;
     if (qlin_status s = vector_of(lengths, "lengths", B, QLIN_DT_I32)) return s;
     if (qlin_status s = vector_of(used, "used", 1, QLIN_DT_I32)) return s;
+    // workgroups read the inputs while others write: what is written is nothing else's memory
+    const Range table = range_of(block_table, "block_table", 4);
+    const Range vectors[] = {range_of(context, "context", 4), range_of(added, "added", 4), range_of(free_blocks, "free_blocks", 4),
+                             range_of(slots, "slots", 8), range_of(positions, "positions", 4), range_of(rows, "rows", 4),
+                             range_of(starts, "starts", 4), range_of(lengths, "lengths", 4), range_of(used, "used", 4)};
+    for (int i = 0; i < 9; ++i) {
+        if (share_memory(vectors[i], table)) return fail(QLIN_EINVAL, "%s and block_table share memory", vectors[i].name);
+        for (int j = 3; j < 9; ++j)
+            if (i != j && share_memory(vectors[i], vectors[j]))
+                return fail(QLIN_EINVAL, "%s and %s share memory", vectors[i].name, vectors[j].name);
+    }
     a.B = (int)B;
     a.context = (const int32_t*)context->data; a.added = (const int32_t*)added->data;
     a.free_blocks = (const int32_t*)free_blocks->data; a.table = (int32_t*)block_table->data;
