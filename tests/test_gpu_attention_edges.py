@@ -247,6 +247,29 @@ def test_the_gradient_of_q_alone_takes_no_longer_than_with_k():
     assert alone < both, (alone, both)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", ["token", "head"])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", [
+    ([4097, 20, 9000], 16, 1, 128, 16),    # split and joined
+    ([3000, 5], 17, 1, 64, 16),            # two groups of a kv head, 9 and 8 heads
+    ([3000, 70], 49, 1, 128, 16),          # four, the last one short
+    ([300, 2000], 16, 1, 256, 16),
+    ([300, 2000], 12, 1, 256, 100),
+    ([257, 3000], 16, 1, 128, 12),
+    ([100, 31], 34, 2, 64, 7),
+])
+def test_many_heads_of_a_kv_head(lengths, heads, kv_heads, dim, page, layout, dtype):
+    s = make(lengths, heads, kv_heads, dim, page, dtype, layout)
+    check(qlin().paged_attention(*s), *s)
+    check(qlin().paged_attention(*s, window=290), *s, window=290)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_many_short_rows_of_many_heads(dtype):
+    s = make([(i * 53) % 120 for i in range(300)], 64, 4, 256, 16, dtype)
+    check(qlin().paged_attention(*s), *s)
+
+
 @pytest.mark.parametrize("page,w", [(1 << 30, 2), (0x7FFFFF80, 1), (100, 0x7FFFFFFF // 100 + 1)])
 def test_positions_to_the_end_of_32_bits(page, w):
     """A window at the end of a row of 2^30 tokens and more (every place of a block is the same memory)."""
