@@ -22,14 +22,15 @@
 // workgroup takes an equal run of them, as many workgroups as the chip holds at once.  So one long row among short ones
 // is spread like the rest, and the host need not know the lengths: every workgroup forms the running sum from them.
 // A row that crosses from one workgroup's run into the next leaves its parts as (O, m, l) in fp32, and a second
-// kernel joins them.  Where the table has no room for long rows, a workgroup takes one row (whole_rows()).
+// kernel joins them.  Where the table has no room for rows longer than whole_rows(), a workgroup takes one row, whatever the
+// others have.
 //
-// Measured on one MI355X (calls back to back, bytes of the cache over the whole call): 1 row of 131071 tokens, 40 heads
-// over 8 of 128 values 90 us, 6.0 TB/s; 64 rows of 100 to 16384, 32 over 8 142 us, 6.1 TB/s; 8 rows of 3000 to 4096 28.7 us,
-// 4.0 TB/s, of which the first loads take some 5 us and the second kernel with its launch 6; 1 row of 77 6.3 us.  Tried
-// and slower: more workgroups than the chip holds, a join by the last workgroup (its agent fences write back and drop
-// the L2: 105 us for the 8 rows), 3 waves a SIMD (spills), the next row's loads before this row's join, loads without
-// branches around them (the waits are exact then; 3% faster for 64 values, 2 to 5% slower for 128).
+// Measured on one MI355X (calls back to back, inputs that are not in the caches, bytes of the cache over the whole call):
+// 1 row of 131071 tokens, 40 heads over 8 of 128 values 89 us, 6.0 TB/s; 64 rows of 100 to 16384, 32 over 8 141 us, 6.1 TB/s;
+// 8 rows of 3000 to 4096 29.0 us, 4.0 TB/s, of which the first loads take some 5 us and the second kernel with its launch 6;
+// 1 row of 77 5.6 us.  Tried and slower: more workgroups than the chip holds, a join by the last workgroup (its agent fences
+// write back and drop the L2: 105 us for the 8 rows), 3 waves a SIMD (spills), the next row's loads before this row's join, loads
+// without branches around them (the waits are exact then; 3% faster for 64 values, 2 to 5% slower for 128).
 #include "attention.h"
 
 namespace qlin {
@@ -48,18 +49,20 @@ constexpr int MOST_GROUPS = 4 * CUS;  // of any head size: see held()
 int64_t held(int64_t D, bool wide) { return CUS * (D <= 64 ? wide ? 3 : 4 : D <= 128 ? 2 : 1); }
 
 // Units up to which rows are not split: a workgroup takes one whole row, without the running sum and the second kernel.
-// Where that fills the chip rows may be longer.  Measured, not split / split (us, 8 kv heads; 1 unit = 128 tokens):
-// D = 128, 1 row of 4 units 10.5 / 12.9, of 8 15.5 / 12.4; 64 rows of 4 21.4 / 27.0, of 8 39.5 / 44.7, of 16 73.6 / 75.0;
-// D = 64, 8 rows of 4 10.1 / 12.4, of 8 15.8 / 13.2; 64 rows of 16 43.3 / 48.7; D = 256, 8 rows of 2 11.9 / 15.1, of 4
-// 18.2 / 16.3; 64 rows of 8 71.0 / 72.2, of 16 128 / 123.
+// Where that fills the chip rows may be longer.  Measured on equal rows that are not in the caches, not split / split (us, 32
+// over 8 heads; 1 unit = 128 tokens): D = 128, 1 row of 2 units 8.2 / 11.5, of 4 12.3 / 11.9, of 6 15.9 / 12.1; 64 rows of 4
+// 27.6 / 30.0, of 8 49.1 / 51.7, of 16 93.1 / 96.0, of 24 137 / 140; D = 64, 8 rows of 4 10.9 / 11.7, of 8 17.2 / 13.2; 64 rows of 16
+// 52.5 / 61.7, of 32 100 / 114; D = 256, 8 rows of 2 12.9 / 15.3, of 4 18.7 / 17.0; 64 rows of 8 88.1 / 89.0, of 16 165 / 166.
+// The host knows the table's room alone, and unequal rows lose by it: D = 128, one row of 1024 tokens among 63 of 60 20.2 /
+// 18.4, of 2048 34.5 / 19.2.
 int64_t whole_rows(int64_t D, int64_t workgroups) {
     return workgroups >= 2 * CUS ? std::min<int64_t>(16, 2048 / D) : D <= 128 ? 4 : 2;
 }
 
 // Whether whole rows of at most `longest` tokens take a wave each instead of a workgroup of four: many rows that leave some
-// of four waves without a tile.  Measured, one wave / four (us, 8 kv heads of 128 values): 200 rows of 30 tokens 8.9 / 19.1,
-// of 60 12.1 / 19.8, of 120 17.7 / 23.1, of 250 31.2 / 38.2, of 500 59.5 / 61.8; 64 rows of 60 8.0 / 8.1, of 120 11.1 / 10.2,
-// of 250 17.1 / 13.7; of 256 values, 64 rows of 120 17.5 / 18.9, of 250 25.7 / 26.0.
+// of four waves without a tile.  Measured as above, one wave / four (us, 8 kv heads of 128 values): 200 rows of 30 tokens 8.9 /
+// 19.5, of 60 13.8 / 21.4, of 120 22.6 / 28.7, of 250 40.7 / 46.0, of 500 76.2 / 80.6; 64 rows of 60 7.9 / 8.0, of 120 12.4 / 10.6,
+// of 250 20.7 / 16.0; of 256 values, 64 rows of 120 19.2 / 21.7, of 250 29.7 / 31.3; of 64, 300 rows of 60 11.7 / 16.0.
 bool one_wave_rows(int64_t D, int64_t longest, int64_t workgroups) {
     return longest <= 512 && 2 * workgroups >= held(D, false) * (longest <= 64 ? 2 : longest <= 128 ? 3 : 6);
 }

@@ -432,11 +432,11 @@ bool aligned(const void* p, std::initializer_list<int64_t> strides, int es, int 
 // else 8 value by value.  Vectors of interleaved pairs hold whole pairs whatever P is.
 //
 // Rows of more than MUCH bytes in all are read nontemporally: what they would take of the caches is left to the outputs,
-// which the next kernel reads.  Measured with a kernel that writes the rows before and one that reads the outputs after
-// (us, all three; nontemporal / not): 9504 tokens x 80 heads of 128 (195 MB) 234 / 245, 4608 x 96 (113) 137 / 150, 4095 x 48
-// (50) 58.0 / 58.4, 1056 x 96 (26) 36.8 / 36.8; the gradient 244 / 264, 145 / 159, -, 50.5 / 49.6; a forward
-// call and its gradient on 1056 x 96 at once, which read the same rows, 44.8 / 41.3.  Nontemporal stores gain nothing there:
-// 245, 139, 63.
+// which the next kernel reads.  Measured between a kernel that writes the rows and one that reads the outputs (us, all three;
+// nontemporal / not): 9504 tokens x 80 heads of 128 (195 MB) 186 / 202, 4608 x 96 (113) 109 / 108, 6000 x 40 (61) 65.3 / 65.8, 3000 x
+// 128 of 64 (49) 54.3 / 53.3, 1056 x 96 (26) 32.2 / 32.6; the gradient 228 / 257, 139 / 144, 89.4 / 87.7, 74.7 / 70.7, 48.6 / 45.3.  Rows
+// that come from memory, normalized into a cache: 4095 x 48 of 128 (50) 23.7 / 25.2.  So 32 to 64 MB gain or lose by up to 6%
+// with what is around them; below, plain loads win, above, the others.  Nontemporal stores gain nothing.
 constexpr int64_t MUCH = 32 << 20;
 
 struct Kind {
@@ -530,8 +530,9 @@ hipError_t run_head_rope(const HeadRopeArgs& a, hipStream_t st) {
     Cut c = cut_of(k, a.D, a.Hq + a.Hk + (a.store ? a.Hk : 0));
     // Equal runs of rows, in whole rounds of the lane groups: a small call is spread over the chip, a row a lane group; a
     // large one over WORKGROUPS at a time, which share a token's cosines among up to 5 rounds.  Measured (us, at
-    // most 3 / 5 / 8 / 16 rounds): 4095 tokens x 56 rows into a cache 29.7 / 26.4 / 26.8 / 26.1, 4608 x 96 41.5 /
-    // 41.1 / 46.4 / 46.4, 9504 x 80 75.1 / 76.9 / 80.5 / 91.5.
+    // most 3 / 5 / 8 / 16 rounds): 4095 tokens x 56 rows into a cache 29.7 / 26.4 / 26.8 / 26.1, 4608 x 96 40.9 /
+    // 40.3 / 47.4 / 47.2, 9504 x 80 66.9 / 65.0 / 67.3 / 76.7, 5000 x 20 of 256 values 25.4 / 23.7 / 23.7 / 23.7, 6000 x 40 27.2 / 27.9 /
+    // 27.9 / 27.8, 3000 x 128 of 64 25.5 / 25.6 / 25.6 / 25.5.
     const int64_t groups = THREADS / c.lanes, rows = a.T * c.heads, round = groups * WORKGROUPS;
     const int64_t times = std::max<int64_t>(1, (rows + MOST_ROUNDS * round - 1) / (MOST_ROUNDS * round));
     int64_t span = std::max<int64_t>(1, (rows + times * round - 1) / (times * round)) * groups;
