@@ -70,6 +70,8 @@ typedef enum {
     QLIN_OP_GGUF_LINEAR_LORA = 11,     /* qlin_gguf_linear_lora: param = the ggml type | R << 8 */
     QLIN_OP_QK_NORM_ROPE_GRAD = 12,    /* qlin_qk_norm_rope_grad: M tokens, N heads of q and k together, K the head size */
     QLIN_OP_PAGED_ATTENTION = 13,      /* qlin_paged_attention: M rows, N query heads, K the head size, param = kv heads */
+    QLIN_OP_ADD_RMS_NORM_GRAD = 14,    /* qlin_add_rms_norm_grad: M rows, K values a row (N, param unused) */
+    QLIN_OP_W8A8_LINEAR = 15,          /* qlin_w8a8_linear: param = QLIN_W8A8_X_ROWS | QLIN_W8A8_W_ROWS as they apply */
 } qlin_op;
 
 /* ggml type ids accepted by the GGUF entry points (enum ggml_type). */
@@ -383,6 +385,64 @@ qlin_status qlin_paged_plan(const qlin_tensor* context, const qlin_tensor* added
 qlin_status qlin_paged_attention(const qlin_tensor* q, const qlin_tensor* k_cache, const qlin_tensor* v_cache,
                                  const qlin_tensor* block_table, const qlin_tensor* lengths, float scale, int64_t window,
                                  qlin_tensor* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * The MLP side of a block: the norm before its first linear, the product of int8 rows, the gated activation between the
+ * two linears.  Row tensors are [rows, values], unit stride along a row, any row stride and alignment; outputs' rows
+ * do not overlap.  Everything is computed in fp32 and rounded once.  An output may be one of the call's inputs
+ * (the same memory and strides); it may not overlap one otherwise.
+ *
+ * 8-bit outputs: with v the row's values (rotated by the ConvRot group first, convrot_groupsize 0: not) and top their largest
+ * magnitude, scale = top / 127 and q = rne(127 v / top), ties to even; a row of zeros has scale 0 and codes 0.  A row
+ * with an infinity or a NaN has a scale that is not finite, which makes every output of a linear over it NaN or infinite.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* h = x + residual, y = weight * h / rms(h), rms(h) = sqrt(mean(h^2) + eps) over the row.  The norm is that of the unrounded
+ * sum.  x, y f32/f16/bf16 of one dtype; residual, h of x's dtype or f32 (both NULL: h is x); weight optional
+ * (NULL = 1) f32/f16/bf16 [values].  Rows of up to 2^20 values. */
+qlin_status qlin_add_rms_norm(const qlin_tensor* x, const qlin_tensor* residual, const qlin_tensor* weight, float eps,
+                              qlin_tensor* y, qlin_tensor* h, void* stream);
+
+/* The same with y in 8 bits: q i8 [rows, values], scale f32 [rows] or [rows, 1]. */
+qlin_status qlin_add_rms_norm_int8(const qlin_tensor* x, const qlin_tensor* residual, const qlin_tensor* weight, float eps,
+                                   int convrot_groupsize, qlin_tensor* q, qlin_tensor* scale, qlin_tensor* h, void* stream);
+
+/* Gradients of qlin_add_rms_norm from those of y and h (dh NULL: none reaches h): with rho = 1 / rms(h) and g = weight dy,
+ *   dx = rho (g - h rho^2 mean(g h)) + dh,  which is x's and the residual's gradient both, in h's dtype,
+ *   dweight = sum over rows of dy h rho     (NULL: not formed; f32/f16/bf16 [values], summed in fp32 in a fixed order).
+ * h is the forward call's (x itself where it had no residual); dy in x's dtype; dh, dx in h's.
+ * Workspace (only with dweight): qlin_workspace_size(QLIN_OP_ADD_RMS_NORM_GRAD, rows, 0, values, 0, dy's dtype). */
+qlin_status qlin_add_rms_norm_grad(const qlin_tensor* dy, const qlin_tensor* dh, const qlin_tensor* h, const qlin_tensor* weight,
+                                   float eps, qlin_tensor* dx, qlin_tensor* dweight, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* f(z) = z / (1 + exp(-t)): t = z, or t = 2 sqrt(2/pi) (z + 0.044715 z^3), which is GELU in its tanh form. */
+enum { QLIN_ACT_SILU = 0, QLIN_ACT_GELU_TANH = 1 };
+
+/* y = f(gate) * up (up NULL: f(gate)), all f32/f16/bf16 of one dtype; the halves of a fused projection's rows go in as they
+ * are.  Rows of up to 2^20 values. */
+qlin_status qlin_gated_act(const qlin_tensor* gate, const qlin_tensor* up, int act, qlin_tensor* y, void* stream);
+
+/* The same with y in 8 bits: q i8 [rows, values], scale f32 [rows] or [rows, 1]. */
+qlin_status qlin_gated_act_int8(const qlin_tensor* gate, const qlin_tensor* up, int act, int convrot_groupsize, qlin_tensor* q,
+                                qlin_tensor* scale, void* stream);
+
+/* dgate = dy up f'(gate), dup = dy f(gate) (up and dup NULL: dgate = dy f'(gate)), all of gate's dtype. */
+qlin_status qlin_gated_act_grad(const qlin_tensor* dy, const qlin_tensor* gate, const qlin_tensor* up, int act,
+                                qlin_tensor* dgate, qlin_tensor* dup, void* stream);
+
+/* qlin_workspace_size's param for QLIN_OP_W8A8_LINEAR: operands that are copied to rows of their own first, because their
+ * rows are not 16-byte aligned, or (the weights') not one behind the other.  Counted anyway when K is not a multiple of 128. */
+enum { QLIN_W8A8_X_ROWS = 1, QLIN_W8A8_W_ROWS = 2 };
+
+/* y[m,n] = x_scale[m] * scale[n] * sum_k x[m,k] qdata[n,k] + bias[n], then (with residual) residual[m,n] + residual_scale[n] *
+ * that; one rounding.  x i8 [M, K] with x_scale f32 [M] or [M, 1], as qlin_quantize_act_int8, qlin_add_rms_norm_int8
+ * and qlin_gated_act_int8 give them; qdata i8 [N, K] with scale f32 [N] or [N, 1]; bias optional f32/f16/bf16 [N];
+ * residual optional f32/f16/bf16 [M, N], residual_scale optional (NULL = 1) f32/f16/bf16 [N]; y f32/f16/bf16 [M, N].
+ * The int32 sums are exact: K up to 131071.  Workspace: qlin_workspace_size(QLIN_OP_W8A8_LINEAR, M, N, K, param, 0). */
+qlin_status qlin_w8a8_linear(const qlin_tensor* x, const qlin_tensor* x_scale, const qlin_tensor* qdata, const qlin_tensor* scale,
+                             const qlin_tensor* bias, const qlin_tensor* residual, const qlin_tensor* residual_scale,
+                             qlin_tensor* y, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

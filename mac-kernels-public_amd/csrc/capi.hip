@@ -12,6 +12,7 @@
 #include "gguf_exact.h"
 #include "qlin_internal.h"
 #include "attention.h"
+#include "mlp.h"
 
 using namespace qlin;
 
@@ -387,6 +388,8 @@ size_t qlin_workspace_size(int op, int64_t M, int64_t N, int64_t K, int param, i
             return ws_gguf(M, N, K, param) + ws_gguf_decoded(M, N, K, param) + align_up((size_t)(M * N * 4)) + 256;
         case QLIN_OP_QK_NORM_ROPE_GRAD: return ws_head_grad(M, N, K);
         case QLIN_OP_PAGED_ATTENTION: return ws_paged_attention(M, N, param, K);
+        case QLIN_OP_ADD_RMS_NORM_GRAD: return ws_add_norm_grad(M, K);
+        case QLIN_OP_W8A8_LINEAR: return ws_w8a8(M, N, K, param);
         case QLIN_OP_LORA: {  // the split partials, then their sum
             const int S = lora_splits(M, K, param);
             return align_up((size_t)(S > 1 ? S + 1 : 1) * M * (size_t)(param > 0 ? param : 0) * 4);

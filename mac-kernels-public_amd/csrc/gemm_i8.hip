@@ -14,6 +14,7 @@
 #include "lora_frag.h"
 #include "prologue_dev.h"
 #include "gemm_pp.h"
+#include "mlp.h"
 
 namespace qlin {
 namespace {
@@ -1293,6 +1294,80 @@ inline bool a8_takes_decode_once(const GemmI8Args& p) {
            (uintptr_t)p.xq % 16 == 0 && (uintptr_t)p.w8 % 16 == 0;
 }
 
+// The GEMM over the int8 weight grid p.w8, as it was decoded or as it is stored.
+hipError_t launch_dense(const GemmI8Args& p, hipStream_t st) {
+    auto tiles = [&](int bm, int bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+    // LoRA term in the epilogue by up dtype (none: -1)
+    const int ldu = !p.lora.t ? -1 : p.lora.up_dt;
+    auto go = [&]<int BMV, int BNV>() {
+        const dim3 grid((unsigned)tiles(BMV, BNV));
+        switch (ldu) {
+            case -1: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false>), grid, dim3(512), 0, st, p, p.w8); break;
+            case DT_BF16: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false, DT_BF16>), grid, dim3(512), 0, st, p, p.w8); break;
+            case DT_F16: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false, DT_F16>), grid, dim3(512), 0, st, p, p.w8); break;
+            case DT_F32: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false, DT_F32>), grid, dim3(512), 0, st, p, p.w8); break;
+        }
+    };
+    if (ldu != -1 && ldu != DT_BF16 && ldu != DT_F16 && ldu != DT_F32) return hipErrorInvalidValue;
+    // the two-group loop from K = 3584: its first loads and its 128 KiB per workgroup are not overlapped with
+    // another tile's work, and short rows do not win that back (us, without and with it: M9504 K1024 N16384 262,
+    // 312; M7000 K1536 N12288 197, 217; M8192 K2048 N16384 336, 349; M4608 K3072 N9216 167, 168; M4096 K4096
+    // N8192 157, 153; M2500 K5120 N13824 241, 219; M1500 K16384 N8192 259, 222)
+    const bool pp = p.K >= 3584;
+    const int64_t m1 = ldu == -1 && tiles(256, 256) >= 192 ? tail_split_rows(p.M, p.N) : 0;
+    if (m1) {  // whole rounds of 256 x 256 tiles, then the rest as one round of 128-row tiles
+        GemmI8Args top = p, rest = p;
+        top.M = m1;
+        rest.M = p.M - m1;
+        rest.xq = p.xq + m1 * p.ldx;
+        rest.sx = p.sx + m1;
+        rest.y = (uint8_t*)p.y + m1 * p.ldy * dt_bytes(p.y_dtype);
+        if (p.res.r) rest.res.r = (const uint8_t*)p.res.r + m1 * p.res.ldr * dt_bytes(p.res.r_dt);
+        auto tiles_of = [](const GemmI8Args& g, int bm) { return ((g.M + bm - 1) / bm) * ((g.N + 255) / 256); };
+        if (pp) hipLaunchKernelGGL(gemm_i8pp_kernel<>, dim3((unsigned)tiles_of(top, 256)), dim3(512), 0, st, top, top.w8);
+        else hipLaunchKernelGGL((gemm_i8dma_kernel<256, 256, 128, 2, false>), dim3((unsigned)tiles_of(top, 256)), dim3(512), 0, st, top, top.w8);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+        // the narrowest tiles that still run in one round: a rest of few rows is bound by how many CUs share
+        // out the weights (the W6A8 MLP at 9504 rows, last 32 rows of N 13824: the two calls 1412 -> 1384 us)
+        auto rest_tiles = [&](int bn) { return ((rest.M + 127) / 128) * ((rest.N + bn - 1) / bn); };
+        if (rest_tiles(64) <= 256)
+            hipLaunchKernelGGL((gemm_i8dma_kernel<128, 64, 128, 2, false>), dim3((unsigned)rest_tiles(64)), dim3(512), 0, st, rest, rest.w8);
+        else if (rest_tiles(128) <= 256)
+            hipLaunchKernelGGL((gemm_i8dma_kernel<128, 128, 128, 2, false>), dim3((unsigned)rest_tiles(128)), dim3(512), 0, st, rest, rest.w8);
+        else
+            hipLaunchKernelGGL((gemm_i8dma_kernel<128, 256, 128, 2, false>), dim3((unsigned)rest_tiles(256)), dim3(512), 0, st, rest, rest.w8);
+        return hipGetLastError();
+    }
+    if (tiles(256, 256) >= 192 && !pp) {
+        go.template operator()<256, 256>();
+    } else if (tiles(256, 256) >= 192) {
+        const dim3 grid((unsigned)tiles(256, 256));
+        switch (ldu) {
+            case -1: hipLaunchKernelGGL(gemm_i8pp_kernel<>, grid, dim3(512), 0, st, p, p.w8); break;
+            case DT_BF16: hipLaunchKernelGGL(gemm_i8pp_kernel<DT_BF16>, grid, dim3(512), 0, st, p, p.w8); break;
+            case DT_F16: hipLaunchKernelGGL(gemm_i8pp_kernel<DT_F16>, grid, dim3(512), 0, st, p, p.w8); break;
+            case DT_F32: hipLaunchKernelGGL(gemm_i8pp_kernel<DT_F32>, grid, dim3(512), 0, st, p, p.w8); break;
+        }
+    }
+    // 128 x 160 tiles (2 x 5 waves, no LoRA term) when they make one round of at least 3/4 of
+    // the 256 CUs and 256 x 256 tiles would not fill the GPU (M1024 N5120: 256 of them)
+    else if (ldu == -1 && tiles(128, 160) >= 192 && tiles(128, 160) <= 256) {
+        const dim3 grid((unsigned)tiles(128, 160));
+        hipLaunchKernelGGL((gemm_i8dma_kernel<128, 160, 128, 2, false, -1, 2, 5>), grid,
+                           dim3(i8dma_threads<2, 5>()), 0, st, p, p.w8);
+    }
+    // 128 x 256 also when it fits one round on the 256 CUs and 128 x 128 would not: one round of
+    // the larger tile beats 1.25 rounds of the smaller (M1024 K13824 N5120: 150.6 vs 157.1 us)
+    else if (tiles(128, 256) >= 192 || (tiles(128, 256) <= 256 && tiles(128, 128) > 256))
+        go.template operator()<128, 256>();
+    else if (tiles(128, 128) >= 128)
+        go.template operator()<128, 128>();
+    else  // grids of fewer than 128 tiles of 128 x 128 (a few hundred rows): twice the workgroups
+        go.template operator()<128, 64>();
+    return hipGetLastError();
+}
+
 template <int BITS, bool CB, typename TSrel>
 hipError_t launch_o(const GemmI8Args& p, hipStream_t st) {
     if (p.y_dtype != DT_F32 && p.y_dtype != DT_F16 && p.y_dtype != DT_BF16) return hipErrorInvalidValue;
@@ -1313,76 +1388,7 @@ hipError_t launch_o(const GemmI8Args& p, hipStream_t st) {
             hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
         }
-        auto tiles = [&](int bm, int bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-        // LoRA term in the epilogue by up dtype (none: -1)
-        const int ldu = !p.lora.t ? -1 : p.lora.up_dt;
-        auto go = [&]<int BMV, int BNV>() {
-            const dim3 grid((unsigned)tiles(BMV, BNV));
-            switch (ldu) {
-                case -1: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false>), grid, dim3(512), 0, st, p, p.w8); break;
-                case DT_BF16: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false, DT_BF16>), grid, dim3(512), 0, st, p, p.w8); break;
-                case DT_F16: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false, DT_F16>), grid, dim3(512), 0, st, p, p.w8); break;
-                case DT_F32: hipLaunchKernelGGL((gemm_i8dma_kernel<BMV, BNV, 128, 2, false, DT_F32>), grid, dim3(512), 0, st, p, p.w8); break;
-            }
-        };
-        if (ldu != -1 && ldu != DT_BF16 && ldu != DT_F16 && ldu != DT_F32) return hipErrorInvalidValue;
-        // the two-group loop from K = 3584: its first loads and its 128 KiB per workgroup are not overlapped with
-        // another tile's work, and short rows do not win that back (us, without and with it: M9504 K1024 N16384 262,
-        // 312; M7000 K1536 N12288 197, 217; M8192 K2048 N16384 336, 349; M4608 K3072 N9216 167, 168; M4096 K4096
-        // N8192 157, 153; M2500 K5120 N13824 241, 219; M1500 K16384 N8192 259, 222)
-        const bool pp = p.K >= 3584;
-        const int64_t m1 = ldu == -1 && tiles(256, 256) >= 192 ? tail_split_rows(p.M, p.N) : 0;
-        if (m1) {  // whole rounds of 256 x 256 tiles, then the rest as one round of 128-row tiles
-            GemmI8Args top = p, rest = p;
-            top.M = m1;
-            rest.M = p.M - m1;
-            rest.xq = p.xq + m1 * p.ldx;
-            rest.sx = p.sx + m1;
-            rest.y = (uint8_t*)p.y + m1 * p.ldy * dt_bytes(p.y_dtype);
-            if (p.res.r) rest.res.r = (const uint8_t*)p.res.r + m1 * p.res.ldr * dt_bytes(p.res.r_dt);
-            auto tiles_of = [](const GemmI8Args& g, int bm) { return ((g.M + bm - 1) / bm) * ((g.N + 255) / 256); };
-            if (pp) hipLaunchKernelGGL(gemm_i8pp_kernel<>, dim3((unsigned)tiles_of(top, 256)), dim3(512), 0, st, top, top.w8);
-            else hipLaunchKernelGGL((gemm_i8dma_kernel<256, 256, 128, 2, false>), dim3((unsigned)tiles_of(top, 256)), dim3(512), 0, st, top, top.w8);
-            const hipError_t err = hipGetLastError();
-            if (err != hipSuccess) return err;
-            // the narrowest tiles that still run in one round: a rest of few rows is bound by how many CUs share
-            // out the weights (the W6A8 MLP at 9504 rows, last 32 rows of N 13824: the two calls 1412 -> 1384 us)
-            auto rest_tiles = [&](int bn) { return ((rest.M + 127) / 128) * ((rest.N + bn - 1) / bn); };
-            if (rest_tiles(64) <= 256)
-                hipLaunchKernelGGL((gemm_i8dma_kernel<128, 64, 128, 2, false>), dim3((unsigned)rest_tiles(64)), dim3(512), 0, st, rest, rest.w8);
-            else if (rest_tiles(128) <= 256)
-                hipLaunchKernelGGL((gemm_i8dma_kernel<128, 128, 128, 2, false>), dim3((unsigned)rest_tiles(128)), dim3(512), 0, st, rest, rest.w8);
-            else
-                hipLaunchKernelGGL((gemm_i8dma_kernel<128, 256, 128, 2, false>), dim3((unsigned)rest_tiles(256)), dim3(512), 0, st, rest, rest.w8);
-            return hipGetLastError();
-        }
-        if (tiles(256, 256) >= 192 && !pp) {
-            go.template operator()<256, 256>();
-        } else if (tiles(256, 256) >= 192) {
-            const dim3 grid((unsigned)tiles(256, 256));
-            switch (ldu) {
-                case -1: hipLaunchKernelGGL(gemm_i8pp_kernel<>, grid, dim3(512), 0, st, p, p.w8); break;
-                case DT_BF16: hipLaunchKernelGGL(gemm_i8pp_kernel<DT_BF16>, grid, dim3(512), 0, st, p, p.w8); break;
-                case DT_F16: hipLaunchKernelGGL(gemm_i8pp_kernel<DT_F16>, grid, dim3(512), 0, st, p, p.w8); break;
-                case DT_F32: hipLaunchKernelGGL(gemm_i8pp_kernel<DT_F32>, grid, dim3(512), 0, st, p, p.w8); break;
-            }
-        }
-        // 128 x 160 tiles (2 x 5 waves, no LoRA term) when they make one round of at least 3/4 of
-        // the 256 CUs and 256 x 256 tiles would not fill the GPU (M1024 N5120: 256 of them)
-        else if (ldu == -1 && tiles(128, 160) >= 192 && tiles(128, 160) <= 256) {
-            const dim3 grid((unsigned)tiles(128, 160));
-            hipLaunchKernelGGL((gemm_i8dma_kernel<128, 160, 128, 2, false, -1, 2, 5>), grid,
-                               dim3(i8dma_threads<2, 5>()), 0, st, p, p.w8);
-        }
-        // 128 x 256 also when it fits one round on the 256 CUs and 128 x 128 would not: one round of
-        // the larger tile beats 1.25 rounds of the smaller (M1024 K13824 N5120: 150.6 vs 157.1 us)
-        else if (tiles(128, 256) >= 192 || (tiles(128, 256) <= 256 && tiles(128, 128) > 256))
-            go.template operator()<128, 256>();
-        else if (tiles(128, 128) >= 128)
-            go.template operator()<128, 128>();
-        else  // grids of fewer than 128 tiles of 128 x 128 (a few hundred rows): twice the workgroups
-            go.template operator()<128, 64>();
-        return hipGetLastError();
+        return launch_dense(p, st);
     }
     // large tiles when the grid still fills the GPU and one scale covers each row's k-tile
     const int64_t big_tiles = ((p.N + 255) / 256) * ((p.M + 255) / 256);
@@ -1501,6 +1507,12 @@ hipError_t run_a8_prepass(const PrologueArgs& a, const GemmI8Args& p, hipStream_
         return a.G == 128 ? by_slots.template operator()<TIn, 128>() : by_slots.template operator()<TIn, 256>();
     };
     return a.x_dtype == DT_F16 ? by_group.template operator()<f16>() : by_group.template operator()<bf16_t>();
+}
+
+hipError_t run_gemm_i8_dense(const GemmI8Args& p, hipStream_t st) {
+    if (p.M == 0 || p.N == 0) return hipSuccess;
+    if (!p.w8 || p.K < 128 || p.K % 128 || p.ldx % 16 || (uintptr_t)p.xq % 16 || (uintptr_t)p.w8 % 16 || p.lora.t) return hipErrorInvalidValue;
+    return launch_dense(p, st);
 }
 
 hipError_t run_gemm_i8(const GemmI8Args& p, hipStream_t st) {

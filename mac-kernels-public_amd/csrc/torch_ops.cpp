@@ -1,9 +1,9 @@
-// Eager entry points for PyTorch: the plain linears (no LoRA, no residual) and the attention side
+// Eager entry points for PyTorch: the plain linears (no LoRA, no residual), the attention side and the MLP side
 // called straight from Python with torch tensors.  Each builds the qlin_tensor descriptors, takes the output and the
 // workspace from torch's allocator and calls the C ABI (include/qlin.h) on the current stream,
 // so an eager call costs one Python -> C++ crossing instead of the descriptor packing and ctypes
-// marshalling of qlin/_lib.py.  The argument rules and declines are those of qlin/ops.py and
-// qlin/attention.py, which run every other call (LoRA, residual) through ctypes.
+// marshalling of qlin/_lib.py.  The argument rules and declines are those of qlin/ops.py,
+// qlin/attention.py and qlin/mlp.py, which run every other call (LoRA, residual) through ctypes.
 //
 // Errors leave as QlinStatusError("<status>:<message>"); qlin/ops.py turns a status into
 // NoCapableBackendError (QLIN_EUNSUPPORTED), ValueError (QLIN_EINVAL, QLIN_EWORKSPACE) or
@@ -431,6 +431,173 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
     return o;
 }
 
+// ---- the MLP side (qlin/mlp.py) ----
+
+// [.., values] as [rows, values] with unit stride along a row (a copy if need be).
+at::Tensor rows_of(const char* op, const at::Tensor& t, const char* name, const at::Tensor* shape = nullptr) {
+    if (t.dim() < 1) fail(QLIN_EINVAL, std::string(op) + ": " + name + " must be [.., values]");
+    if (shape && t.sizes() != shape->sizes()) fail(QLIN_EINVAL, std::string(op) + ": " + name + " has another shape than the rows before it");
+    if (t.dim() == 2) return dense(t);
+    int64_t rows = 1;
+    for (int64_t i = 0; i < t.dim() - 1; ++i) rows *= t.size(i);
+    return dense(t.reshape({rows, t.size(-1)}));
+}
+
+// A new tensor shaped like x [.., values], and its rows.
+struct Fresh {
+    at::Tensor t;
+    Opt rows;
+    Fresh() = default;
+    Fresh(const at::Tensor& x, const at::Tensor& x2, at::ScalarType dt) : t(at::empty(x.sizes(), x.options().dtype(dt))), rows(x.dim() == 2 ? t : t.view(x2.sizes())) {}
+};
+
+// int8 codes like x and a scale a row.
+struct Codes {
+    at::Tensor q, scale;
+    Opt dq, ds;
+    Codes(const at::Tensor& x, const at::Tensor& x2) : q(at::empty(x.sizes(), x.options().dtype(at::kChar))) {
+        std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+        sizes.back() = 1;
+        scale = at::empty(sizes, x.options().dtype(at::kFloat));
+        dq = Opt(x.dim() == 2 ? q : q.view(x2.sizes()));
+        ds = Opt(x.dim() == 2 ? scale : scale.view({x2.size(0), 1}));
+    }
+};
+
+pybind11::tuple add_rms_norm(const at::Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps) {
+    const char* op = "add_rms_norm";
+    const OptTensor xt = x;
+    all_on_device(op, {&xt, &residual, &weight});
+    Opt x2(rows_of(op, x, "x")), r2, w = vec(weight);
+    if (residual) r2 = Opt(rows_of(op, *residual, "residual", &x));
+    Fresh y(x, x2.t, x.scalar_type()), h;
+    if (residual) h = Fresh(x, x2.t, residual->scalar_type());
+    check(qlin_add_rms_norm(x2.p(), r2.p(), w.p(), (float)eps, y.rows.p(), h.rows.p(), current_stream(x)));
+    return pybind11::make_tuple(y.t, residual ? h.t : x);
+}
+
+pybind11::tuple add_rms_norm_int8(const at::Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps, int64_t group) {
+    const char* op = "add_rms_norm_int8";
+    const OptTensor xt = x;
+    all_on_device(op, {&xt, &residual, &weight});
+    Opt x2(rows_of(op, x, "x")), r2, w = vec(weight);
+    if (residual) r2 = Opt(rows_of(op, *residual, "residual", &x));
+    Codes c(x, x2.t);
+    Fresh h;
+    if (residual) h = Fresh(x, x2.t, residual->scalar_type());
+    check(qlin_add_rms_norm_int8(x2.p(), r2.p(), w.p(), (float)eps, (int)group, c.dq.p(), c.ds.p(), h.rows.p(), current_stream(x)));
+    return pybind11::make_tuple(c.q, c.scale, residual ? h.t : x);
+}
+
+pybind11::tuple add_rms_norm_grad(const at::Tensor& dy, const OptTensor& dh, const at::Tensor& h, const OptTensor& weight, double eps,
+                                  bool weight_grad) {
+    const char* op = "add_rms_norm_grad";
+    const OptTensor gt = dy, ht = h;
+    all_on_device(op, {&gt, &dh, &ht, &weight});
+    Opt g2(rows_of(op, dy, "dy")), h2(rows_of(op, h, "h", &dy)), d2, w = vec(weight), dw;
+    if (dh) d2 = Opt(rows_of(op, *dh, "dh", &dy));
+    Fresh dx(h, h2.t, h.scalar_type());
+    const hipStream_t st = current_stream(dy);
+    at::Tensor ws;
+    if (weight_grad && weight) {
+        dw = Opt(at::empty_like(w.t));
+        ws = workspace_for(qlin_workspace_size(QLIN_OP_ADD_RMS_NORM_GRAD, g2.t.size(0), 0, g2.t.size(1), 0, g2.d.dtype), dy, st);
+    }
+    check(qlin_add_rms_norm_grad(g2.p(), d2.p(), h2.p(), w.p(), (float)eps, dx.rows.p(), dw.p(), ws.defined() ? ws.data_ptr() : nullptr,
+                                 ws.defined() ? (size_t)ws.numel() : 0, st));
+    return pybind11::make_tuple(dx.t, dw.there ? pybind11::cast(dw.t) : pybind11::object(pybind11::none()));
+}
+
+at::Tensor gated_act(const at::Tensor& gate, const OptTensor& up, int64_t act) {
+    const char* op = "gated_act";
+    const OptTensor gt = gate;
+    all_on_device(op, {&gt, &up});
+    Opt g2(rows_of(op, gate, "gate")), u2;
+    if (up) u2 = Opt(rows_of(op, *up, "up", &gate));
+    Fresh y(gate, g2.t, gate.scalar_type());
+    check(qlin_gated_act(g2.p(), u2.p(), (int)act, y.rows.p(), current_stream(gate)));
+    return y.t;
+}
+
+pybind11::tuple gated_act_int8(const at::Tensor& gate, const OptTensor& up, int64_t act, int64_t group) {
+    const char* op = "gated_act_int8";
+    const OptTensor gt = gate;
+    all_on_device(op, {&gt, &up});
+    Opt g2(rows_of(op, gate, "gate")), u2;
+    if (up) u2 = Opt(rows_of(op, *up, "up", &gate));
+    Codes c(gate, g2.t);
+    check(qlin_gated_act_int8(g2.p(), u2.p(), (int)act, (int)group, c.dq.p(), c.ds.p(), current_stream(gate)));
+    return pybind11::make_tuple(c.q, c.scale);
+}
+
+pybind11::tuple gated_act_grad(const at::Tensor& dy, const at::Tensor& gate, const OptTensor& up, int64_t act) {
+    const char* op = "gated_act_grad";
+    const OptTensor gt = gate, dt = dy;
+    all_on_device(op, {&dt, &gt, &up});
+    Opt g2(rows_of(op, gate, "gate")), d2(rows_of(op, dy, "dy", &gate)), u2;
+    const int64_t n = g2.t.size(1);
+    if (!up) {
+        Fresh d(gate, g2.t, gate.scalar_type());
+        check(qlin_gated_act_grad(d2.p(), g2.p(), nullptr, (int)act, d.rows.p(), nullptr, current_stream(gate)));
+        return pybind11::make_tuple(d.t, pybind11::none());
+    }
+    u2 = Opt(rows_of(op, *up, "up", &gate));
+    std::vector<int64_t> sizes(gate.sizes().begin(), gate.sizes().end());
+    sizes.back() = 2 * n;
+    const at::Tensor both = at::empty(sizes, gate.options()), flat = both.view({g2.t.size(0), 2 * n});
+    Opt a(flat.narrow(1, 0, n)), b(flat.narrow(1, n, n));
+    check(qlin_gated_act_grad(d2.p(), g2.p(), u2.p(), (int)act, a.p(), b.p(), current_stream(gate)));
+    return pybind11::make_tuple(both.narrow(-1, 0, n), both.narrow(-1, n, n));
+}
+
+at::Tensor w8a8_int8_linear(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& qdata, const at::Tensor& scale,
+                            const OptTensor& bias, const c10::optional<at::ScalarType>& out_dtype, const OptTensor& residual,
+                            const OptTensor& residual_scale) {
+    const char* op = "w8a8_int8_linear";
+    const OptTensor xt = x, xst = x_scale, qt = qdata, st_ = scale;
+    all_on_device(op, {&xt, &xst, &qt, &st_, &bias, &residual, &residual_scale});
+    Opt x2(rows_of(op, x, "x"));
+    if (qdata.dim() != 2) fail(QLIN_EUNSUPPORTED, "qdata must be a 2-D int8 tensor");
+    const int64_t m = x2.t.size(0), k = x2.t.size(1), n = qdata.size(0);
+    const auto count = [&](const at::Tensor& t, const char* name, int64_t want) {
+        if (t.numel() != want)
+            fail(QLIN_EINVAL, std::string(op) + ": " + name + " has " + std::to_string(t.numel()) + " elements, expected " + std::to_string(want));
+    };
+    count(x_scale, "x_scale", m);
+    if (scale.numel() != 1) count(scale, "scale", n);
+    std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = n;
+    Opt r, rs;
+    if (residual) {
+        if (residual->sizes() != at::IntArrayRef(sizes)) fail(QLIN_EINVAL, std::string(op) + ": residual has another shape than the output");
+        r = Opt(rows_of(op, *residual, "residual"));
+        if (r.t.size(0) > 1 && r.t.stride(0) < n) r = Opt(r.t.contiguous());
+        if (residual_scale) {
+            count(*residual_scale, "residual_scale", n);
+            rs = Opt(residual_scale->reshape({n}).contiguous());
+        }
+    } else if (residual_scale) {
+        fail(QLIN_EINVAL, std::string(op) + ": residual_scale given without residual");
+    }
+    const at::ScalarType dt = out_dtype.value_or(residual ? residual->scalar_type() : at::kBFloat16);
+    if (!is_float(dt)) fail(QLIN_EUNSUPPORTED, "out_dtype unsupported");
+    const at::Tensor y = at::empty(sizes, x.options().dtype(dt));
+    const at::Tensor w = dense(qdata);
+    at::Tensor ws_ = f32_1d(scale);
+    if (ws_.numel() != n) ws_ = ws_.expand({n}).contiguous();
+    const auto b = bias_1d(bias, n);
+    const auto aligned = [](const at::Tensor& t) {
+        return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(0) <= 1 || t.stride(0) % 16 == 0);
+    };
+    const int param = (aligned(x2.t) ? 0 : QLIN_W8A8_X_ROWS) | (aligned(w) && (n <= 1 || w.stride(0) == k) ? 0 : QLIN_W8A8_W_ROWS);
+    const hipStream_t st = current_stream(x);
+    const at::Tensor room = workspace_for(qlin_workspace_size(QLIN_OP_W8A8_LINEAR, m, n, k, param, 0), x, st);
+    Opt xs(f32_1d(x_scale)), dw(w), ds(ws_), yo(x.dim() == 2 ? y : y.view({m, n}));
+    qlin_tensor db;
+    check(qlin_w8a8_linear(x2.p(), xs.p(), dw.p(), ds.p(), opt(b, db), r.p(), rs.p(), yo.p(), room.data_ptr(), (size_t)room.numel(), st));
+    return y;
+}
+
 // The cached workspace for (device of `like`, current stream), at least nbytes (for the ctypes
 // calls of qlin/ops.py, so that both routes share one buffer per stream).
 at::Tensor workspace(int64_t nbytes, const at::Tensor& like) {
@@ -460,6 +627,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("qk_norm_rope_grad", &qk_norm_rope_grad);
     m.def("paged_plan", &paged_plan);
     m.def("paged_attention", &paged_attention);
+    m.def("add_rms_norm", &add_rms_norm);
+    m.def("add_rms_norm_int8", &add_rms_norm_int8);
+    m.def("add_rms_norm_grad", &add_rms_norm_grad);
+    m.def("gated_act", &gated_act);
+    m.def("gated_act_int8", &gated_act_int8);
+    m.def("gated_act_grad", &gated_act_grad);
+    m.def("w8a8_int8_linear", &w8a8_int8_linear);
     m.def("workspace", &workspace);
     m.def("release_workspaces", &release_workspaces);
 }

@@ -24,6 +24,8 @@ OP_INT8_LINEAR_LORA, OP_W4A8_LINEAR_LORA = 6, 7
 OP_INT8_LINEAR_RESIDUAL, OP_W4A8_LINEAR_RESIDUAL, OP_GGUF_LINEAR_RESIDUAL = 8, 9, 10
 OP_GGUF_LINEAR_LORA = 11
 OP_QK_NORM_ROPE_GRAD, OP_PAGED_ATTENTION = 12, 13
+OP_ADD_RMS_NORM_GRAD, OP_W8A8_LINEAR = 14, 15
+W8A8_X_ROWS, W8A8_W_ROWS = 1, 2
 ROPE_INTERLEAVED, ROPE_INVERSE = 1, 2
 
 _TORCH_DT = {
@@ -42,6 +44,8 @@ EXPORTS = (
     "qlin_gguf_linear_lora",
     "qlin_axis_rope", "qlin_qk_norm_rope", "qlin_qk_norm_rope_store", "qlin_qk_norm_rope_grad", "qlin_paged_plan",
     "qlin_paged_attention",
+    "qlin_add_rms_norm", "qlin_add_rms_norm_int8", "qlin_add_rms_norm_grad", "qlin_gated_act", "qlin_gated_act_int8",
+    "qlin_gated_act_grad", "qlin_w8a8_linear",
 )
 
 
@@ -100,6 +104,13 @@ def load():
         "qlin_qk_norm_rope_grad": (I, [T, T, T, T, T, T, ctypes.c_float, T, T, T, I, T, T, T, T, P, SZ, P]),
         "qlin_paged_plan": (I, [T, T, T, I64, T, T, T, T, T, T, T, P]),
         "qlin_paged_attention": (I, [T, T, T, T, T, ctypes.c_float, I64, T, P, SZ, P]),
+        "qlin_add_rms_norm": (I, [T, T, T, ctypes.c_float, T, T, P]),
+        "qlin_add_rms_norm_int8": (I, [T, T, T, ctypes.c_float, I, T, T, T, P]),
+        "qlin_add_rms_norm_grad": (I, [T, T, T, T, ctypes.c_float, T, T, P, SZ, P]),
+        "qlin_gated_act": (I, [T, T, I, T, P]),
+        "qlin_gated_act_int8": (I, [T, T, I, I, T, T, P]),
+        "qlin_gated_act_grad": (I, [T, T, T, I, T, T, P]),
+        "qlin_w8a8_linear": (I, [T, T, T, T, T, T, T, T, P, SZ, P]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

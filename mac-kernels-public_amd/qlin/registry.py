@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import os
 
-from . import attention, ops
+from . import attention, mlp, ops
 from .exceptions import NoCapableBackendError
 
 # func name -> (callable, keyword arguments the backend accepts beyond the plain signature)
@@ -31,6 +31,13 @@ _HIP = {
     "qk_norm_rope_grad": (attention.qk_norm_rope_grad, set()),
     "paged_plan": (attention.paged_plan, set()),
     "paged_attention": (attention.paged_attention, set()),
+    "add_rms_norm": (mlp.add_rms_norm, set()),
+    "add_rms_norm_int8": (mlp.add_rms_norm_int8, set()),
+    "add_rms_norm_grad": (mlp.add_rms_norm_grad, set()),
+    "gated_act": (mlp.gated_act, set()),
+    "gated_act_int8": (mlp.gated_act_int8, set()),
+    "gated_act_grad": (mlp.gated_act_grad, set()),
+    "w8a8_int8_linear": (mlp.w8a8_int8_linear, set()),
 }
 _OPT_IN = {"lora_down", "lora_up", "lora_scale", "correction"}
 
