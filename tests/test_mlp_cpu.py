@@ -150,6 +150,9 @@ def test_activation_gradient_refuses(over, status):
     assert lb.qlin_gated_act_grad(d(a["dy"]), d(a["gate"]), d(a["up"]), a["act"], d(a["dgate"]), d(a["dup"]), None) == status
 
 
+MANY = dict(x=z(300, 256, dtype=I8), sx=z(300, 1, dtype=F32), y=z(300, 20))
+
+
 @pytest.mark.parametrize("over,status", [
     (dict(x=None), INVALID),
     (dict(x=z(3, 256)), DECLINED),
@@ -172,8 +175,8 @@ def test_activation_gradient_refuses(over, status):
     (dict(y=z(1, 20).expand(3, 20)), INVALID),
     (dict(x=z(3, 0, dtype=I8), w=z(20, 0, dtype=I8)), DECLINED),
     (dict(x=z(1, 131072, dtype=I8), w=z(2, 131072, dtype=I8), sx=z(1, dtype=F32), sw=z(2, dtype=F32), y=z(1, 2)), DECLINED),
-    (dict(x=z(3, 250, dtype=I8), w=z(20, 250, dtype=I8)), NO_ROOM),
-    (dict(w=z(20, 272, dtype=I8)[:, :256]), NO_ROOM),
+    (dict(MANY, x=z(300, 250, dtype=I8), w=z(20, 250, dtype=I8)), NO_ROOM),   # rows that are not whole are copied
+    (dict(MANY, w=z(20, 272, dtype=I8)[:, :256]), NO_ROOM),
 ])
 def test_linear_refuses(over, status):
     L, lb = lib()
@@ -212,6 +215,6 @@ def test_workspaces():
     L, lb = lib()
     a = lambda v: (v + 255) // 256 * 256  # noqa: E731
     size = lambda m, n, k, param=0: lb.qlin_workspace_size(L.OP_W8A8_LINEAR, m, n, k, param, 0)  # noqa: E731
-    assert size(3, 20, 250) == size(3, 20, 250, 3) >= a(3 * 256) + a(20 * 256)   # rows that are not whole are copied
+    assert size(300, 20, 250) == size(300, 20, 250, 3) >= a(300 * 256) + a(20 * 256)   # rows that are not whole are copied
     assert size(300, 4096, 256, L.W8A8_W_ROWS) - size(300, 4096, 256) == a(4096 * 256)
     assert lb.qlin_workspace_size(L.OP_ADD_RMS_NORM_GRAD, 5, 0, 100, 0, L.DT_F16) >= 400
