@@ -71,7 +71,7 @@ typedef enum {
     QLIN_OP_QK_NORM_ROPE_GRAD = 12,    /* qlin_qk_norm_rope_grad: M tokens, N heads of q and k together, K the head size */
     QLIN_OP_PAGED_ATTENTION = 13,      /* qlin_paged_attention: M rows, N query heads, K the head size, param = kv heads */
     QLIN_OP_ADD_RMS_NORM_GRAD = 14,    /* qlin_add_rms_norm_grad: M rows, K values a row (N, param unused) */
-    QLIN_OP_W8A8_LINEAR = 15,          /* qlin_w8a8_linear: param = QLIN_W8A8_X_ROWS | QLIN_W8A8_W_ROWS as they apply */
+    QLIN_OP_W8A8_LINEAR = 15,          /* qlin_w8a8_linear: param = QLIN_W8A8_X_ROWS | .. as they apply */
 } qlin_op;
 
 /* ggml type ids accepted by the GGUF entry points (enum ggml_type). */
@@ -431,9 +431,10 @@ qlin_status qlin_gated_act_int8(const qlin_tensor* gate, const qlin_tensor* up, 
 qlin_status qlin_gated_act_grad(const qlin_tensor* dy, const qlin_tensor* gate, const qlin_tensor* up, int act,
                                 qlin_tensor* dgate, qlin_tensor* dup, void* stream);
 
-/* qlin_workspace_size's param for QLIN_OP_W8A8_LINEAR: operands that are copied to rows of their own first, because their
- * rows are not 16-byte aligned, or (the weights') not one behind the other.  Counted anyway when K is not a multiple of 128. */
-enum { QLIN_W8A8_X_ROWS = 1, QLIN_W8A8_W_ROWS = 2 };
+/* qlin_workspace_size's param for QLIN_OP_W8A8_LINEAR: x's rows, the weights' rows are not all 16-byte aligned or 2^25 and more
+ * bytes apart (these two count only where K is a multiple of 16); the weights' rows are not one behind the other.  Some calls
+ * copy such operands, and those of a K that is not a multiple of 128, to rows of their own in the workspace. */
+enum { QLIN_W8A8_X_ROWS = 1, QLIN_W8A8_W_ROWS = 2, QLIN_W8A8_W_APART = 4 };
 
 /* y[m,n] = x_scale[m] * scale[n] * sum_k x[m,k] qdata[n,k] + bias[n], then (with residual) residual[m,n] + residual_scale[n] *
  * that; one rounding.  x i8 [M, K] with x_scale f32 [M] or [M, 1], as qlin_quantize_act_int8, qlin_add_rms_norm_int8

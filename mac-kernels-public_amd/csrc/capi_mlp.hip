@@ -284,7 +284,7 @@ qlin_status qlin_w8a8_linear(const qlin_tensor* x, const qlin_tensor* x_scale, c
     }
     if (a.M == 0 || a.N == 0) return QLIN_OK;
     if (a.K == 0) return fail(QLIN_EUNSUPPORTED, "rows of no values");
-    const size_t need = ws_w8a8(a.M, a.N, a.K, w8a8_packs(a));
+    const size_t need = ws_w8a8(a.M, a.N, a.K, w8a8_apart(a));
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256))
         return fail(QLIN_EWORKSPACE, "workspace of %zu bytes, needs %zu (256-byte aligned)", workspace_bytes, need);
     a.ws = workspace;

@@ -86,14 +86,17 @@ struct W8A8Args {
     int64_t ldy = 0;
     void* ws = nullptr;                // ws_w8a8() bytes, 256-byte aligned
 };
-// What of a call's operands is copied to whole, aligned rows of its own first (bits of `param`).
-enum { W8A8_PACK_X = QLIN_W8A8_X_ROWS, W8A8_PACK_W = QLIN_W8A8_W_ROWS };
-int w8a8_packs(const W8A8Args& a);
-size_t ws_w8a8(int64_t M, int64_t N, int64_t K, int packs);
+// What keeps a call's operands from being taken as they are (bits of `param`).
+enum { W8A8_X_ROWS = QLIN_W8A8_X_ROWS, W8A8_W_ROWS = QLIN_W8A8_W_ROWS, W8A8_W_APART = QLIN_W8A8_W_APART };
+constexpr int64_t W8A8_MOST_APART = 1 << 25;  // row strides below it: the kernels' offsets in a tile are 32 bits
+int w8a8_apart(const W8A8Args& a);
+size_t ws_w8a8(int64_t M, int64_t N, int64_t K, int apart);
 hipError_t run_w8a8(const W8A8Args& a, hipStream_t st);
 
 // The int8 GEMM over whole rows of K values, K a multiple of 128, 16-byte aligned rows, weights K
-// apart (gemm_i8.hip): p.xq, p.sx, p.w8, p.s_ch, bias, residual and y.
-hipError_t run_gemm_i8_dense(const GemmI8Args& p, hipStream_t st);
+// apart (gemm_i8.hip): p.xq, p.sx, p.w8, p.s_ch, bias, residual and y, in tiles of the given shape.  256 x 256: as the decoded grids
+// take them, with the rows past whole rounds in smaller ones.
+enum { I8_128x64, I8_128x128, I8_256x128, I8_128x256, I8_256x256 };
+hipError_t run_gemm_i8_dense(const GemmI8Args& p, int shape, hipStream_t st);
 
 }  // namespace qlin

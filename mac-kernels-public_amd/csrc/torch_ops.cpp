@@ -586,10 +586,12 @@ at::Tensor w8a8_int8_linear(const at::Tensor& x, const at::Tensor& x_scale, cons
     at::Tensor ws_ = f32_1d(scale);
     if (ws_.numel() != n) ws_ = ws_.expand({n}).contiguous();
     const auto b = bias_1d(bias, n);
-    const auto aligned = [](const at::Tensor& t) {
-        return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(0) <= 1 || t.stride(0) % 16 == 0);
+    const auto off = [k](const at::Tensor& t) {
+        const int64_t ld = t.size(0) > 1 ? t.stride(0) : 0;
+        return k % 16 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || ld % 16 || ld >= (1 << 25));
     };
-    const int param = (aligned(x2.t) ? 0 : QLIN_W8A8_X_ROWS) | (aligned(w) && (n <= 1 || w.stride(0) == k) ? 0 : QLIN_W8A8_W_ROWS);
+    const int param = (off(x2.t) ? QLIN_W8A8_X_ROWS : 0) | (off(w) ? QLIN_W8A8_W_ROWS : 0) |
+                      (n > 1 && w.stride(0) != k ? QLIN_W8A8_W_APART : 0);
     const hipStream_t st = current_stream(x);
     const at::Tensor room = workspace_for(qlin_workspace_size(QLIN_OP_W8A8_LINEAR, m, n, k, param, 0), x, st);
     Opt xs(f32_1d(x_scale)), dw(w), ds(ws_), yo(x.dim() == 2 ? y : y.view({m, n}));

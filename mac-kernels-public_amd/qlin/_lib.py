@@ -25,7 +25,7 @@ OP_INT8_LINEAR_RESIDUAL, OP_W4A8_LINEAR_RESIDUAL, OP_GGUF_LINEAR_RESIDUAL = 8, 9
 OP_GGUF_LINEAR_LORA = 11
 OP_QK_NORM_ROPE_GRAD, OP_PAGED_ATTENTION = 12, 13
 OP_ADD_RMS_NORM_GRAD, OP_W8A8_LINEAR = 14, 15
-W8A8_X_ROWS, W8A8_W_ROWS = 1, 2
+W8A8_X_ROWS, W8A8_W_ROWS, W8A8_W_APART = 1, 2, 4
 ROPE_INTERLEAVED, ROPE_INVERSE = 1, 2
 
 _TORCH_DT = {

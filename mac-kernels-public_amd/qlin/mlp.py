@@ -198,7 +198,8 @@ def w8a8_int8_linear(x, x_scale, qdata, scale, bias=None, out_dtype=None, *, res
     r, rs = res if res is not None else (None, None)
     xs = ops._f32_1d(x_scale)
     b = ops._bias(bias, n)
-    param = (0 if _aligned(x2) else _lib.W8A8_X_ROWS) | (0 if _aligned(w) and (n <= 1 or w.stride(0) == k) else _lib.W8A8_W_ROWS)
+    param = (0 if k % 16 or _aligned(x2) else _lib.W8A8_X_ROWS) | (0 if k % 16 or _aligned(w) else _lib.W8A8_W_ROWS) | (
+        0 if n <= 1 or w.stride(0) == k else _lib.W8A8_W_APART)
     room = ops._workspace(_lib.OP_W8A8_LINEAR, m, n, k, param, x2)
     _run(op, "qlin_w8a8_linear", x.device, x2, xs, w, ws, b, r, rs, _flat(y), room.data_ptr(), room.numel())
     return y
@@ -210,7 +211,7 @@ def _scale(scale, n):
 
 
 def _aligned(t):
-    return t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) % 16 == 0)
+    return t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (t.stride(0) % 16 == 0 and t.stride(0) < 1 << 25))
 
 
 # ------------------------------------------------------------------------------------------------

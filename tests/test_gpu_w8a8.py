@@ -51,7 +51,8 @@ def test_bias_and_residual(m, dtype):
             check(y, *s, b, r, f)
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 5120, 13824), (8, 13824, 1000), (64, 16384, 300), (333, 5120, 5120), (1200, 4096, 6144), (2500, 5120, 4864)])
+@pytest.mark.parametrize("m,k,n", [(1, 5120, 13824), (8, 13824, 1000), (64, 16384, 300), (64, 5120, 13824), (130, 13824, 5120), (250, 13824, 5120), (256, 4096, 4096), (512, 4096, 500), (333, 5120, 5120), (1200, 4096, 6144), (2500, 5120, 4864),
+                                   (900, 1024, 4096), (800, 16384, 4100), (2048, 2048, 4096), (333, 4112, 4096), (1500, 4100, 1000)])
 def test_large(m, k, n):
     s = make(m, k, n)
     bias = rand(n, seed=1, dtype=BF16).to(DEV)

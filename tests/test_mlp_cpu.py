@@ -176,7 +176,7 @@ MANY = dict(x=z(300, 256, dtype=I8), sx=z(300, 1, dtype=F32), y=z(300, 20))
     (dict(x=z(3, 0, dtype=I8), w=z(20, 0, dtype=I8)), DECLINED),
     (dict(x=z(1, 131072, dtype=I8), w=z(2, 131072, dtype=I8), sx=z(1, dtype=F32), sw=z(2, dtype=F32), y=z(1, 2)), DECLINED),
     (dict(MANY, x=z(300, 250, dtype=I8), w=z(20, 250, dtype=I8)), NO_ROOM),   # rows that are not whole are copied
-    (dict(MANY, w=z(20, 272, dtype=I8)[:, :256]), NO_ROOM),
+    (dict(MANY, w=z(20, 257, dtype=I8)[:, :256]), NO_ROOM),
 ])
 def test_linear_refuses(over, status):
     L, lb = lib()
@@ -216,5 +216,7 @@ def test_workspaces():
     a = lambda v: (v + 255) // 256 * 256  # noqa: E731
     size = lambda m, n, k, param=0: lb.qlin_workspace_size(L.OP_W8A8_LINEAR, m, n, k, param, 0)  # noqa: E731
     assert size(300, 20, 250) == size(300, 20, 250, 3) >= a(300 * 256) + a(20 * 256)   # rows that are not whole are copied
-    assert size(300, 4096, 256, L.W8A8_W_ROWS) - size(300, 4096, 256) == a(4096 * 256)
+    assert size(300, 4096, 256) == size(64, 300, 250) == 0
+    assert size(3000, 4096, 256, L.W8A8_W_ROWS) == a(4096 * 256) and size(3000, 4096, 256, L.W8A8_X_ROWS) == a(3000 * 256)
+    assert size(9504, 4096, 4096, L.W8A8_W_APART) == a(4096 * 4096) and size(9504, 4096, 4096) == 0
     assert lb.qlin_workspace_size(L.OP_ADD_RMS_NORM_GRAD, 5, 0, 100, 0, L.DT_F16) >= 400
