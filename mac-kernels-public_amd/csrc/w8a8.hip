@@ -87,6 +87,22 @@ __global__ __launch_bounds__(64 * WAVES) void w8a8_tile_kernel(W8A8Args a, int m
         bias[e] = a.bias ? load_bits_rt(a.bias, a.bias_dt, n) : 0u;
     }
 
+    const int count = (int)max<int64_t>(0, min<int64_t>(4, a.N - nc));
+    const int es = a.res.r_dt == DT_F32 ? 16 : 8;  // bytes of 4 residual values
+    const bool res4 = a.res.r && a.res.ldr % 4 == 0 && (uintptr_t)a.res.r % es == 0;  // n0 is a multiple of 16
+    u32x4 res[Q];
+    if (res4 && count == 4)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const uint8_t* p = (const uint8_t*)a.res.r + (min<int64_t>(m0 + (tid + T * q) / C4, a.M - 1) * a.res.ldr + nc) * (es / 4);
+            if (es == 16) {
+                res[q] = *reinterpret_cast<const u32x4*>(p);
+            } else {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+                res[q] = u32x4{v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
+            }
+        }
+
     const int K = (int)a.K, stages = (K + 127) / 128;
     const int first = stages * wave / WAVES, n = stages * (wave + 1) / WAVES - first;
     uint8_t* ring = smem + wave * ST * SB;
@@ -177,7 +193,9 @@ __global__ __launch_bounds__(64 * WAVES) void w8a8_tile_kernel(W8A8Args a, int m
             for (int v = 0; v < 4; ++v) sums[(wave * R + 16 * p + 4 * g + v) * LDC + 16 * q + r16] = acc[p][q][v];
     __syncthreads();
     const bool vec = a.ldy % 4 == 0 && (uintptr_t)a.y % 16 == 0;
-    const int count = (int)max<int64_t>(0, min<int64_t>(4, a.N - nc));
+    float rs[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rs[e] = a.res.rs ? load_rt(a.res.rs, a.res.rs_dt, min<int64_t>(nc + e, a.N - 1)) : 1.0f;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         const int row = (tid + T * q) / C4;
@@ -189,7 +207,12 @@ __global__ __launch_bounds__(64 * WAVES) void w8a8_tile_kernel(W8A8Args a, int m
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = scaled(sum[e], sx[q], sw[e], a.bias, bits_to_f32_rt(bias[e], a.bias_dt));
-        if (a.res.r) residual_apply4(a.res, m, nc, a.N, y);
+        if (a.res.r) {
+            if (res4 && count == 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(rs[e], y[e], bits_to_f32_rt(res[q][e], a.res.r_dt));
+            else residual_apply4(a.res, m, nc, a.N, y);
+        }
         store4_rt(a.y, a.y_dt, m * a.ldy + nc, y, count, vec);
     }
 }
