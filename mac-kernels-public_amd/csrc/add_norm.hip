@@ -1,220 +1,231 @@
 // Root-mean-square norm with the residual's addition: h = x + r, y = w h rho, rho = (mean h^2 + eps)^-1/2, y in 16 or 32
 // bits or in 8 with a scale a row, and its gradient.  Bound by memory: every value is read once and written once.
 //
-// A row stays in registers between its reads and its writes.  8 bits: the codes are rne(127 v / top) with v = w h
-// (rotated, for weights that are stored so) and top the row's largest |v|; rho cancels in them, so that one
-// exchange between a row's threads gives both the sum of squares and top, and the scale is top rho / 127.
-#include <algorithm>
-
+// A row stays in registers between its reads and its writes, 8 or 16 values a thread, a row (or a few short ones) a workgroup.  8
+// bits: the codes are rne(127 v / top) with v = w h (rotated, for weights that are stored so) and top the row's largest |v|;
+// rho cancels in them, so that one exchange between a row's threads gives both the sum of squares and top, and the scale is
+// top rho / 127.  (Workgroups that take rows in turn, the next one's reads in flight: 4608 x 6144 to bf16 50 us against 49 and, with
+// nontemporal writes, 40; the gradient is so because its workgroups keep partial sums.)
 #include "mlp_rows.h"
 
 namespace qlin {
 namespace {
 
-// The sum of a and the largest of b over the threads of a row: a wave's lanes, or all of a workgroup's.
-template <bool WAVE>
-__device__ __forceinline__ void row_sum_max(float& a, uint32_t& b) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// T: x and y, H: the residual and h.  RUN 16: rotated.  RES: with a residual.  ONCE: nontemporal reads and writes.
+template <typename T, typename H, int RUN, int SLOTS, bool INT8, bool RES, bool ONCE>
+__global__ __launch_bounds__(1024, 6) void add_norm_kernel(AddNormArgs a, int64_t t0, int per, int groups) {
+    const Group g(per);
+    const int64_t t = t0 + (int64_t)blockIdx.x * groups + g.wave / g.waves;
+    const bool live = t < a.T;
+    Run<T, RUN> x[SLOTS];
+    Run<H, RUN> r[SLOTS];
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        a += __shfl_xor(a, m, 64);
-        b = max(b, (uint32_t)__shfl_xor((int)b, m, 64));
+    for (int s = 0; s < SLOTS; ++s) {
+        const int e0 = (s * per + g.at) * RUN, n = live ? a.W - e0 : 0;
+        x[s] = load_raw<ONCE, T, RUN>((const T*)a.x.p + t * a.x.ld + e0, n);
+        if constexpr (RES) r[s] = load_raw<ONCE, H, RUN>((const H*)a.r.p + t * a.r.ld + e0, n);
     }
-    if constexpr (!WAVE) {
-        __shared__ float sums[16];
-        __shared__ uint32_t tops[16];
-        if (lane == 0) {
-            sums[wave] = a;
-            tops[wave] = b;
+    float v[SLOTS][RUN];
+    float ss = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        const int e0 = (s * per + g.at) * RUN;
+        float w[RUN];
+        if (a.w) load_run_rt<RUN>(a.w, a.w_dt, e0, a.W - e0, w);
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) v[s][i] = RES ? (float)x[s].v[i] + (float)r[s].v[i] : (float)x[s].v[i];
+        if (RES && live && e0 < a.W) store_run<ONCE, H, RUN>((H*)a.h.p + t * a.h.ld + e0, a.W - e0, v[s]);
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[s][i], v[s][i], ss);
+        if (a.w)
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) v[s][i] *= w[i];
+        if constexpr (INT8 && RUN == 16) rotate_run(v[s], a.G, g.lane);
+        if constexpr (INT8)
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[s][i]));
+    }
+    g.sums(ss, top, 0, [](uint32_t p, uint32_t q) { return max(p, q); });
+    const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
+    if (!live) return;
+    if constexpr (INT8) {
+        const float most = __uint_as_float(top);
+        float first;
+        const float inv = code_factor(most, first);
+        if (g.at == 0) a.scale[t] = most / 127.0f * rho;
+        if (first != 1.0f)
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) v[s][i] *= first;
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            const int e0 = (s * per + g.at) * RUN;
+            if (e0 < a.W) store_codes<ONCE, RUN>(a.q + t * a.ldq + e0, a.W - e0, v[s], inv);
         }
-        __syncthreads();
-        a = 0.0f;
-        for (int i = 0; i < waves; ++i) {
-            a += sums[i];
-            b = max(b, tops[i]);
+    } else {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            const int e0 = (s * per + g.at) * RUN;
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) v[s][i] *= rho;
+            if (e0 < a.W) store_run<ONCE, T, RUN>((T*)a.y.p + t * a.y.ld + e0, a.W - e0, v[s]);
         }
     }
 }
 
-// A row a workgroup, or (WAVE) a wave; every thread holds SLOTS runs of RUN values.  SLOTS 0: rows of any length, read
-// twice.  T: x and y, H: the residual and h.
-template <typename T, typename H, int RUN, int SLOTS, bool INT8, bool WAVE>
-__global__ __launch_bounds__(1024) void add_norm_kernel(AddNormArgs a, int64_t t0) {
-    const int lane = threadIdx.x & 63;
-    const int per = WAVE ? 64 : (int)blockDim.x, at = WAVE ? lane : (int)threadIdx.x;
-    const int64_t t = t0 + (WAVE ? (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6) : (int64_t)blockIdx.x);
-    if (t >= a.T) return;  // a whole wave's (WAVE), or no thread's
-    const T* x = (const T*)a.x.p + t * a.x.ld;
-    const H* r = a.r.p ? (const H*)a.r.p + t * a.r.ld : nullptr;
-    H* h = a.r.p ? (H*)a.h.p + t * a.h.ld : nullptr;
-    float ss = 0.0f;
-    uint32_t top = 0;
-    auto sum_of = [&](int e0, float* v) {
-        const int n = a.W - e0;
-        load_run<T, RUN>(x + e0, n, v);
-        if (r) {
-            float u[RUN];
-            load_run<H, RUN>(r + e0, n, u);
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) v[i] += u[i];
-        }
-    };
-    // the weighted values, rotated: what the 8-bit output holds but for rho
-    auto weigh = [&](int e0, float* v) {
-        if (a.w) {
-            float w[RUN];
-            load_run_rt<RUN>(a.w, a.w_dt, e0, a.W - e0, w);
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) v[i] *= w[i];
-        }
-        if constexpr (INT8 && RUN == 16) rotate_run(v, a.G, lane);
-    };
-    auto squares = [&](const float* v) {
-#pragma unroll
-        for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
-    };
-    auto largest = [&](const float* v) {
-#pragma unroll
-        for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[i]));
-    };
-    auto emit = [&](int e0, float* v, float rho, float inv, float first) {
-        const int n = a.W - e0;
-        if constexpr (INT8) {
-            if (first != 1.0f)
-#pragma unroll
-                for (int i = 0; i < RUN; ++i) v[i] *= first;
-            if (n > 0) store_codes<RUN>(a.q + t * a.ldq + e0, n, v, inv);
-        } else {
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) v[i] *= rho;
-            if (n > 0) store_run<T, RUN>((T*)a.y.p + t * a.y.ld + e0, n, v);
-        }
-    };
-    auto finish = [&](float& rho, float& inv, float& first) {
-        row_sum_max<WAVE>(ss, top);
-        rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
-        if constexpr (INT8) {
-            const float largest_v = __uint_as_float(top);
-            inv = code_factor(largest_v, first);
-            if (at == 0) a.scale[t] = largest_v / 127.0f * rho;
-        }
-    };
-    float rho, inv = 0.0f, first = 1.0f;
-    if constexpr (SLOTS > 0) {
-        float v[SLOTS][RUN];
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) sum_of((s * per + at) * RUN, v[s]);
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + at) * RUN;
-            if (h && e0 < a.W) store_run<H, RUN>(h + e0, a.W - e0, v[s]);
-            squares(v[s]);
-            weigh(e0, v[s]);
-            if constexpr (INT8) largest(v[s]);
-        }
-        finish(rho, inv, first);
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) emit((s * per + at) * RUN, v[s], rho, inv, first);
-    } else {
+// Rows of any length, read twice.
+template <typename T, typename H, int RUN, bool INT8>
+__global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
+    const Group g(512);
+    int turn = 0;
+    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
+        const T* x = (const T*)a.x.p + t * a.x.ld;
+        const H* r = a.r.p ? (const H*)a.r.p + t * a.r.ld : nullptr;
         float v[RUN];
-        for (int c = 0; c < a.W; c += per * RUN) {
-            sum_of(c + at * RUN, v);
-            squares(v);
+        auto sum_of = [&](int e0) {
+            load_run<T, RUN>(x + e0, a.W - e0, v);
+            if (r) {
+                float u[RUN];
+                load_run<H, RUN>(r + e0, a.W - e0, u);
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) v[i] += u[i];
+            }
+        };
+        auto weigh = [&](int e0) {
+            if (a.w) {
+                float u[RUN];
+                load_run_rt<RUN>(a.w, a.w_dt, e0, a.W - e0, u);
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) v[i] *= u[i];
+            }
+            if constexpr (INT8 && RUN == 16) rotate_run(v, a.G, g.lane);
+        };
+        float ss = 0.0f;
+        uint32_t top = 0;
+        for (int c = 0; c < a.W; c += 512 * RUN) {
+            const int e0 = c + g.at * RUN;
+            sum_of(e0);
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
             if constexpr (INT8) {
-                weigh(c + at * RUN, v);
-                largest(v);
+                weigh(e0);
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[i]));
             }
         }
-        finish(rho, inv, first);
-        for (int c = 0; c < a.W; c += per * RUN) {
-            const int e0 = c + at * RUN;
-            sum_of(e0, v);
-            if (h && e0 < a.W) store_run<H, RUN>(h + e0, a.W - e0, v);
-            weigh(e0, v);
-            emit(e0, v, rho, inv, first);
+        g.sums(ss, top, turn, [](uint32_t p, uint32_t q) { return max(p, q); });
+        const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps), most = __uint_as_float(top);
+        float first = 1.0f;
+        const float inv = INT8 ? code_factor(most, first) : 0.0f;
+        if (INT8 && g.at == 0) a.scale[t] = most / 127.0f * rho;
+        for (int c = 0; c < a.W; c += 512 * RUN) {
+            const int e0 = c + g.at * RUN;
+            sum_of(e0);
+            if (r && e0 < a.W) store_run<false, H, RUN>((H*)a.h.p + t * a.h.ld + e0, a.W - e0, v);
+            weigh(e0);
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) v[i] *= INT8 ? first : rho;
+            if (e0 >= a.W) continue;
+            if constexpr (INT8) store_codes<false, RUN>(a.q + t * a.ldq + e0, a.W - e0, v, inv);
+            else store_run<false, T, RUN>((T*)a.y.p + t * a.y.ld + e0, a.W - e0, v);
         }
     }
 }
 
 // dx = rho (g - h rho^2 mean(g h)) + dh with g = w dy, and a workgroup's part of dw = sum_t dy h rho.
-template <typename T, typename H, int SLOTS>
-__global__ __launch_bounds__(1024) void add_norm_grad_kernel(AddNormGradArgs a) {
+template <typename T, typename H, int SLOTS, bool DH, bool ONCE, int THREADS>
+__global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs a, int per, int groups) {
     constexpr int RUN = 8;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int per = blockDim.x, at = threadIdx.x;
-    __shared__ float red[2][16][2];
+    const Group g(per);
+    struct Raw {
+        Run<T, RUN> dy;
+        Run<H, RUN> h, dh;
+    };
+    auto fetch = [&](int64_t t, Raw (&o)[SLOTS]) {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            const int e0 = (s * per + g.at) * RUN;
+            const int n = t < a.T ? a.W - e0 : 0;
+            o[s].dy = load_raw<ONCE, T, RUN>((const T*)a.dy.p + t * a.dy.ld + e0, n);
+            o[s].h = load_raw<ONCE, H, RUN>((const H*)a.h.p + t * a.h.ld + e0, n);
+            if constexpr (DH) o[s].dh = load_raw<ONCE, H, RUN>((const H*)a.dh.p + t * a.dh.ld + e0, n);
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * groups;
+    int64_t t = (int64_t)blockIdx.x * groups + g.wave / g.waves;
+    Raw raw[SLOTS];
+    fetch(t, raw);
     float w[SLOTS][RUN], dw[SLOTS][RUN];
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s)
+    for (int s = 0; s < SLOTS; ++s) {
+        const int e0 = (s * per + g.at) * RUN;
+        if (a.w) load_run_rt<RUN>(a.w, a.w_dt, e0, a.W - e0, w[s]);
 #pragma unroll
         for (int i = 0; i < RUN; ++i) {
-            w[s][i] = 1.0f;
+            if (!a.w) w[s][i] = 1.0f;
             dw[s][i] = 0.0f;
         }
-    if (a.w)
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + at) * RUN;
-            load_run_rt<RUN>(a.w, a.w_dt, e0, a.W - e0, w[s]);
-        }
+    }
     int turn = 0;
-    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
-        float g[SLOTS][RUN], h[SLOTS][RUN], d[SLOTS][RUN];
-        float ss = 0.0f, gh = 0.0f;
+    for (int64_t base = (int64_t)blockIdx.x * groups; base < a.T; base += step, t += step, turn ^= 1) {
+        Raw now[SLOTS];
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + at) * RUN, n = a.W - e0;
-            load_run<T, RUN>((const T*)a.dy.p + t * a.dy.ld + e0, n, g[s]);
-            load_run<H, RUN>((const H*)a.h.p + t * a.h.ld + e0, n, h[s]);
-            if (a.dh.p) load_run<H, RUN>((const H*)a.dh.p + t * a.dh.ld + e0, n, d[s]);
-        }
+        for (int s = 0; s < SLOTS; ++s) now[s] = raw[s];
+        fetch(t + step, raw);
+        float ss = 0.0f, gh = 0.0f;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                ss = __builtin_fmaf(h[s][i], h[s][i], ss);
-                gh = __builtin_fmaf(g[s][i] * w[s][i], h[s][i], gh);
+                const float h = (float)now[s].h.v[i];
+                ss = __builtin_fmaf(h, h, ss);
+                gh = __builtin_fmaf((float)now[s].dy.v[i] * w[s][i], h, gh);
             }
-        ss = wave_sum(ss);
-        gh = wave_sum(gh);
-        if (lane == 0) {
-            red[turn][wave][0] = ss;
-            red[turn][wave][1] = gh;
-        }
-        __syncthreads();  // the other turn's sums were read before this barrier
-        ss = gh = 0.0f;
-        for (int i = 0; i < waves; ++i) {
-            ss += red[turn][i][0];
-            gh += red[turn][i][1];
-        }
+        g.sums(ss, gh, turn, [](float p, float q) { return p + q; });
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
         const float c = rho * rho * (gh / (float)a.W);
+        if (t >= a.T) continue;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + at) * RUN;
+            const int e0 = (s * per + g.at) * RUN;
             float o[RUN];
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                dw[s][i] = __builtin_fmaf(g[s][i], h[s][i] * rho, dw[s][i]);
-                o[i] = rho * (g[s][i] * w[s][i] - h[s][i] * c);
-                if (a.dh.p) o[i] += d[s][i];
+                const float d = (float)now[s].dy.v[i], h = (float)now[s].h.v[i];
+                dw[s][i] = __builtin_fmaf(d, h * rho, dw[s][i]);
+                o[i] = rho * (d * w[s][i] - h * c);
+                if constexpr (DH) o[i] += (float)now[s].dh.v[i];
             }
-            if (e0 < a.W) store_run<H, RUN>((H*)a.dx.p + t * a.dx.ld + e0, a.W - e0, o);
+            if (e0 < a.W) store_run<ONCE, H, RUN>((H*)a.dx.p + t * a.dx.ld + e0, a.W - e0, o);
         }
     }
-    if (a.dw)
+    if (!a.dw) return;
+    // the groups' sums, in their order, are the workgroup's
+    __shared__ float other[256 * RUN];  // groups of fewer than 256 threads: one slot
+    for (int k = 1; k < groups; ++k) {
+        __syncthreads();
+        if (g.wave / g.waves == k)
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + at) * RUN;
-            if (e0 < a.W) store_run<float, RUN>(a.part + (int64_t)blockIdx.x * a.W + e0, a.W - e0, dw[s]);
-        }
+            for (int i = 0; i < RUN; ++i) other[g.at * RUN + i] = dw[0][i];
+        __syncthreads();
+        if (g.wave / g.waves == 0)
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) dw[0][i] += other[g.at * RUN + i];
+    }
+    if (g.wave / g.waves) return;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        const int e0 = (s * per + g.at) * RUN;
+        if (e0 < a.W) store_run<false, float, RUN>(a.part + (int64_t)blockIdx.x * a.W + e0, a.W - e0, dw[s]);
+    }
 }
 
-// Rows of any length: the row's sums, then its gradient; dw by add_norm_dw_kernel from rho.
+// Rows of any length: the row's sums, then its gradient.
 template <typename T, typename H>
-__global__ __launch_bounds__(1024) void add_norm_grad_long_kernel(AddNormGradArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __shared__ float red[2][16][2];
+__global__ __launch_bounds__(512) void add_norm_grad_long_kernel(AddNormGradArgs a) {
+    const Group g(512);
     float* part = a.dw ? a.part + (int64_t)blockIdx.x * a.W : nullptr;
     int turn = 0;
     bool begun = false;
@@ -224,29 +235,18 @@ __global__ __launch_bounds__(1024) void add_norm_grad_long_kernel(AddNormGradArg
         const H* dh = a.dh.p ? (const H*)a.dh.p + t * a.dh.ld : nullptr;
         H* dx = (H*)a.dx.p + t * a.dx.ld;
         float ss = 0.0f, gh = 0.0f;
-        for (int e = threadIdx.x; e < a.W; e += blockDim.x) {
-            const float v = (float)h[e], g = (float)dy[e] * (a.w ? load_rt(a.w, a.w_dt, e) : 1.0f);
+        for (int e = threadIdx.x; e < a.W; e += 512) {
+            const float v = (float)h[e], d = (float)dy[e] * (a.w ? load_rt(a.w, a.w_dt, e) : 1.0f);
             ss = __builtin_fmaf(v, v, ss);
-            gh = __builtin_fmaf(g, v, gh);
+            gh = __builtin_fmaf(d, v, gh);
         }
-        ss = wave_sum(ss);
-        gh = wave_sum(gh);
-        if (lane == 0) {
-            red[turn][wave][0] = ss;
-            red[turn][wave][1] = gh;
-        }
-        __syncthreads();
-        ss = gh = 0.0f;
-        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) {
-            ss += red[turn][i][0];
-            gh += red[turn][i][1];
-        }
+        g.sums(ss, gh, turn, [](float p, float q) { return p + q; });
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
         const float c = rho * rho * (gh / (float)a.W);
-        for (int e = threadIdx.x; e < a.W; e += blockDim.x) {  // an element is the same thread's in every row
-            const float v = (float)h[e], g = (float)dy[e], w = a.w ? load_rt(a.w, a.w_dt, e) : 1.0f;
-            if (part) part[e] = __builtin_fmaf(g, v * rho, begun ? part[e] : 0.0f);
-            dx[e] = (H)(rho * (g * w - v * c) + (dh ? (float)dh[e] : 0.0f));
+        for (int e = threadIdx.x; e < a.W; e += 512) {  // an element is the same thread's in every row
+            const float v = (float)h[e], d = (float)dy[e], w = a.w ? load_rt(a.w, a.w_dt, e) : 1.0f;
+            if (part) part[e] = __builtin_fmaf(d, v * rho, begun ? part[e] : 0.0f);
+            dx[e] = (H)(rho * (d * w - v * c) + (dh ? (float)dh[e] : 0.0f));
         }
         begun = true;
     }
@@ -257,8 +257,18 @@ __global__ __launch_bounds__(256) void add_norm_dw_kernel(const float* part, int
     __shared__ float sums[16][17];
     const int c = threadIdx.x & 15, i = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
     float s = 0.0f;
-    if (e < W)
-        for (int p = i; p < parts; p += 16) s += part[(int64_t)p * W + e];
+    if (e < W) {
+        const float* p = part + e;
+        int k = i;
+        for (; k + 7 * 16 < parts; k += 8 * 16) {  // eight in flight
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = p[(int64_t)(k + 16 * j) * W];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; k < parts; k += 16) s += p[(int64_t)k * W];
+    }
     sums[i][c] = s;
     __syncthreads();
     if (i || e >= W) return;
@@ -266,48 +276,53 @@ __global__ __launch_bounds__(256) void add_norm_dw_kernel(const float* part, int
     store_rt(dw, dw_dt, e, s);
 }
 
-constexpr int GRAD_PARTS = 512;
+// The gradient's workgroups leave W partial sums each: as many as the chip holds at once, and no more.
+RowCut grad_cut(int64_t T, int W) { return cut_rows(T, W, 8, 16); }
 
-int grad_parts(int64_t T) { return (int)std::min<int64_t>(T, GRAD_PARTS); }
-
-template <typename T, typename H, int RUN, bool INT8>
+template <typename T, typename H, int RUN, bool INT8, bool RES>
 hipError_t launch_norm(const AddNormArgs& a, hipStream_t st) {
-    int slots = 0;
-    const int n = row_threads(a.W, RUN, slots);
-    const int64_t most = (int64_t)(0x7FFFFFFF / n);  // workgroups of one launch: a grid's threads count to 2^32
-    for (int64_t t0 = 0; t0 < a.T; t0 += most) {
-        const dim3 grid((unsigned)std::min<int64_t>(most, a.T - t0)), block((unsigned)n);
-        switch (slots) {
-            case 1: hipLaunchKernelGGL((add_norm_kernel<T, H, RUN, 1, INT8, false>), grid, block, 0, st, a, t0); break;
-            case 2: hipLaunchKernelGGL((add_norm_kernel<T, H, RUN, 2, INT8, false>), grid, block, 0, st, a, t0); break;
-            case 4: hipLaunchKernelGGL((add_norm_kernel<T, H, RUN, 4, INT8, false>), grid, block, 0, st, a, t0); break;
-            default: hipLaunchKernelGGL((add_norm_kernel<T, H, RUN, 0, INT8, false>), grid, block, 0, st, a, t0); break;
-        }
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+    const RowCut c = cut_rows(a.T, a.W, RUN, 0);
+    if (!c.slots) {
+        hipLaunchKernelGGL((add_norm_long_kernel<T, H, RUN, INT8>), dim3(c.grid), c.block(), 0, st, a);
+        return hipGetLastError();
     }
-    return hipSuccess;
+    const bool pieces = aligned(a.x, sizeof(T)) && aligned(a.r, sizeof(H)) && aligned(a.y, sizeof(T)) && aligned(a.h, sizeof(H)) &&
+                        aligned({a.q, a.ldq}, 1);
+    const bool once = pieces && a.T * a.W * (int64_t)(sizeof(T) + (RES ? sizeof(H) : 0)) > ONCE_BYTES;
+    return by_parts(c, a.T, [&](dim3 grid, int64_t t0) {
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, c.block(), 0, st, a, t0, c.per, c.groups); };
+        if (c.slots == 1) once ? go(add_norm_kernel<T, H, RUN, 1, INT8, RES, true>) : go(add_norm_kernel<T, H, RUN, 1, INT8, RES, false>);
+        else if constexpr (RUN == 8) once ? go(add_norm_kernel<T, H, 8, 2, INT8, RES, true>) : go(add_norm_kernel<T, H, 8, 2, INT8, RES, false>);
+    });
 }
 
 template <typename T, typename H>
 hipError_t norm_of(const AddNormArgs& a, hipStream_t st) {
-    if (!a.q) return launch_norm<T, H, 8, false>(a, st);
-    return a.G ? launch_norm<T, H, 16, true>(a, st) : launch_norm<T, H, 8, true>(a, st);
+    auto by_res = [&]<int RUN, bool INT8>() {
+        return a.r.p ? launch_norm<T, H, RUN, INT8, true>(a, st) : launch_norm<T, H, RUN, INT8, false>(a, st);
+    };
+    if (!a.q) return by_res.template operator()<8, false>();
+    return a.G ? by_res.template operator()<16, true>() : by_res.template operator()<8, true>();
 }
 
 template <typename T, typename H>
 hipError_t grad_of(const AddNormGradArgs& a, hipStream_t st) {
-    int slots = 0;
-    const int n = row_threads(a.W, 8, slots), parts = grad_parts(a.T);
-    const dim3 grid((unsigned)parts), block((unsigned)n);
-    switch (slots) {
-        case 1: hipLaunchKernelGGL((add_norm_grad_kernel<T, H, 1>), grid, block, 0, st, a); break;
-        case 2: hipLaunchKernelGGL((add_norm_grad_kernel<T, H, 2>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((add_norm_grad_long_kernel<T, H>), grid, block, 0, st, a); break;
+    const RowCut c = grad_cut(a.T, a.W);
+    const bool once = a.T * a.W * (int64_t)(sizeof(T) + sizeof(H)) > ONCE_BYTES && aligned(a.dy, sizeof(T)) && aligned(a.h, sizeof(H)) &&
+                      aligned(a.dh, sizeof(H)) && aligned(a.dx, sizeof(H));
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(c.grid), c.block(), 0, st, a, c.per, c.groups); };
+    auto by_slots = [&]<int SLOTS, int THREADS>() {
+        if (a.dh.p) once ? go(add_norm_grad_kernel<T, H, SLOTS, true, true, THREADS>) : go(add_norm_grad_kernel<T, H, SLOTS, true, false, THREADS>);
+        else once ? go(add_norm_grad_kernel<T, H, SLOTS, false, true, THREADS>) : go(add_norm_grad_kernel<T, H, SLOTS, false, false, THREADS>);
+    };
+    switch (c.slots) {
+        case 1: by_slots.template operator()<1, 512>(); break;
+        case 2: c.per <= 512 ? by_slots.template operator()<2, 512>() : by_slots.template operator()<2, 1024>(); break;
+        default: hipLaunchKernelGGL((add_norm_grad_long_kernel<T, H>), dim3(c.grid), c.block(), 0, st, a); break;
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.dw) return e;
-    hipLaunchKernelGGL(add_norm_dw_kernel, dim3((unsigned)((a.W + 15) / 16)), dim3(256), 0, st, a.part, parts, a.W, a.dw, a.dw_dt);
+    hipLaunchKernelGGL(add_norm_dw_kernel, dim3((unsigned)((a.W + 15) / 16)), dim3(256), 0, st, a.part, (int)c.grid, a.W, a.dw, a.dw_dt);
     return hipGetLastError();
 }
 
@@ -325,7 +340,9 @@ hipError_t run_add_norm(const AddNormArgs& a, hipStream_t st) {
     return by_types(a, [&]<typename T, typename H>() { return norm_of<T, H>(a, st); });
 }
 
-size_t ws_add_norm_grad(int64_t T, int64_t W) { return (size_t)grad_parts(T) * W * 4; }
+size_t ws_add_norm_grad(int64_t T, int64_t W) {
+    return T <= 0 || W <= 0 || W > MLP_MAX_WIDTH ? 0 : (size_t)grad_cut(T, (int)W).grid * (size_t)W * 4;
+}
 
 hipError_t run_add_norm_grad(const AddNormGradArgs& a, hipStream_t st) {
     if (a.W == 0) return hipSuccess;

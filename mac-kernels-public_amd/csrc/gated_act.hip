@@ -4,8 +4,6 @@
 //
 // 8 bits: a row stays in registers until its largest |value| is known; the codes are rne(127 v / top), v rotated first for
 // weights that are stored so, the scale is top / 127.
-#include <algorithm>
-
 #include "mlp_rows.h"
 
 namespace qlin {
@@ -33,121 +31,134 @@ __device__ __forceinline__ void gate_of(float z, float& s, float& dt) {
         dt = GELU_C * __builtin_fmaf(3.0f * GELU_A, z2, 1.0f);
     }
 }
-// y = f(gate) up, 8 values a thread.
-template <typename T, int ACT, bool GATED>
+// y = f(gate) up, 8 values a thread.  ONCE: nontemporal reads and writes.
+template <typename T, int ACT, bool GATED, bool ONCE>
 __global__ __launch_bounds__(256) void gated_act_kernel(GatedActArgs a, int64_t t0, uint32_t units, uint32_t per) {
     const uint32_t u = blockIdx.x * 256u + threadIdx.x;
     if (u >= units) return;
     const uint32_t row = u / per;
     const int e0 = (int)(u - row * per) * 8, n = a.W - e0;
     const int64_t t = t0 + row;
-    float z[8], v[8];
-    load_run<T, 8>((const T*)a.gate.p + t * a.gate.ld + e0, n, z);
-    if constexpr (GATED) load_run<T, 8>((const T*)a.up.p + t * a.up.ld + e0, n, v);
+    const auto z = load_raw<ONCE, T, 8>((const T*)a.gate.p + t * a.gate.ld + e0, n);
+    Run<T, 8> w;
+    if constexpr (GATED) w = load_raw<ONCE, T, 8>((const T*)a.up.p + t * a.up.ld + e0, n);
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float s, dt;
-        gate_of<T, ACT>(z[i], s, dt);
-        const float f = z[i] * s;
-        v[i] = GATED ? f * v[i] : f;
+        gate_of<T, ACT>((float)z.v[i], s, dt);
+        v[i] = (float)z.v[i] * s;
+        if constexpr (GATED) v[i] *= (float)w.v[i];
     }
-    store_run<T, 8>((T*)a.y.p + t * a.y.ld + e0, n, v);
+    store_run<ONCE, T, 8>((T*)a.y.p + t * a.y.ld + e0, n, v);
 }
 
-template <typename T, int ACT, bool GATED>
+template <typename T, int ACT, bool GATED, bool ONCE>
 __global__ __launch_bounds__(256) void gated_act_grad_kernel(GatedActArgs a, int64_t t0, uint32_t units, uint32_t per) {
     const uint32_t u = blockIdx.x * 256u + threadIdx.x;
     if (u >= units) return;
     const uint32_t row = u / per;
     const int e0 = (int)(u - row * per) * 8, n = a.W - e0;
     const int64_t t = t0 + row;
-    float z[8], v[8], g[8];
-    load_run<T, 8>((const T*)a.gate.p + t * a.gate.ld + e0, n, z);
-    if constexpr (GATED) load_run<T, 8>((const T*)a.up.p + t * a.up.ld + e0, n, v);
-    load_run<T, 8>((const T*)a.dy.p + t * a.dy.ld + e0, n, g);
+    const auto z = load_raw<ONCE, T, 8>((const T*)a.gate.p + t * a.gate.ld + e0, n);
+    Run<T, 8> w;
+    if constexpr (GATED) w = load_raw<ONCE, T, 8>((const T*)a.up.p + t * a.up.ld + e0, n);
+    const auto d = load_raw<ONCE, T, 8>((const T*)a.dy.p + t * a.dy.ld + e0, n);
+    float dg[8], du[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float s, dt;
-        gate_of<T, ACT>(z[i], s, dt);
-        const float f = z[i] * s, p = s * (1.0f - s);
-        const float df = p == 0.0f ? s : s + z[i] * p * dt;  // far from 0, where z dt may be infinite, sigma
-        const float up = GATED ? v[i] : 1.0f;
-        v[i] = g[i] * f;
-        z[i] = g[i] * up * df;
+        const float x = (float)z.v[i], g = (float)d.v[i];
+        gate_of<T, ACT>(x, s, dt);
+        const float p = s * (1.0f - s);
+        const float df = p == 0.0f ? s : s + x * p * dt;  // far from 0, where x dt may be infinite, sigma
+        du[i] = g * (x * s);
+        dg[i] = g * (GATED ? (float)w.v[i] : 1.0f) * df;
     }
-    store_run<T, 8>((T*)a.dgate.p + t * a.dgate.ld + e0, n, z);
-    if constexpr (GATED) store_run<T, 8>((T*)a.dup.p + t * a.dup.ld + e0, n, v);
+    store_run<ONCE, T, 8>((T*)a.dgate.p + t * a.dgate.ld + e0, n, dg);
+    if constexpr (GATED) store_run<ONCE, T, 8>((T*)a.dup.p + t * a.dup.ld + e0, n, du);
 }
 
-__device__ __forceinline__ uint32_t row_max(uint32_t b) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// f(gate) up of a run, rotated (RUN 16).
+template <typename T, int ACT, bool GATED, int RUN>
+__device__ __forceinline__ void values_of(const Run<T, RUN>& z, const Run<T, RUN>& w, int G, int lane, float* v) {
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) b = max(b, (uint32_t)__shfl_xor((int)b, m, 64));
-    __shared__ uint32_t tops[16];
-    if (lane == 0) tops[wave] = b;
-    __syncthreads();
-    for (int i = 0; i < waves; ++i) b = max(b, tops[i]);
-    return b;
+    for (int i = 0; i < RUN; ++i) {
+        float s, dt;
+        gate_of<T, ACT>((float)z.v[i], s, dt);
+        v[i] = (float)z.v[i] * s;
+        if constexpr (GATED) v[i] *= (float)w.v[i];
+    }
+    if constexpr (RUN == 16) rotate_run(v, G, lane);
 }
 
-// A row a workgroup, SLOTS runs of RUN values a thread (RUN 16: rotated); SLOTS 0: rows of any length, read twice.
-template <typename T, int ACT, bool GATED, int RUN, int SLOTS>
-__global__ __launch_bounds__(1024) void gated_act_int8_kernel(GatedActArgs a, int64_t t0) {
-    const int per = blockDim.x, at = threadIdx.x, lane = threadIdx.x & 63;
-    const int64_t t = t0 + blockIdx.x;
-    const T* gate = (const T*)a.gate.p + t * a.gate.ld;
-    const T* up = GATED ? (const T*)a.up.p + t * a.up.ld : nullptr;
-    auto value = [&](int e0, float* v) {
-        const int n = a.W - e0;
-        float z[RUN];
-        load_run<T, RUN>(gate + e0, n, z);
-        if constexpr (GATED) load_run<T, RUN>(up + e0, n, v);
+template <typename T, int ACT, bool GATED, int RUN, int SLOTS, bool ONCE>
+__global__ __launch_bounds__(1024, 6) void gated_act_int8_kernel(GatedActArgs a, int64_t t0, int per, int groups) {
+    const Group g(per);
+    const int64_t t = t0 + (int64_t)blockIdx.x * groups + g.wave / g.waves;
+    const bool live = t < a.T;
+    Run<T, RUN> z[SLOTS], w[SLOTS];
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-            float s, dt;
-            gate_of<T, ACT>(z[i], s, dt);
-            const float f = z[i] * s;
-            v[i] = GATED ? f * v[i] : f;
-        }
-        if constexpr (RUN == 16) rotate_run(v, a.G, lane);
-    };
+    for (int s = 0; s < SLOTS; ++s) {
+        const int e0 = (s * per + g.at) * RUN, n = live ? a.W - e0 : 0;
+        z[s] = load_raw<ONCE, T, RUN>((const T*)a.gate.p + t * a.gate.ld + e0, n);
+        if constexpr (GATED) w[s] = load_raw<ONCE, T, RUN>((const T*)a.up.p + t * a.up.ld + e0, n);
+    }
+    float v[SLOTS][RUN], none = 0.0f;
     uint32_t top = 0;
-    float inv, first;
-    auto finish = [&] {
-        top = row_max(top);
-        inv = code_factor(__uint_as_float(top), first);
-        if (at == 0) a.scale[t] = __uint_as_float(top) / 127.0f;
-    };
-    auto emit = [&](int e0, float* v) {
-        if (first != 1.0f)
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        values_of<T, ACT, GATED, RUN>(z[s], w[s], a.G, g.lane, v[s]);
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[s][i]));
+    }
+    g.sums(none, top, 0, [](uint32_t p, uint32_t q) { return max(p, q); });
+    if (!live) return;
+    float first;
+    const float inv = code_factor(__uint_as_float(top), first);
+    if (g.at == 0) a.scale[t] = __uint_as_float(top) / 127.0f;
+    if (first != 1.0f)
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) v[s][i] *= first;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        const int e0 = (s * per + g.at) * RUN;
+        if (e0 < a.W) store_codes<ONCE, RUN>(a.q + t * a.ldq + e0, a.W - e0, v[s], inv);
+    }
+}
+
+// Rows of any length, read twice.
+template <typename T, int ACT, bool GATED, int RUN>
+__global__ __launch_bounds__(512) void gated_act_int8_long_kernel(GatedActArgs a) {
+    const Group g(512);
+    int turn = 0;
+    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
+        const T *gate = (const T*)a.gate.p + t * a.gate.ld, *up = GATED ? (const T*)a.up.p + t * a.up.ld : nullptr;
+        float v[RUN], none = 0.0f;
+        uint32_t top = 0;
+        auto value = [&](int e0) {
+            const auto z = load_raw<false, T, RUN>(gate + e0, a.W - e0);
+            Run<T, RUN> w;
+            if constexpr (GATED) w = load_raw<false, T, RUN>(up + e0, a.W - e0);
+            values_of<T, ACT, GATED, RUN>(z, w, a.G, g.lane, v);
+        };
+        for (int c = 0; c < a.W; c += 512 * RUN) {
+            value(c + g.at * RUN);
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[i]));
+        }
+        g.sums(none, top, turn, [](uint32_t p, uint32_t q) { return max(p, q); });
+        float first;
+        const float inv = code_factor(__uint_as_float(top), first);
+        if (g.at == 0) a.scale[t] = __uint_as_float(top) / 127.0f;
+        for (int c = 0; c < a.W; c += 512 * RUN) {
+            const int e0 = c + g.at * RUN;
+            value(e0);
 #pragma unroll
             for (int i = 0; i < RUN; ++i) v[i] *= first;
-        if (e0 < a.W) store_codes<RUN>(a.q + t * a.ldq + e0, a.W - e0, v, inv);
-    };
-    auto largest = [&](const float* v) {
-#pragma unroll
-        for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[i]));
-    };
-    if constexpr (SLOTS > 0) {
-        float v[SLOTS][RUN];
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            value((s * per + at) * RUN, v[s]);
-            largest(v[s]);
-        }
-        finish();
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) emit((s * per + at) * RUN, v[s]);
-    } else {
-        float v[RUN];
-        for (int c = 0; c < a.W; c += per * RUN) {
-            value(c + at * RUN, v);
-            largest(v);
-        }
-        finish();
-        for (int c = 0; c < a.W; c += per * RUN) {
-            value(c + at * RUN, v);
-            emit(c + at * RUN, v);
+            if (e0 < a.W) store_codes<false, RUN>(a.q + t * a.ldq + e0, a.W - e0, v, inv);
         }
     }
 }
@@ -162,6 +173,11 @@ hipError_t by_kind(const GatedActArgs& a, F&& f) {
     };
     if (a.dtype == DT_F32) return acts.template operator()<float>();
     return a.dtype == DT_F16 ? acts.template operator()<f16>() : acts.template operator()<__bf16>();
+}
+
+template <typename T>
+bool once_of(const GatedActArgs& a, int tensors) {
+    return a.T * a.W * (int64_t)sizeof(T) * tensors > ONCE_BYTES && aligned(a.gate, sizeof(T)) && aligned(a.up, sizeof(T)) && aligned(a.y, sizeof(T));
 }
 
 // f(first row, units, units a row) over parts of fewer than 2^31 units of 8 values.
@@ -179,20 +195,17 @@ hipError_t by_units(const GatedActArgs& a, F&& f) {
 
 template <typename T, int ACT, bool GATED, int RUN>
 hipError_t launch_int8(const GatedActArgs& a, hipStream_t st) {
-    int slots = 0;
-    const int n = row_threads(a.W, RUN, slots);
-    const int64_t most = (int64_t)(0x7FFFFFFF / n);
-    for (int64_t t0 = 0; t0 < a.T; t0 += most) {
-        const dim3 grid((unsigned)std::min<int64_t>(most, a.T - t0)), block((unsigned)n);
-        switch (slots) {
-            case 1: hipLaunchKernelGGL((gated_act_int8_kernel<T, ACT, GATED, RUN, 1>), grid, block, 0, st, a, t0); break;
-            case 2: hipLaunchKernelGGL((gated_act_int8_kernel<T, ACT, GATED, RUN, 2>), grid, block, 0, st, a, t0); break;
-            default: hipLaunchKernelGGL((gated_act_int8_kernel<T, ACT, GATED, RUN, 0>), grid, block, 0, st, a, t0); break;
-        }
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+    const RowCut c = cut_rows(a.T, a.W, RUN, 0);
+    if (!c.slots) {
+        hipLaunchKernelGGL((gated_act_int8_long_kernel<T, ACT, GATED, RUN>), dim3(c.grid), c.block(), 0, st, a);
+        return hipGetLastError();
     }
-    return hipSuccess;
+    const bool once = once_of<T>(a, GATED ? 2 : 1) && aligned({a.q, a.ldq}, 1);
+    return by_parts(c, a.T, [&](dim3 grid, int64_t t0) {
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, c.block(), 0, st, a, t0, c.per, c.groups); };
+        if (c.slots == 1) once ? go(gated_act_int8_kernel<T, ACT, GATED, RUN, 1, true>) : go(gated_act_int8_kernel<T, ACT, GATED, RUN, 1, false>);
+        else if constexpr (RUN == 8) once ? go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, false>);
+    });
 }
 
 }  // namespace
@@ -201,8 +214,10 @@ hipError_t run_gated_act(const GatedActArgs& a, hipStream_t st) {
     if (a.T == 0 || a.W == 0) return hipSuccess;
     return by_kind(a, [&]<typename T, int ACT, bool GATED>() {
         if (a.q) return a.G ? launch_int8<T, ACT, GATED, 16>(a, st) : launch_int8<T, ACT, GATED, 8>(a, st);
+        const bool once = once_of<T>(a, GATED ? 2 : 1);
         return by_units(a, [&](dim3 grid, int64_t t0, uint32_t units, uint32_t per) {
-            hipLaunchKernelGGL((gated_act_kernel<T, ACT, GATED>), grid, dim3(256), 0, st, a, t0, units, per);
+            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a, t0, units, per); };
+            once ? go(gated_act_kernel<T, ACT, GATED, true>) : go(gated_act_kernel<T, ACT, GATED, false>);
         });
     });
 }
@@ -210,8 +225,10 @@ hipError_t run_gated_act(const GatedActArgs& a, hipStream_t st) {
 hipError_t run_gated_act_grad(const GatedActArgs& a, hipStream_t st) {
     if (a.T == 0 || a.W == 0) return hipSuccess;
     return by_kind(a, [&]<typename T, int ACT, bool GATED>() {
+        const bool once = once_of<T>(a, GATED ? 3 : 2) && aligned(a.dy, sizeof(T)) && aligned(a.dgate, sizeof(T)) && aligned(a.dup, sizeof(T));
         return by_units(a, [&](dim3 grid, int64_t t0, uint32_t units, uint32_t per) {
-            hipLaunchKernelGGL((gated_act_grad_kernel<T, ACT, GATED>), grid, dim3(256), 0, st, a, t0, units, per);
+            auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a, t0, units, per); };
+            once ? go(gated_act_grad_kernel<T, ACT, GATED, true>) : go(gated_act_grad_kernel<T, ACT, GATED, false>);
         });
     });
 }
