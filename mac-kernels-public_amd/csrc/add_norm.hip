@@ -11,37 +11,43 @@
 namespace qlin {
 namespace {
 
-// T: x and y, H: the residual and h.  RUN 16: rotated.  RES: with a residual.  ONCE: nontemporal reads and writes.
+// T: x and y, H: the residual and h.  RUN 4: rotated.  RES: with a residual.  ONCE: nontemporal reads and writes.
 template <typename T, typename H, int RUN, int SLOTS, bool INT8, bool RES, bool ONCE>
 __global__ __launch_bounds__(1024, 6) void add_norm_kernel(AddNormArgs a, int64_t t0, int per, int groups) {
     const Group g(per);
+    const Rotation turned(RUN == 4 ? a.G : 1, g.lane);
     const int64_t t = t0 + (int64_t)blockIdx.x * groups + g.wave / g.waves;
     const bool live = t < a.T;
+    const int64_t from = live ? t : a.T - 1;
+    const int e0 = g.place<RUN>(), apart = per * RUN;
     Run<T, RUN> x[SLOTS];
     Run<H, RUN> r[SLOTS];
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const int e0 = (s * per + g.at) * RUN, n = live ? a.W - e0 : 0;
-        x[s] = load_raw<ONCE, T, RUN>((const T*)a.x.p + t * a.x.ld + e0, n);
-        if constexpr (RES) r[s] = load_raw<ONCE, H, RUN>((const H*)a.r.p + t * a.r.ld + e0, n);
+        x[s] = load_piece<ONCE, T, RUN>((const T*)a.x.p + from * a.x.ld, e0 + s * apart, a.W);
+        if constexpr (RES) r[s] = load_piece<ONCE, H, RUN>((const H*)a.r.p + from * a.r.ld, e0 + s * apart, a.W);
     }
-    float v[SLOTS][RUN];
+    float v[SLOTS][RUN], w[SLOTS][RUN];
+    if (a.w) load_pieces_rt<RUN, SLOTS>(a.w, a.w_dt, e0, apart, a.W, w);
     float ss = 0.0f;
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const int e0 = (s * per + g.at) * RUN;
-        float w[RUN];
-        if (a.w) load_run_rt<RUN>(a.w, a.w_dt, e0, a.W - e0, w);
+        const int e = e0 + s * apart;
+        trimmed<T, RUN>(x[s], e, a.W, v[s]);
+        if constexpr (RES) {
+            float u[RUN];
+            trimmed<H, RUN>(r[s], e, a.W, u);
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) v[s][i] = RES ? (float)x[s].v[i] + (float)r[s].v[i] : (float)x[s].v[i];
-        if (RES && live && e0 < a.W) store_run<ONCE, H, RUN>((H*)a.h.p + t * a.h.ld + e0, a.W - e0, v[s]);
+            for (int i = 0; i < RUN; ++i) v[s][i] += u[i];
+            if (live && e < a.W) store_run<ONCE, H, RUN>((H*)a.h.p + t * a.h.ld + e, a.W - e, v[s]);
+        }
 #pragma unroll
         for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[s][i], v[s][i], ss);
         if (a.w)
 #pragma unroll
-            for (int i = 0; i < RUN; ++i) v[s][i] *= w[i];
-        if constexpr (INT8 && RUN == 16) rotate_run(v[s], a.G, g.lane);
+            for (int i = 0; i < RUN; ++i) v[s][i] *= w[s][i];
+        if constexpr (RUN == 4) turned(v[s]);
         if constexpr (INT8)
 #pragma unroll
             for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[s][i]));
@@ -53,7 +59,7 @@ __global__ __launch_bounds__(1024, 6) void add_norm_kernel(AddNormArgs a, int64_
         const float most = __uint_as_float(top);
         float first;
         const float inv = code_factor(most, first);
-        if (g.at == 0) a.scale[t] = most / 127.0f * rho;
+        if (g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.norm : 1.0f) / 127.0f * rho;
         if (first != 1.0f)
 #pragma unroll
             for (int s = 0; s < SLOTS; ++s)
@@ -61,16 +67,16 @@ __global__ __launch_bounds__(1024, 6) void add_norm_kernel(AddNormArgs a, int64_
                 for (int i = 0; i < RUN; ++i) v[s][i] *= first;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + g.at) * RUN;
-            if (e0 < a.W) store_codes<ONCE, RUN>(a.q + t * a.ldq + e0, a.W - e0, v[s], inv);
+            const int e = e0 + s * apart;
+            if (e < a.W) store_codes<ONCE, RUN>(a.q + t * a.ldq + e, a.W - e, v[s], inv);
         }
     } else {
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + g.at) * RUN;
+            const int e = e0 + s * apart;
 #pragma unroll
             for (int i = 0; i < RUN; ++i) v[s][i] *= rho;
-            if (e0 < a.W) store_run<ONCE, T, RUN>((T*)a.y.p + t * a.y.ld + e0, a.W - e0, v[s]);
+            if (e < a.W) store_run<ONCE, T, RUN>((T*)a.y.p + t * a.y.ld + e, a.W - e, v[s]);
         }
     }
 }
@@ -79,6 +85,7 @@ __global__ __launch_bounds__(1024, 6) void add_norm_kernel(AddNormArgs a, int64_
 template <typename T, typename H, int RUN, bool INT8>
 __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
     const Group g(512);
+    const Rotation turned(RUN == 4 ? a.G : 1, g.lane);
     int turn = 0;
     for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
         const T* x = (const T*)a.x.p + t * a.x.ld;
@@ -100,12 +107,12 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
 #pragma unroll
                 for (int i = 0; i < RUN; ++i) v[i] *= u[i];
             }
-            if constexpr (INT8 && RUN == 16) rotate_run(v, a.G, g.lane);
+            if constexpr (RUN == 4) turned(v);
         };
         float ss = 0.0f;
         uint32_t top = 0;
         for (int c = 0; c < a.W; c += 512 * RUN) {
-            const int e0 = c + g.at * RUN;
+            const int e0 = c + g.place<RUN>();
             sum_of(e0);
 #pragma unroll
             for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
@@ -119,9 +126,9 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps), most = __uint_as_float(top);
         float first = 1.0f;
         const float inv = INT8 ? code_factor(most, first) : 0.0f;
-        if (INT8 && g.at == 0) a.scale[t] = most / 127.0f * rho;
+        if (INT8 && g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.norm : 1.0f) / 127.0f * rho;
         for (int c = 0; c < a.W; c += 512 * RUN) {
-            const int e0 = c + g.at * RUN;
+            const int e0 = c + g.place<RUN>();
             sum_of(e0);
             if (r && e0 < a.W) store_run<false, H, RUN>((H*)a.h.p + t * a.h.ld + e0, a.W - e0, v);
             weigh(e0);
@@ -143,14 +150,14 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
         Run<T, RUN> dy;
         Run<H, RUN> h, dh;
     };
+    const int e0 = g.at * RUN, apart = per * RUN;
     auto fetch = [&](int64_t t, Raw (&o)[SLOTS]) {
+        t = min(t, a.T - 1);
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + g.at) * RUN;
-            const int n = t < a.T ? a.W - e0 : 0;
-            o[s].dy = load_raw<ONCE, T, RUN>((const T*)a.dy.p + t * a.dy.ld + e0, n);
-            o[s].h = load_raw<ONCE, H, RUN>((const H*)a.h.p + t * a.h.ld + e0, n);
-            if constexpr (DH) o[s].dh = load_raw<ONCE, H, RUN>((const H*)a.dh.p + t * a.dh.ld + e0, n);
+            o[s].dy = load_piece<ONCE, T, RUN>((const T*)a.dy.p + t * a.dy.ld, e0 + s * apart, a.W);
+            o[s].h = load_piece<ONCE, H, RUN>((const H*)a.h.p + t * a.h.ld, e0 + s * apart, a.W);
+            if constexpr (DH) o[s].dh = load_piece<ONCE, H, RUN>((const H*)a.dh.p + t * a.dh.ld, e0 + s * apart, a.W);
         }
     };
     const int64_t step = (int64_t)gridDim.x * groups;
@@ -158,30 +165,32 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
     Raw raw[SLOTS];
     fetch(t, raw);
     float w[SLOTS][RUN], dw[SLOTS][RUN];
+    if (a.w) load_pieces_rt<RUN, SLOTS>(a.w, a.w_dt, e0, apart, a.W, w);
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-        const int e0 = (s * per + g.at) * RUN;
-        if (a.w) load_run_rt<RUN>(a.w, a.w_dt, e0, a.W - e0, w[s]);
+    for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
         for (int i = 0; i < RUN; ++i) {
             if (!a.w) w[s][i] = 1.0f;
             dw[s][i] = 0.0f;
         }
-    }
     int turn = 0;
     for (int64_t base = (int64_t)blockIdx.x * groups; base < a.T; base += step, t += step, turn ^= 1) {
-        Raw now[SLOTS];
+        float d[SLOTS][RUN], h[SLOTS][RUN];
+        Run<H, RUN> dh[SLOTS];
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) now[s] = raw[s];
-        fetch(t + step, raw);
+        for (int s = 0; s < SLOTS; ++s) {
+            trimmed<T, RUN>(raw[s].dy, e0 + s * apart, a.W, d[s]);
+            trimmed<H, RUN>(raw[s].h, e0 + s * apart, a.W, h[s]);
+            if constexpr (DH) dh[s] = raw[s].dh;
+        }
+        if (base + step < a.T) fetch(t + step, raw);
         float ss = 0.0f, gh = 0.0f;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                const float h = (float)now[s].h.v[i];
-                ss = __builtin_fmaf(h, h, ss);
-                gh = __builtin_fmaf((float)now[s].dy.v[i] * w[s][i], h, gh);
+                ss = __builtin_fmaf(h[s][i], h[s][i], ss);
+                gh = __builtin_fmaf(d[s][i] * w[s][i], h[s][i], gh);
             }
         g.sums(ss, gh, turn, [](float p, float q) { return p + q; });
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
@@ -189,16 +198,16 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
         if (t >= a.T) continue;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            const int e0 = (s * per + g.at) * RUN;
-            float o[RUN];
+            const int e = e0 + s * apart;
+            float o[RUN], more[RUN];
+            if constexpr (DH) trimmed<H, RUN>(dh[s], e, a.W, more);
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                const float d = (float)now[s].dy.v[i], h = (float)now[s].h.v[i];
-                dw[s][i] = __builtin_fmaf(d, h * rho, dw[s][i]);
-                o[i] = rho * (d * w[s][i] - h * c);
-                if constexpr (DH) o[i] += (float)now[s].dh.v[i];
+                dw[s][i] = __builtin_fmaf(d[s][i], h[s][i] * rho, dw[s][i]);
+                o[i] = rho * (d[s][i] * w[s][i] - h[s][i] * c);
+                if constexpr (DH) o[i] += more[i];
             }
-            if (e0 < a.W) store_run<ONCE, H, RUN>((H*)a.dx.p + t * a.dx.ld + e0, a.W - e0, o);
+            if (e < a.W) store_run<ONCE, H, RUN>((H*)a.dx.p + t * a.dx.ld + e, a.W - e, o);
         }
     }
     if (!a.dw) return;
@@ -217,8 +226,8 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
     if (g.wave / g.waves) return;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const int e0 = (s * per + g.at) * RUN;
-        if (e0 < a.W) store_run<false, float, RUN>(a.part + (int64_t)blockIdx.x * a.W + e0, a.W - e0, dw[s]);
+        const int e = e0 + s * apart;
+        if (e < a.W) store_run<false, float, RUN>(a.part + (int64_t)blockIdx.x * a.W + e, a.W - e, dw[s]);
     }
 }
 
@@ -288,11 +297,12 @@ hipError_t launch_norm(const AddNormArgs& a, hipStream_t st) {
     }
     const bool pieces = aligned(a.x, sizeof(T)) && aligned(a.r, sizeof(H)) && aligned(a.y, sizeof(T)) && aligned(a.h, sizeof(H)) &&
                         aligned({a.q, a.ldq}, 1);
-    const bool once = pieces && a.T * a.W * (int64_t)(sizeof(T) + (RES ? sizeof(H) : 0)) > ONCE_BYTES;
+    const bool once = pieces && a.W % RUN == 0 && a.T * a.W * (int64_t)(sizeof(T) + (RES ? sizeof(H) : 0)) > ONCE_BYTES;
     return by_parts(c, a.T, [&](dim3 grid, int64_t t0) {
         auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, c.block(), 0, st, a, t0, c.per, c.groups); };
-        if (c.slots == 1) once ? go(add_norm_kernel<T, H, RUN, 1, INT8, RES, true>) : go(add_norm_kernel<T, H, RUN, 1, INT8, RES, false>);
-        else if constexpr (RUN == 8) once ? go(add_norm_kernel<T, H, 8, 2, INT8, RES, true>) : go(add_norm_kernel<T, H, 8, 2, INT8, RES, false>);
+        if (RUN == 8 && c.slots == 1) once ? go(add_norm_kernel<T, H, 8, 1, INT8, RES, true>) : go(add_norm_kernel<T, H, 8, 1, INT8, RES, false>);
+        else if constexpr (RUN == 4) once ? go(add_norm_kernel<T, H, 4, 4, INT8, RES, true>) : go(add_norm_kernel<T, H, 4, 4, INT8, RES, false>);
+        else once ? go(add_norm_kernel<T, H, 8, 2, INT8, RES, true>) : go(add_norm_kernel<T, H, 8, 2, INT8, RES, false>);
     });
 }
 
@@ -302,13 +312,13 @@ hipError_t norm_of(const AddNormArgs& a, hipStream_t st) {
         return a.r.p ? launch_norm<T, H, RUN, INT8, true>(a, st) : launch_norm<T, H, RUN, INT8, false>(a, st);
     };
     if (!a.q) return by_res.template operator()<8, false>();
-    return a.G ? by_res.template operator()<16, true>() : by_res.template operator()<8, true>();
+    return a.G ? by_res.template operator()<4, true>() : by_res.template operator()<8, true>();
 }
 
 template <typename T, typename H>
 hipError_t grad_of(const AddNormGradArgs& a, hipStream_t st) {
     const RowCut c = grad_cut(a.T, a.W);
-    const bool once = a.T * a.W * (int64_t)(sizeof(T) + sizeof(H)) > ONCE_BYTES && aligned(a.dy, sizeof(T)) && aligned(a.h, sizeof(H)) &&
+    const bool once = a.W % 8 == 0 && a.T * a.W * (int64_t)(sizeof(T) + sizeof(H)) > ONCE_BYTES && aligned(a.dy, sizeof(T)) && aligned(a.h, sizeof(H)) &&
                       aligned(a.dh, sizeof(H)) && aligned(a.dx, sizeof(H));
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(c.grid), c.block(), 0, st, a, c.per, c.groups); };
     auto by_slots = [&]<int SLOTS, int THREADS>() {

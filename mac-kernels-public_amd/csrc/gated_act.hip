@@ -31,26 +31,39 @@ __device__ __forceinline__ void gate_of(float z, float& s, float& dt) {
         dt = GELU_C * __builtin_fmaf(3.0f * GELU_A, z2, 1.0f);
     }
 }
+// Where a thread of an elementwise kernel works: 8 values of a row.  Rows shorter than that are read value by value.
+template <bool ONCE, typename T>
+struct Values {
+    Run<T, 8> r;
+    const T* row;
+    __device__ __forceinline__ Values(const RowView& v, int64_t t, int e0, int W) : row((const T*)v.p + t * v.ld) {
+        if (W >= 8) r = load_piece<ONCE, T, 8>(row, e0, W);
+    }
+    __device__ __forceinline__ void to(int e0, int W, float* v) const {
+        if (W >= 8) trimmed<T, 8>(r, e0, W, v);
+        else load_run<T, 8>(row + e0, W - e0, v);
+    }
+};
+
 // y = f(gate) up, 8 values a thread.  ONCE: nontemporal reads and writes.
 template <typename T, int ACT, bool GATED, bool ONCE>
 __global__ __launch_bounds__(256) void gated_act_kernel(GatedActArgs a, int64_t t0, uint32_t units, uint32_t per) {
     const uint32_t u = blockIdx.x * 256u + threadIdx.x;
     if (u >= units) return;
     const uint32_t row = u / per;
-    const int e0 = (int)(u - row * per) * 8, n = a.W - e0;
+    const int e0 = (int)(u - row * per) * 8;
     const int64_t t = t0 + row;
-    const auto z = load_raw<ONCE, T, 8>((const T*)a.gate.p + t * a.gate.ld + e0, n);
-    Run<T, 8> w;
-    if constexpr (GATED) w = load_raw<ONCE, T, 8>((const T*)a.up.p + t * a.up.ld + e0, n);
-    float v[8];
+    const Values<ONCE, T> gate(a.gate, t, e0, a.W), up(GATED ? a.up : a.gate, t, e0, a.W);
+    float z[8], v[8];
+    gate.to(e0, a.W, z);
+    if constexpr (GATED) up.to(e0, a.W, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float s, dt;
-        gate_of<T, ACT>((float)z.v[i], s, dt);
-        v[i] = (float)z.v[i] * s;
-        if constexpr (GATED) v[i] *= (float)w.v[i];
+        gate_of<T, ACT>(z[i], s, dt);
+        v[i] = GATED ? z[i] * s * v[i] : z[i] * s;
     }
-    store_run<ONCE, T, 8>((T*)a.y.p + t * a.y.ld + e0, n, v);
+    store_run<ONCE, T, 8>((T*)a.y.p + t * a.y.ld + e0, a.W - e0, v);
 }
 
 template <typename T, int ACT, bool GATED, bool ONCE>
@@ -58,57 +71,60 @@ __global__ __launch_bounds__(256) void gated_act_grad_kernel(GatedActArgs a, int
     const uint32_t u = blockIdx.x * 256u + threadIdx.x;
     if (u >= units) return;
     const uint32_t row = u / per;
-    const int e0 = (int)(u - row * per) * 8, n = a.W - e0;
+    const int e0 = (int)(u - row * per) * 8;
     const int64_t t = t0 + row;
-    const auto z = load_raw<ONCE, T, 8>((const T*)a.gate.p + t * a.gate.ld + e0, n);
-    Run<T, 8> w;
-    if constexpr (GATED) w = load_raw<ONCE, T, 8>((const T*)a.up.p + t * a.up.ld + e0, n);
-    const auto d = load_raw<ONCE, T, 8>((const T*)a.dy.p + t * a.dy.ld + e0, n);
-    float dg[8], du[8];
+    const Values<ONCE, T> gate(a.gate, t, e0, a.W), up(GATED ? a.up : a.gate, t, e0, a.W), dy(a.dy, t, e0, a.W);
+    float z[8], v[8], g[8];
+    gate.to(e0, a.W, z);
+    if constexpr (GATED) up.to(e0, a.W, v);
+    dy.to(e0, a.W, g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float s, dt;
-        const float x = (float)z.v[i], g = (float)d.v[i];
-        gate_of<T, ACT>(x, s, dt);
-        const float p = s * (1.0f - s);
-        const float df = p == 0.0f ? s : s + x * p * dt;  // far from 0, where x dt may be infinite, sigma
-        du[i] = g * (x * s);
-        dg[i] = g * (GATED ? (float)w.v[i] : 1.0f) * df;
+        gate_of<T, ACT>(z[i], s, dt);
+        const float p = s * (1.0f - s), f = z[i] * s;
+        const float df = p == 0.0f ? s : s + z[i] * p * dt;  // far from 0, where z dt may be infinite, sigma
+        z[i] = g[i] * (GATED ? v[i] : 1.0f) * df;
+        v[i] = g[i] * f;
     }
-    store_run<ONCE, T, 8>((T*)a.dgate.p + t * a.dgate.ld + e0, n, dg);
-    if constexpr (GATED) store_run<ONCE, T, 8>((T*)a.dup.p + t * a.dup.ld + e0, n, du);
+    store_run<ONCE, T, 8>((T*)a.dgate.p + t * a.dgate.ld + e0, a.W - e0, z);
+    if constexpr (GATED) store_run<ONCE, T, 8>((T*)a.dup.p + t * a.dup.ld + e0, a.W - e0, v);
 }
 
-// f(gate) up of a run, rotated (RUN 16).
+// f(z) w of a run into w, rotated (RUN 4).
 template <typename T, int ACT, bool GATED, int RUN>
-__device__ __forceinline__ void values_of(const Run<T, RUN>& z, const Run<T, RUN>& w, int G, int lane, float* v) {
+__device__ __forceinline__ void values_of(const float* z, float* w, const Rotation& turned) {
 #pragma unroll
     for (int i = 0; i < RUN; ++i) {
         float s, dt;
-        gate_of<T, ACT>((float)z.v[i], s, dt);
-        v[i] = (float)z.v[i] * s;
-        if constexpr (GATED) v[i] *= (float)w.v[i];
+        gate_of<T, ACT>(z[i], s, dt);
+        w[i] = GATED ? z[i] * s * w[i] : z[i] * s;
     }
-    if constexpr (RUN == 16) rotate_run(v, G, lane);
+    if constexpr (RUN == 4) turned(w);
 }
 
 template <typename T, int ACT, bool GATED, int RUN, int SLOTS, bool ONCE>
 __global__ __launch_bounds__(1024, 6) void gated_act_int8_kernel(GatedActArgs a, int64_t t0, int per, int groups) {
     const Group g(per);
+    const Rotation turned(RUN == 4 ? a.G : 1, g.lane);
     const int64_t t = t0 + (int64_t)blockIdx.x * groups + g.wave / g.waves;
     const bool live = t < a.T;
-    Run<T, RUN> z[SLOTS], w[SLOTS];
+    const int64_t from = live ? t : a.T - 1;
+    const int e0 = g.place<RUN>(), apart = per * RUN;
+    Run<T, RUN> gate[SLOTS], up[SLOTS];
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const int e0 = (s * per + g.at) * RUN, n = live ? a.W - e0 : 0;
-        z[s] = load_raw<ONCE, T, RUN>((const T*)a.gate.p + t * a.gate.ld + e0, n);
-        if constexpr (GATED) w[s] = load_raw<ONCE, T, RUN>((const T*)a.up.p + t * a.up.ld + e0, n);
+        gate[s] = load_piece<ONCE, T, RUN>((const T*)a.gate.p + from * a.gate.ld, e0 + s * apart, a.W);
+        if constexpr (GATED) up[s] = load_piece<ONCE, T, RUN>((const T*)a.up.p + from * a.up.ld, e0 + s * apart, a.W);
     }
     float v[SLOTS][RUN], none = 0.0f;
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        values_of<T, ACT, GATED, RUN>(z[s], w[s], a.G, g.lane, v[s]);
+        float z[RUN];
+        trimmed<T, RUN>(gate[s], e0 + s * apart, a.W, z);
+        if constexpr (GATED) trimmed<T, RUN>(up[s], e0 + s * apart, a.W, v[s]);
+        values_of<T, ACT, GATED, RUN>(z, v[s], turned);
 #pragma unroll
         for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[s][i]));
     }
@@ -116,7 +132,7 @@ __global__ __launch_bounds__(1024, 6) void gated_act_int8_kernel(GatedActArgs a,
     if (!live) return;
     float first;
     const float inv = code_factor(__uint_as_float(top), first);
-    if (g.at == 0) a.scale[t] = __uint_as_float(top) / 127.0f;
+    if (g.at == 0) a.scale[t] = __uint_as_float(top) * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
     if (first != 1.0f)
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s)
@@ -124,8 +140,8 @@ __global__ __launch_bounds__(1024, 6) void gated_act_int8_kernel(GatedActArgs a,
             for (int i = 0; i < RUN; ++i) v[s][i] *= first;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const int e0 = (s * per + g.at) * RUN;
-        if (e0 < a.W) store_codes<ONCE, RUN>(a.q + t * a.ldq + e0, a.W - e0, v[s], inv);
+        const int e = e0 + s * apart;
+        if (e < a.W) store_codes<ONCE, RUN>(a.q + t * a.ldq + e, a.W - e, v[s], inv);
     }
 }
 
@@ -133,28 +149,29 @@ __global__ __launch_bounds__(1024, 6) void gated_act_int8_kernel(GatedActArgs a,
 template <typename T, int ACT, bool GATED, int RUN>
 __global__ __launch_bounds__(512) void gated_act_int8_long_kernel(GatedActArgs a) {
     const Group g(512);
+    const Rotation turned(RUN == 4 ? a.G : 1, g.lane);
     int turn = 0;
     for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
         const T *gate = (const T*)a.gate.p + t * a.gate.ld, *up = GATED ? (const T*)a.up.p + t * a.up.ld : nullptr;
         float v[RUN], none = 0.0f;
         uint32_t top = 0;
         auto value = [&](int e0) {
-            const auto z = load_raw<false, T, RUN>(gate + e0, a.W - e0);
-            Run<T, RUN> w;
-            if constexpr (GATED) w = load_raw<false, T, RUN>(up + e0, a.W - e0);
-            values_of<T, ACT, GATED, RUN>(z, w, a.G, g.lane, v);
+            float z[RUN];
+            load_run<T, RUN>(gate + e0, a.W - e0, z);
+            if constexpr (GATED) load_run<T, RUN>(up + e0, a.W - e0, v);
+            values_of<T, ACT, GATED, RUN>(z, v, turned);
         };
         for (int c = 0; c < a.W; c += 512 * RUN) {
-            value(c + g.at * RUN);
+            value(c + g.place<RUN>());
 #pragma unroll
             for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[i]));
         }
         g.sums(none, top, turn, [](uint32_t p, uint32_t q) { return max(p, q); });
         float first;
         const float inv = code_factor(__uint_as_float(top), first);
-        if (g.at == 0) a.scale[t] = __uint_as_float(top) / 127.0f;
+        if (g.at == 0) a.scale[t] = __uint_as_float(top) * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
         for (int c = 0; c < a.W; c += 512 * RUN) {
-            const int e0 = c + g.at * RUN;
+            const int e0 = c + g.place<RUN>();
             value(e0);
 #pragma unroll
             for (int i = 0; i < RUN; ++i) v[i] *= first;
@@ -177,7 +194,7 @@ hipError_t by_kind(const GatedActArgs& a, F&& f) {
 
 template <typename T>
 bool once_of(const GatedActArgs& a, int tensors) {
-    return a.T * a.W * (int64_t)sizeof(T) * tensors > ONCE_BYTES && aligned(a.gate, sizeof(T)) && aligned(a.up, sizeof(T)) && aligned(a.y, sizeof(T));
+    return a.W % 8 == 0 && a.T * a.W * (int64_t)sizeof(T) * tensors > ONCE_BYTES && aligned(a.gate, sizeof(T)) && aligned(a.up, sizeof(T)) && aligned(a.y, sizeof(T));
 }
 
 // f(first row, units, units a row) over parts of fewer than 2^31 units of 8 values.
@@ -203,8 +220,9 @@ hipError_t launch_int8(const GatedActArgs& a, hipStream_t st) {
     const bool once = once_of<T>(a, GATED ? 2 : 1) && aligned({a.q, a.ldq}, 1);
     return by_parts(c, a.T, [&](dim3 grid, int64_t t0) {
         auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, c.block(), 0, st, a, t0, c.per, c.groups); };
-        if (c.slots == 1) once ? go(gated_act_int8_kernel<T, ACT, GATED, RUN, 1, true>) : go(gated_act_int8_kernel<T, ACT, GATED, RUN, 1, false>);
-        else if constexpr (RUN == 8) once ? go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, false>);
+        if (RUN == 8 && c.slots == 1) once ? go(gated_act_int8_kernel<T, ACT, GATED, 8, 1, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 8, 1, false>);
+        else if constexpr (RUN == 4) once ? go(gated_act_int8_kernel<T, ACT, GATED, 4, 4, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 4, 4, false>);
+        else once ? go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, false>);
     });
 }
 
@@ -213,7 +231,7 @@ hipError_t launch_int8(const GatedActArgs& a, hipStream_t st) {
 hipError_t run_gated_act(const GatedActArgs& a, hipStream_t st) {
     if (a.T == 0 || a.W == 0) return hipSuccess;
     return by_kind(a, [&]<typename T, int ACT, bool GATED>() {
-        if (a.q) return a.G ? launch_int8<T, ACT, GATED, 16>(a, st) : launch_int8<T, ACT, GATED, 8>(a, st);
+        if (a.q) return a.G ? launch_int8<T, ACT, GATED, 4>(a, st) : launch_int8<T, ACT, GATED, 8>(a, st);
         const bool once = once_of<T>(a, GATED ? 2 : 1);
         return by_units(a, [&](dim3 grid, int64_t t0, uint32_t units, uint32_t per) {
             auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a, t0, units, per); };

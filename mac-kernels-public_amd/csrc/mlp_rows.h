@@ -2,41 +2,76 @@
 #pragma once
 #include <algorithm>
 
-#include "hadamard.h"
 #include "mlp.h"
 
 namespace qlin {
 
-// N values as they are in memory, rows of any alignment (global loads take any); zeros past the n-th.  ONCE: read
-// nontemporally, 16-byte aligned.
+// N values as they are in memory.
 template <typename T, int N>
 struct Run {
     T v[N];
 };
+// Values e0 .. e0 + N - 1 of a row of W >= N, at any alignment (global loads take any), without a branch, so that a thread's loads
+// are in flight together: a run that reaches past the row's end gets its last N values, which trimmed() puts right once
+// all loads have been issued.  ONCE: nontemporal, whole 16-byte (8-byte: RUN 4 of 16 bits) pieces.
 template <bool ONCE, typename T, int N>
-__device__ __forceinline__ Run<T, N> load_raw(const T* p, int n) {
+__device__ __forceinline__ Run<T, N> load_piece(const T* row, int e0, int W) {
+    const T* p = row + min(e0, W - N);
     Run<T, N> r;
-    if (n >= N) {
-        if constexpr (ONCE) {
-            constexpr int W = sizeof r / 16;
-            struct { u32x4 w[W]; } q;
+    if constexpr (ONCE) {
+        typedef uint32_t Words __attribute__((ext_vector_type(sizeof r % 16 ? 2 : 4)));
+        struct { Words w[sizeof r / sizeof(Words)]; } q;
 #pragma unroll
-            for (int i = 0; i < W; ++i) q.w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + i);
-            r = __builtin_bit_cast(Run<T, N>, q);
-        } else {
-            __builtin_memcpy(&r, p, sizeof r);
-        }
+        for (int i = 0; i < (int)(sizeof r / sizeof(Words)); ++i) q.w[i] = __builtin_nontemporal_load(reinterpret_cast<const Words*>(p) + i);
+        r = __builtin_bit_cast(Run<T, N>, q);
     } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
+        __builtin_memcpy(&r, p, sizeof r);
     }
     return r;
 }
+// A piece's values in fp32, zeros past the row's end.
 template <typename T, int N>
-__device__ __forceinline__ void load_run(const T* p, int n, float* v) {
-    const Run<T, N> r = load_raw<false, T, N>(p, n);
+__device__ __forceinline__ void trimmed(const Run<T, N>& r, int e0, int W, float* v) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)r.v[i];
+    if (e0 + N > W) {
+        const int d = e0 - (W - N);  // value i is the piece's i + d
+#pragma unroll
+        for (int step = 1; step < N; step *= 2)
+            if (d & step)
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = i + step < N ? v[i + step] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i + d < N ? v[i] : 0.0f;
+    }
+}
+// The same of a vector of float32, float16 or bfloat16, S pieces `apart` values from one another.
+template <int N, int S>
+__device__ __forceinline__ void load_pieces_rt(const void* p, int dt, int e0, int apart, int W, float (&v)[S][N]) {
+    auto of = [&]<typename T>() {
+        Run<T, N> r[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) r[s] = load_piece<false, T, N>((const T*)p, e0 + s * apart, W);
+#pragma unroll
+        for (int s = 0; s < S; ++s) trimmed<T, N>(r[s], e0 + s * apart, W, v[s]);
+    };
+    if (dt == DT_F32) of.template operator()<float>();
+    else if (dt == DT_F16) of.template operator()<f16>();
+    else of.template operator()<__bf16>();
+}
+
+// Rows of any length, short ones too.
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T* p, int n, float* v) {
+    if (n >= N) {
+        Run<T, N> r;
+        __builtin_memcpy(&r, p, sizeof r);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (float)r.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
+    }
 }
 template <int N>
 __device__ __forceinline__ void load_run_rt(const void* p, int dt, int64_t e0, int n, float* v) {
@@ -48,11 +83,11 @@ template <bool ONCE, typename T, int N>
 __device__ __forceinline__ void store_raw(T* p, int n, const Run<T, N>& r) {
     if (n >= N) {
         if constexpr (ONCE) {
-            constexpr int W = sizeof r / 16;
-            struct Words { u32x4 w[W]; };
-            const Words q = __builtin_bit_cast(Words, r);
+            typedef uint32_t Words __attribute__((ext_vector_type(sizeof r % 16 ? 2 : 4)));
+            struct Pieces { Words w[sizeof r / sizeof(Words)]; };
+            const Pieces q = __builtin_bit_cast(Pieces, r);
 #pragma unroll
-            for (int i = 0; i < W; ++i) __builtin_nontemporal_store(q.w[i], reinterpret_cast<u32x4*>(p) + i);
+            for (int i = 0; i < (int)(sizeof r / sizeof(Words)); ++i) __builtin_nontemporal_store(q.w[i], reinterpret_cast<Words*>(p) + i);
         } else {
             __builtin_memcpy(p, &r, sizeof r);
         }
@@ -89,8 +124,12 @@ __device__ __forceinline__ void store_codes(int8_t* p, int n, const float* v, fl
     }
     if (n >= N) {
         if constexpr (ONCE) {
-            typedef uint32_t Words __attribute__((ext_vector_type(N / 4)));
-            __builtin_nontemporal_store(__builtin_bit_cast(Words, r), reinterpret_cast<Words*>(p));
+            if constexpr (N == 4) {
+                __builtin_nontemporal_store(r.w[0], reinterpret_cast<uint32_t*>(p));
+            } else {
+                typedef uint32_t Words __attribute__((ext_vector_type(N / 4)));
+                __builtin_nontemporal_store(__builtin_bit_cast(Words, r), reinterpret_cast<Words*>(p));
+            }
         } else {
             __builtin_memcpy(p, &r, sizeof r);
         }
@@ -108,26 +147,67 @@ __device__ __forceinline__ float code_factor(float top, float& first) {
     return top > 0.0f ? 127.0f / (top * first) : 0.0f;
 }
 
-// A run of 16 values through the rotation of its group of G, shared by a wave's lanes.  (Stage after stage, each under a condition of
-// its own, the exchanges' latencies do not overlap: 9504 x 5120 to 8 bits 112 us against 74.)
-__device__ __forceinline__ void rotate_run(float* v, int G, int lane) {
-    float n = 1.0f;
-    auto by = [&]<int S>() {
-        hadamard16<S>(v, lane);
-        n = hadamard_norm<S>();
-    };
-    switch (G) {
-        case 4: by.template operator()<4>(); break;
-        case 8: by.template operator()<8>(); break;
-        case 16: by.template operator()<16>(); break;
-        case 32: by.template operator()<32>(); break;
-        case 64: by.template operator()<64>(); break;
-        case 128: by.template operator()<128>(); break;
-        default: by.template operator()<256>(); break;
+// The rotation of 256 values on the matrix cores.  As a 16 x 16 matrix V[a][b] of values 16 a + b they become M_a V M_b with M_b the
+// Hadamard matrix of the group's lowest (at most) two base-4 digits and M_a that of the higher ones, block diagonal where the
+// group is smaller than 256 values: entries 0, 1 and -1, exact in bf16.  Lane l holds values 16 (l % 16) + 4 (l / 16) .. + 3,
+// which are its part of V as the first operand; the product's registers, taken as a first operand again, are its transpose, and the
+// second product comes out in the layout of the values.  Unnormalized: by sqrt(G).
+//
+// A value enters a product as two bf16 parts of 8 bits each, off by 2^-18 of it.  Over both products that is at most 2^-17 of
+// the group's norm, so, the row's largest value being at least a 16th of that, 127 * 16 * 2^-17 < 0.016 steps of a code.  (In
+// fp32 across the lanes, 10 vector instructions and 3 LDS exchanges a value against 6, 9504 x 13824 took 157 us; see gated_act.hip.)
+typedef short bf16x4_bits __attribute__((ext_vector_type(4)));
+struct RotationTable {
+    uint64_t m[5][64];  // sizes 1, 2, 4, 8, 16: lane l's entries [4 (l / 16) + i][l % 16]
+    static constexpr int entry(int size, int r, int c) {
+        if (r / size != c / size) return 0;
+        r %= size;
+        c %= size;
+        int s = 1;
+        for (; size >= 4; size /= 4, r /= 4, c /= 4) s = r % 4 + c % 4 == 3 ? -s : s;
+        return size == 2 && r && c ? -s : s;
     }
+    constexpr RotationTable() : m() {
+        for (int k = 0; k < 5; ++k)
+            for (int l = 0; l < 64; ++l)
+                for (int i = 0; i < 4; ++i) {
+                    const int e = entry(1 << k, 4 * (l / 16) + i, l % 16);
+                    m[k][l] |= (uint64_t)(e == 0 ? 0 : e == 1 ? 0x3F80 : 0xBF80) << (16 * i);
+                }
+    }
+};
+__device__ const RotationTable rotation_table;
+
+struct Rotation {
+    bf16x4_bits low, high;  // M_b, M_a
+    float norm;
+    __device__ __forceinline__ Rotation(int G, int lane) {
+        const int k = 31 - __clz(G);
+        low = __builtin_bit_cast(bf16x4_bits, rotation_table.m[min(k, 4)][lane]);
+        high = __builtin_bit_cast(bf16x4_bits, rotation_table.m[max(k - 4, 0)][lane]);
+        norm = k % 2 ? 0.70710678118654752f / (float)(1 << (k / 2)) : 1.0f / (float)(1 << (k / 2));
+    }
+    static __device__ __forceinline__ f32x4 product(const f32x4 v, const bf16x4_bits m) {
+        typedef float F2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+        u32x2 hi, lo;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] *= n;
-}
+        for (int i = 0; i < 2; ++i) {  // two values an instruction, their parts side by side as the product takes them
+            const F2 a = {v[2 * i], v[2 * i + 1]};
+            hi[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(a, B2));
+            const F2 rest = {a.x - __uint_as_float(hi[i] << 16), a.y - __uint_as_float(hi[i] & 0xFFFF0000u)};
+            lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, B2));
+        }
+        f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+        d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, lo), m, d, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, hi), m, d, 0, 0, 0);
+    }
+    __device__ __forceinline__ void operator()(float* v) const {
+        const f32x4 d = product(product(f32x4{v[0], v[1], v[2], v[3]}, low), high);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = d[i];
+    }
+};
 
 // A row's threads: the waves of a group of the workgroup.  All of a workgroup's threads call sums() the same number of times; `turn`
 // alternates, so that one barrier a call separates a buffer's writes from its next ones.
@@ -138,6 +218,11 @@ struct Group {
         wave = threadIdx.x >> 6;
         waves = per >> 6;
         at = (int)threadIdx.x - wave / waves * per;
+    }
+    // Where the thread's first run of RUN values is: one thread's behind the other's, or (RUN 4) as Rotation has them.
+    template <int RUN>
+    __device__ __forceinline__ int place() const {
+        return RUN == 4 ? 256 * (at >> 6) + 16 * (lane & 15) + 4 * (lane >> 4) : at * RUN;
     }
     // a and b of all of the group's threads by the functions' rules
     template <typename B, typename F>
@@ -173,22 +258,24 @@ inline bool aligned(const RowView& v, int es) { return !v.p || ((uintptr_t)v.p %
 constexpr int64_t ONCE_BYTES = 32 << 20;
 
 // How rows are dealt: `per` threads hold a row, `slots` runs each; `groups` rows a workgroup; `grid` workgroups, each of which takes
-// every grid-th of the row groups (by_parts: one each).  slots 0: rows longer than any.
+// every grid-th of the row groups (by_parts: one each).  slots 0: rows longer than any, or shorter than a
+// run.
 struct RowCut {
     int per = 64, groups = 1, slots = 1;
     unsigned grid = 1;
     dim3 block() const { return dim3((unsigned)(per * groups)); }
 };
-// Rows of 8-value runs: up to 512 threads with one slot, 1024 with two; rotated ones, of 16-value runs: up to 1024 with one (more
-// spill).  waves: that a CU is to hold, where workgroups take rows in turn.
+// Rows of 8-value runs: up to 512 threads with one slot, 1024 with two; rotated ones, of 4-value runs: up to 1024 with four.
+// waves: that a CU is to hold, where workgroups take rows in turn.
 inline RowCut cut_rows(int64_t T, int W, int run, int waves) {
     RowCut c;
-    const int64_t runs = (W + run - 1) / run;
+    const int64_t runs = run == 4 ? (W + 255) / 256 * 64 : (W + run - 1) / run;
     c.slots = 0;
     c.per = 512;
-    for (int s : {1, 2}) {
+    for (int s : {1, 2, 4}) {
+        if (W < run) break;
         const int64_t n = ((runs + s - 1) / s + 63) / 64 * 64;
-        if (n > (s * run == 8 ? 512 : 1024) || s * run > 16) continue;
+        if (run == 4 ? n > 1024 || s < 4 : n > 512 * s || s > 2) continue;
         c.slots = s;
         c.per = (int)n;
         break;

@@ -51,7 +51,7 @@ def test_int8(group, dtype, h_dtype):
             q, s, h = qlin().add_rms_norm_int8(x, res, weight, convrot_groupsize=group)
             want, wh = norm(*wide(x, res, weight))
             assert q.dtype == torch.int8 and s.dtype == F32
-            check_codes(q, s, rotated(want, group))
+            check_codes(q, s, rotated(want, group), group)
             if res is not None:
                 within(h, wh, rounded(h_dtype, wh, U * wh.abs()))
 

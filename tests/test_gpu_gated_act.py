@@ -48,7 +48,9 @@ def test_forward(t, w, dtype, kind):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("group", [0, 4, 8, 16, 32, 64, 128, 256])
 def test_int8(group, dtype, kind):
-    """sigma is off by 2^-14 at most where it is above 2^-24 of the row's largest value's: 127 * 2^-14 < 0.01 of a step."""
+    """sigma is off by 2^-14 at most where it is above 2^-24 of the row's largest value's: 127 * 2^-14 < 0.008 of a step.  Through a
+    rotation that is 2^-14 of the group's norm, at most 16 times the row's largest value: 2^-10 of the scale, 0.124 of a step,
+    and what check_codes says."""
     for t, w in [(1, 4), (3, 20), (2, 100), (3, 1024), (2, 13824), (2, 16640), (1, 33024)] if group else SIZES:
         if group and w % group:
             continue
@@ -60,9 +62,9 @@ def test_int8(group, dtype, kind):
             f = act(z, kind)[0]
             want = rotated(f if v is None else f * v, group)
             codes, scale, top = q.cpu().double(), s.cpu().double(), want.abs().amax(-1, keepdim=True)
-            within(scale, top / 127, top / 127 * 2.0 ** -14)
+            within(scale, top / 127, top / 127 * (2.0 ** -13 + 2.0 ** -10 if group else 2.0 ** -14))
             steps = torch.where(top > 0, want * 127 / torch.where(top > 0, top, 1.0), 0.0)
-            assert float((codes - steps).abs().max()) <= 0.52
+            assert float((codes - steps).abs().max()) <= (0.65 if group else 0.51)
             if group == 0 and dtype == F32:
                 check_codes(q, s, want)
 
