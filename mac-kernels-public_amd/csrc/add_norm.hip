@@ -13,7 +13,7 @@ namespace {
 
 // T: x and y, H: the residual and h.  RUN 4: rotated.  RES: with a residual.  ONCE: nontemporal reads and writes.
 template <typename T, typename H, int RUN, int SLOTS, bool INT8, bool RES, bool ONCE>
-__global__ __launch_bounds__(1024, 6) void add_norm_kernel(AddNormArgs a, int64_t t0, int per, int groups) {
+__global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void add_norm_kernel(AddNormArgs a, int64_t t0, int per, int groups) {
     const Group g(per);
     const Rotation turned(RUN == 4 ? a.G : 1, g.lane);
     const int64_t t = t0 + (int64_t)blockIdx.x * groups + g.wave / g.waves;
@@ -28,16 +28,16 @@ __global__ __launch_bounds__(1024, 6) void add_norm_kernel(AddNormArgs a, int64_
         if constexpr (RES) r[s] = load_piece<ONCE, H, RUN>((const H*)a.r.p + from * a.r.ld, e0 + s * apart, a.W);
     }
     float v[SLOTS][RUN], w[SLOTS][RUN];
-    if (a.w) load_pieces_rt<RUN, SLOTS>(a.w, a.w_dt, e0, apart, a.W, w);
+    if (a.w) load_pieces_rt<ONCE, RUN, SLOTS>(a.w, a.w_dt, e0, apart, a.W, w);
     float ss = 0.0f;
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         const int e = e0 + s * apart;
-        trimmed<T, RUN>(x[s], e, a.W, v[s]);
+        trimmed<ONCE, T, RUN>(x[s], e, a.W, v[s]);
         if constexpr (RES) {
             float u[RUN];
-            trimmed<H, RUN>(r[s], e, a.W, u);
+            trimmed<ONCE, H, RUN>(r[s], e, a.W, u);
 #pragma unroll
             for (int i = 0; i < RUN; ++i) v[s][i] += u[i];
             if (live && e < a.W) store_run<ONCE, H, RUN>((H*)a.h.p + t * a.h.ld + e, a.W - e, v[s]);
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
     Raw raw[SLOTS];
     fetch(t, raw);
     float w[SLOTS][RUN], dw[SLOTS][RUN];
-    if (a.w) load_pieces_rt<RUN, SLOTS>(a.w, a.w_dt, e0, apart, a.W, w);
+    if (a.w) load_pieces_rt<ONCE, RUN, SLOTS>(a.w, a.w_dt, e0, apart, a.W, w);
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s)
 #pragma unroll
@@ -179,8 +179,8 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
         Run<H, RUN> dh[SLOTS];
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            trimmed<T, RUN>(raw[s].dy, e0 + s * apart, a.W, d[s]);
-            trimmed<H, RUN>(raw[s].h, e0 + s * apart, a.W, h[s]);
+            trimmed<ONCE, T, RUN>(raw[s].dy, e0 + s * apart, a.W, d[s]);
+            trimmed<ONCE, H, RUN>(raw[s].h, e0 + s * apart, a.W, h[s]);
             if constexpr (DH) dh[s] = raw[s].dh;
         }
         if (base + step < a.T) fetch(t + step, raw);
@@ -199,13 +199,17 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
             const int e = e0 + s * apart;
-            float o[RUN], more[RUN];
-            if constexpr (DH) trimmed<H, RUN>(dh[s], e, a.W, more);
+            float o[RUN], more[RUN] = {};
+            if constexpr (DH) trimmed<ONCE, H, RUN>(dh[s], e, a.W, more);
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
                 dw[s][i] = __builtin_fmaf(d[s][i], h[s][i] * rho, dw[s][i]);
-                o[i] = rho * (d[s][i] * w[s][i] - h[s][i] * c);
-                if constexpr (DH) o[i] += more[i];
+                {
+#pragma clang fp contract(off)
+                    // the same operations in every variant: rows of any alignment give the same bits
+                    const float in = __builtin_fmaf(d[s][i], w[s][i], -(h[s][i] * c));
+                    o[i] = DH ? __builtin_fmaf(rho, in, more[i]) : rho * in;
+                }
             }
             if (e < a.W) store_run<ONCE, H, RUN>((H*)a.dx.p + t * a.dx.ld + e, a.W - e, o);
         }
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(512) void add_norm_grad_long_kernel(AddNormGradArgs
         for (int e = threadIdx.x; e < a.W; e += 512) {  // an element is the same thread's in every row
             const float v = (float)h[e], d = (float)dy[e], w = a.w ? load_rt(a.w, a.w_dt, e) : 1.0f;
             if (part) part[e] = __builtin_fmaf(d, v * rho, begun ? part[e] : 0.0f);
-            dx[e] = (H)(rho * (d * w - v * c) + (dh ? (float)dh[e] : 0.0f));
+            dx[e] = (H)__builtin_fmaf(rho, __builtin_fmaf(d, w, -(v * c)), dh ? (float)dh[e] : 0.0f);
         }
         begun = true;
     }
@@ -286,18 +290,17 @@ __global__ __launch_bounds__(256) void add_norm_dw_kernel(const float* part, int
 }
 
 // The gradient's workgroups leave W partial sums each: as many as the chip holds at once, and no more.
-RowCut grad_cut(int64_t T, int W) { return cut_rows(T, W, 8, 16); }
+RowCut grad_cut(int64_t T, int W) { return cut_rows(T, W, 8, 2, 1024, 16); }
 
 template <typename T, typename H, int RUN, bool INT8, bool RES>
 hipError_t launch_norm(const AddNormArgs& a, hipStream_t st) {
-    const RowCut c = cut_rows(a.T, a.W, RUN, 0);
+    const RowCut c = cut_rows(a.T, a.W, RUN, RUN == 4 ? 4 : 2, 1024, 0);
     if (!c.slots) {
         hipLaunchKernelGGL((add_norm_long_kernel<T, H, RUN, INT8>), dim3(c.grid), c.block(), 0, st, a);
         return hipGetLastError();
     }
-    const bool pieces = aligned(a.x, sizeof(T)) && aligned(a.r, sizeof(H)) && aligned(a.y, sizeof(T)) && aligned(a.h, sizeof(H)) &&
-                        aligned({a.q, a.ldq}, 1);
-    const bool once = pieces && a.W % RUN == 0 && a.T * a.W * (int64_t)(sizeof(T) + (RES ? sizeof(H) : 0)) > ONCE_BYTES;
+    const bool once = whole(a.x, a.W, RUN, sizeof(T)) && whole(a.r, a.W, RUN, sizeof(H)) && whole(a.h, a.W, RUN, sizeof(H)) &&
+                      whole(a.y, a.W, RUN, sizeof(T)) && whole({a.q, a.ldq}, a.W, RUN, 1);
     return by_parts(c, a.T, [&](dim3 grid, int64_t t0) {
         auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, c.block(), 0, st, a, t0, c.per, c.groups); };
         if (RUN == 8 && c.slots == 1) once ? go(add_norm_kernel<T, H, 8, 1, INT8, RES, true>) : go(add_norm_kernel<T, H, 8, 1, INT8, RES, false>);
@@ -318,8 +321,8 @@ hipError_t norm_of(const AddNormArgs& a, hipStream_t st) {
 template <typename T, typename H>
 hipError_t grad_of(const AddNormGradArgs& a, hipStream_t st) {
     const RowCut c = grad_cut(a.T, a.W);
-    const bool once = a.W % 8 == 0 && a.T * a.W * (int64_t)(sizeof(T) + sizeof(H)) > ONCE_BYTES && aligned(a.dy, sizeof(T)) && aligned(a.h, sizeof(H)) &&
-                      aligned(a.dh, sizeof(H)) && aligned(a.dx, sizeof(H));
+    const bool once = whole(a.dy, a.W, 8, sizeof(T)) && whole(a.h, a.W, 8, sizeof(H)) && whole(a.dh, a.W, 8, sizeof(H)) &&
+                      whole(a.dx, a.W, 8, sizeof(H));
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(c.grid), c.block(), 0, st, a, c.per, c.groups); };
     auto by_slots = [&]<int SLOTS, int THREADS>() {
         if (a.dh.p) once ? go(add_norm_grad_kernel<T, H, SLOTS, true, true, THREADS>) : go(add_norm_grad_kernel<T, H, SLOTS, true, false, THREADS>);

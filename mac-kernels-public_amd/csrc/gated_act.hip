@@ -40,7 +40,7 @@ struct Values {
         if (W >= 8) r = load_piece<ONCE, T, 8>(row, e0, W);
     }
     __device__ __forceinline__ void to(int e0, int W, float* v) const {
-        if (W >= 8) trimmed<T, 8>(r, e0, W, v);
+        if (W >= 8) trimmed<ONCE, T, 8>(r, e0, W, v);
         else load_run<T, 8>(row + e0, W - e0, v);
     }
 };
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256) void gated_act_grad_kernel(GatedActArgs a, int
         float s, dt;
         gate_of<T, ACT>(z[i], s, dt);
         const float p = s * (1.0f - s), f = z[i] * s;
-        const float df = p == 0.0f ? s : s + z[i] * p * dt;  // far from 0, where z dt may be infinite, sigma
+        const float df = p == 0.0f ? s : __builtin_fmaf(z[i] * p, dt, s);  // far from 0, where z dt may be infinite, sigma
         z[i] = g[i] * (GATED ? v[i] : 1.0f) * df;
         v[i] = g[i] * f;
     }
@@ -104,7 +104,7 @@ __device__ __forceinline__ void values_of(const float* z, float* w, const Rotati
 }
 
 template <typename T, int ACT, bool GATED, int RUN, int SLOTS, bool ONCE>
-__global__ __launch_bounds__(1024, 6) void gated_act_int8_kernel(GatedActArgs a, int64_t t0, int per, int groups) {
+__global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void gated_act_int8_kernel(GatedActArgs a, int64_t t0, int per, int groups) {
     const Group g(per);
     const Rotation turned(RUN == 4 ? a.G : 1, g.lane);
     const int64_t t = t0 + (int64_t)blockIdx.x * groups + g.wave / g.waves;
@@ -122,8 +122,8 @@ __global__ __launch_bounds__(1024, 6) void gated_act_int8_kernel(GatedActArgs a,
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         float z[RUN];
-        trimmed<T, RUN>(gate[s], e0 + s * apart, a.W, z);
-        if constexpr (GATED) trimmed<T, RUN>(up[s], e0 + s * apart, a.W, v[s]);
+        trimmed<ONCE, T, RUN>(gate[s], e0 + s * apart, a.W, z);
+        if constexpr (GATED) trimmed<ONCE, T, RUN>(up[s], e0 + s * apart, a.W, v[s]);
         values_of<T, ACT, GATED, RUN>(z, v[s], turned);
 #pragma unroll
         for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[s][i]));
@@ -192,11 +192,6 @@ hipError_t by_kind(const GatedActArgs& a, F&& f) {
     return a.dtype == DT_F16 ? acts.template operator()<f16>() : acts.template operator()<__bf16>();
 }
 
-template <typename T>
-bool once_of(const GatedActArgs& a, int tensors) {
-    return a.W % 8 == 0 && a.T * a.W * (int64_t)sizeof(T) * tensors > ONCE_BYTES && aligned(a.gate, sizeof(T)) && aligned(a.up, sizeof(T)) && aligned(a.y, sizeof(T));
-}
-
 // f(first row, units, units a row) over parts of fewer than 2^31 units of 8 values.
 template <typename F>
 hipError_t by_units(const GatedActArgs& a, F&& f) {
@@ -212,17 +207,23 @@ hipError_t by_units(const GatedActArgs& a, F&& f) {
 
 template <typename T, int ACT, bool GATED, int RUN>
 hipError_t launch_int8(const GatedActArgs& a, hipStream_t st) {
-    const RowCut c = cut_rows(a.T, a.W, RUN, 0);
+    const RowCut c = cut_rows(a.T, a.W, RUN, RUN == 4 ? 8 : 4, 640, 0);
     if (!c.slots) {
         hipLaunchKernelGGL((gated_act_int8_long_kernel<T, ACT, GATED, RUN>), dim3(c.grid), c.block(), 0, st, a);
         return hipGetLastError();
     }
-    const bool once = once_of<T>(a, GATED ? 2 : 1) && aligned({a.q, a.ldq}, 1);
+    const bool once = whole(a.gate, a.W, RUN, sizeof(T)) && whole(a.up, a.W, RUN, sizeof(T)) && whole({a.q, a.ldq}, a.W, RUN, 1);
     return by_parts(c, a.T, [&](dim3 grid, int64_t t0) {
         auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, c.block(), 0, st, a, t0, c.per, c.groups); };
-        if (RUN == 8 && c.slots == 1) once ? go(gated_act_int8_kernel<T, ACT, GATED, 8, 1, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 8, 1, false>);
-        else if constexpr (RUN == 4) once ? go(gated_act_int8_kernel<T, ACT, GATED, 4, 4, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 4, 4, false>);
-        else once ? go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, true>) : go(gated_act_int8_kernel<T, ACT, GATED, 8, 2, false>);
+        auto by_slots = [&]<int SLOTS>() {
+            once ? go(gated_act_int8_kernel<T, ACT, GATED, RUN, SLOTS, true>) : go(gated_act_int8_kernel<T, ACT, GATED, RUN, SLOTS, false>);
+        };
+        switch (c.slots) {
+            case 1: if constexpr (RUN == 8) by_slots.template operator()<1>(); break;
+            case 2: if constexpr (RUN == 8) by_slots.template operator()<2>(); break;
+            case 4: by_slots.template operator()<4>(); break;
+            case 8: if constexpr (RUN == 4) by_slots.template operator()<8>(); break;
+        }
     });
 }
 
@@ -232,7 +233,7 @@ hipError_t run_gated_act(const GatedActArgs& a, hipStream_t st) {
     if (a.T == 0 || a.W == 0) return hipSuccess;
     return by_kind(a, [&]<typename T, int ACT, bool GATED>() {
         if (a.q) return a.G ? launch_int8<T, ACT, GATED, 4>(a, st) : launch_int8<T, ACT, GATED, 8>(a, st);
-        const bool once = once_of<T>(a, GATED ? 2 : 1);
+        const bool once = whole(a.gate, a.W, 8, sizeof(T)) && whole(a.up, a.W, 8, sizeof(T)) && whole(a.y, a.W, 8, sizeof(T));
         return by_units(a, [&](dim3 grid, int64_t t0, uint32_t units, uint32_t per) {
             auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a, t0, units, per); };
             once ? go(gated_act_kernel<T, ACT, GATED, true>) : go(gated_act_kernel<T, ACT, GATED, false>);
@@ -243,7 +244,8 @@ hipError_t run_gated_act(const GatedActArgs& a, hipStream_t st) {
 hipError_t run_gated_act_grad(const GatedActArgs& a, hipStream_t st) {
     if (a.T == 0 || a.W == 0) return hipSuccess;
     return by_kind(a, [&]<typename T, int ACT, bool GATED>() {
-        const bool once = once_of<T>(a, GATED ? 3 : 2) && aligned(a.dy, sizeof(T)) && aligned(a.dgate, sizeof(T)) && aligned(a.dup, sizeof(T));
+        const bool once = whole(a.gate, a.W, 8, sizeof(T)) && whole(a.up, a.W, 8, sizeof(T)) && whole(a.dy, a.W, 8, sizeof(T)) &&
+                          whole(a.dgate, a.W, 8, sizeof(T)) && whole(a.dup, a.W, 8, sizeof(T));
         return by_units(a, [&](dim3 grid, int64_t t0, uint32_t units, uint32_t per) {
             auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a, t0, units, per); };
             once ? go(gated_act_grad_kernel<T, ACT, GATED, true>) : go(gated_act_grad_kernel<T, ACT, GATED, false>);

@@ -29,12 +29,12 @@ __device__ __forceinline__ Run<T, N> load_piece(const T* row, int e0, int W) {
     }
     return r;
 }
-// A piece's values in fp32, zeros past the row's end.
-template <typename T, int N>
+// A piece's values in fp32, zeros past the row's end.  WHOLE: a piece is all in its row or all behind it.
+template <bool WHOLE, typename T, int N>
 __device__ __forceinline__ void trimmed(const Run<T, N>& r, int e0, int W, float* v) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (float)r.v[i];
-    if (e0 + N > W) {
+    for (int i = 0; i < N; ++i) v[i] = !WHOLE || e0 < W ? (float)r.v[i] : 0.0f;
+    if (!WHOLE && e0 + N > W) {
         const int d = e0 - (W - N);  // value i is the piece's i + d
 #pragma unroll
         for (int step = 1; step < N; step *= 2)
@@ -46,14 +46,14 @@ __device__ __forceinline__ void trimmed(const Run<T, N>& r, int e0, int W, float
     }
 }
 // The same of a vector of float32, float16 or bfloat16, S pieces `apart` values from one another.
-template <int N, int S>
+template <bool WHOLE, int N, int S>
 __device__ __forceinline__ void load_pieces_rt(const void* p, int dt, int e0, int apart, int W, float (&v)[S][N]) {
     auto of = [&]<typename T>() {
         Run<T, N> r[S];
 #pragma unroll
         for (int s = 0; s < S; ++s) r[s] = load_piece<false, T, N>((const T*)p, e0 + s * apart, W);
 #pragma unroll
-        for (int s = 0; s < S; ++s) trimmed<T, N>(r[s], e0 + s * apart, W, v[s]);
+        for (int s = 0; s < S; ++s) trimmed<WHOLE, T, N>(r[s], e0 + s * apart, W, v[s]);
     };
     if (dt == DT_F32) of.template operator()<float>();
     else if (dt == DT_F16) of.template operator()<f16>();
@@ -250,12 +250,11 @@ struct Group {
     }
 };
 
-// Whether 16-byte pieces of the rows are aligned.
-inline bool aligned(const RowView& v, int es) { return !v.p || ((uintptr_t)v.p % 16 == 0 && v.ld * es % 16 == 0); }
-
-// Calls that read more than this read and write nontemporally: what they touch is not in the caches when it is needed again (4608
-// x 6144 norm to bf16, reads and writes: 56 us neither so, 49 the reads, 40 both).
-constexpr int64_t ONCE_BYTES = 32 << 20;
+// Whether rows of W values of es bytes divide into aligned pieces of `run` values; rows that are absent do.
+inline bool whole(const RowView& v, int W, int run, int es) {
+    const int piece = std::min(16, run * es);
+    return !v.p || (W % run == 0 && (uintptr_t)v.p % piece == 0 && v.ld * es % piece == 0);
+}
 
 // How rows are dealt: `per` threads hold a row, `slots` runs each; `groups` rows a workgroup; `grid` workgroups, each of which takes
 // every grid-th of the row groups (by_parts: one each).  slots 0: rows longer than any, or shorter than a
@@ -265,24 +264,25 @@ struct RowCut {
     unsigned grid = 1;
     dim3 block() const { return dim3((unsigned)(per * groups)); }
 };
-// Rows of 8-value runs: up to 512 threads with one slot, 1024 with two; rotated ones, of 4-value runs: up to 1024 with four.
+// 8-value runs: a slot more from 512 threads on (norm 4608 x 6144 to int8, 384 threads of two slots 35.5 us, 768 of one 38.2), up to
+// `most` slots and, with these, 1024 threads; fewer slots hold up to `threads`.  4-value runs: four slots, and eight where
+// `most` says so and a row has more than 20 times 256 values (activation 9504 x 13824: four 147 us, eight 120; 9504 x 5120: 47.6, 49.1).
 // waves: that a CU is to hold, where workgroups take rows in turn.
-inline RowCut cut_rows(int64_t T, int W, int run, int waves) {
+inline RowCut cut_rows(int64_t T, int W, int run, int most, int threads, int waves) {
     RowCut c;
     const int64_t runs = run == 4 ? (W + 255) / 256 * 64 : (W + run - 1) / run;
     c.slots = 0;
     c.per = 512;
-    for (int s : {1, 2, 4}) {
-        if (W < run) break;
+    for (int s = run == 4 ? (most == 8 && runs > 20 * 64 ? 8 : 4) : 1; s <= most && W >= run; s *= 2) {
         const int64_t n = ((runs + s - 1) / s + 63) / 64 * 64;
-        if (run == 4 ? n > 1024 || s < 4 : n > 512 * s || s > 2) continue;
+        if (n > (s == most ? 1024 : s == 1 ? 512 : threads)) continue;
         c.slots = s;
         c.per = (int)n;
         break;
     }
     c.groups = c.slots && c.per < 256 ? 256 / c.per : 1;
-    const int64_t blocks = (T + c.groups - 1) / c.groups, most = 256 * (int64_t)std::max(1, waves * 64 / (c.per * c.groups));
-    const int64_t rounds = (blocks + most - 1) / most;
+    const int64_t blocks = (T + c.groups - 1) / c.groups, held = 256 * (int64_t)std::max(1, waves * 64 / (c.per * c.groups));
+    const int64_t rounds = (blocks + held - 1) / held;
     c.grid = (unsigned)((blocks + rounds - 1) / rounds);
     return c;
 }
