@@ -30,7 +30,7 @@ __global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void add_norm_kerne
     float v[SLOTS][RUN], w[SLOTS][RUN];
     if (a.w) load_pieces_rt<ONCE, RUN, SLOTS>(a.w, a.w_dt, e0, apart, a.W, w);
     float ss = 0.0f;
-    uint32_t top = 0;
+    float top = 0.0f;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         const int e = e0 + s * apart;
@@ -42,21 +42,21 @@ __global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void add_norm_kerne
             for (int i = 0; i < RUN; ++i) v[s][i] += u[i];
             if (live && e < a.W) store_run<ONCE, H, RUN>((H*)a.h.p + t * a.h.ld + e, a.W - e, v[s]);
         }
+        float sq = 0.0f;
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[s][i], v[s][i], ss);
+        for (int i = 0; i < RUN; ++i) sq = __builtin_fmaf(v[s][i], v[s][i], sq);
+        ss += e < a.W ? sq : 0.0f;
         if (a.w)
 #pragma unroll
             for (int i = 0; i < RUN; ++i) v[s][i] *= w[s][i];
         if constexpr (RUN == 4) turned(v[s]);
-        if constexpr (INT8)
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[s][i]));
+        if constexpr (INT8) top = larger(top, e < a.W ? largest<RUN>(v[s]) : 0.0f);
     }
-    g.sums(ss, top, 0, [](uint32_t p, uint32_t q) { return max(p, q); });
+    g.sums(ss, top, 0, larger);
     const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
     if (!live) return;
     if constexpr (INT8) {
-        const float most = __uint_as_float(top);
+        const float most = top;
         float first;
         const float inv = code_factor(most, first);
         if (g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.norm : 1.0f) / 127.0f * rho;
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
             if constexpr (RUN == 4) turned(v);
         };
         float ss = 0.0f;
-        uint32_t top = 0;
+        float top = 0.0f;
         for (int c = 0; c < a.W; c += 512 * RUN) {
             const int e0 = c + g.place<RUN>();
             sum_of(e0);
@@ -118,12 +118,11 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
             for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
             if constexpr (INT8) {
                 weigh(e0);
-#pragma unroll
-                for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[i]));
+                top = larger(top, largest<RUN>(v));
             }
         }
-        g.sums(ss, top, turn, [](uint32_t p, uint32_t q) { return max(p, q); });
-        const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps), most = __uint_as_float(top);
+        g.sums(ss, top, turn, larger);
+        const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps), most = top;
         float first = 1.0f;
         const float inv = INT8 ? code_factor(most, first) : 0.0f;
         if (INT8 && g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.norm : 1.0f) / 127.0f * rho;
@@ -186,12 +185,17 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
         if (base + step < a.T) fetch(t + step, raw);
         float ss = 0.0f, gh = 0.0f;
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s)
+        for (int s = 0; s < SLOTS; ++s) {
+            float sq = 0.0f, pr = 0.0f;
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                ss = __builtin_fmaf(h[s][i], h[s][i], ss);
-                gh = __builtin_fmaf(d[s][i] * w[s][i], h[s][i], gh);
+                sq = __builtin_fmaf(h[s][i], h[s][i], sq);
+                pr = __builtin_fmaf(d[s][i] * w[s][i], h[s][i], pr);
             }
+            const bool in = e0 + s * apart < a.W;
+            ss += in ? sq : 0.0f;
+            gh += in ? pr : 0.0f;
+        }
         g.sums(ss, gh, turn, [](float p, float q) { return p + q; });
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
         const float c = rho * rho * (gh / (float)a.W);
@@ -211,7 +215,7 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
                     o[i] = DH ? __builtin_fmaf(rho, in, more[i]) : rho * in;
                 }
             }
-            if (e < a.W) store_run<ONCE, H, RUN>((H*)a.dx.p + t * a.dx.ld + e, a.W - e, o);
+            if (e < a.W) store_run<ONCE && SLOTS == 1, H, RUN>((H*)a.dx.p + t * a.dx.ld + e, a.W - e, o);  // see grad_cut
         }
     }
     if (!a.dw) return;
@@ -289,8 +293,10 @@ __global__ __launch_bounds__(256) void add_norm_dw_kernel(const float* part, int
     store_rt(dw, dw_dt, e, s);
 }
 
-// The gradient's workgroups leave W partial sums each: as many as the chip holds at once, and no more.
-RowCut grad_cut(int64_t T, int W) { return cut_rows(T, W, 8, 2, 1024, 16); }
+// The gradient's workgroups leave W partial sums each and take rows in turn: one a CU for wide rows, two of 256 threads for short
+// ones (9504 x 5120: 251 workgroups 78 us, 501 84, 732 94; 9504 x 1024: 251 27, 501 22).  Wide rows are written through the
+// caches (78 us; nontemporally 95), short ones not (9504 x 1024: 24.5, 22.3).
+RowCut grad_cut(int64_t T, int W) { return cut_rows(T, W, 8, 2, 1024, 8); }
 
 template <typename T, typename H, int RUN, bool INT8, bool RES>
 hipError_t launch_norm(const AddNormArgs& a, hipStream_t st) {

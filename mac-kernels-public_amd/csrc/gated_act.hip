@@ -118,21 +118,20 @@ __global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void gated_act_int8
         if constexpr (GATED) up[s] = load_piece<ONCE, T, RUN>((const T*)a.up.p + from * a.up.ld, e0 + s * apart, a.W);
     }
     float v[SLOTS][RUN], none = 0.0f;
-    uint32_t top = 0;
+    float top = 0.0f;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         float z[RUN];
         trimmed<ONCE, T, RUN>(gate[s], e0 + s * apart, a.W, z);
         if constexpr (GATED) trimmed<ONCE, T, RUN>(up[s], e0 + s * apart, a.W, v[s]);
         values_of<T, ACT, GATED, RUN>(z, v[s], turned);
-#pragma unroll
-        for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[s][i]));
+        top = larger(top, e0 + s * apart < a.W ? largest<RUN>(v[s]) : 0.0f);
     }
-    g.sums(none, top, 0, [](uint32_t p, uint32_t q) { return max(p, q); });
+    g.sums(none, top, 0, larger);
     if (!live) return;
     float first;
-    const float inv = code_factor(__uint_as_float(top), first);
-    if (g.at == 0) a.scale[t] = __uint_as_float(top) * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
+    const float inv = code_factor(top, first);
+    if (g.at == 0) a.scale[t] = top * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
     if (first != 1.0f)
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s)
@@ -154,7 +153,7 @@ __global__ __launch_bounds__(512) void gated_act_int8_long_kernel(GatedActArgs a
     for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
         const T *gate = (const T*)a.gate.p + t * a.gate.ld, *up = GATED ? (const T*)a.up.p + t * a.up.ld : nullptr;
         float v[RUN], none = 0.0f;
-        uint32_t top = 0;
+        float top = 0.0f;
         auto value = [&](int e0) {
             float z[RUN];
             load_run<T, RUN>(gate + e0, a.W - e0, z);
@@ -163,13 +162,12 @@ __global__ __launch_bounds__(512) void gated_act_int8_long_kernel(GatedActArgs a
         };
         for (int c = 0; c < a.W; c += 512 * RUN) {
             value(c + g.place<RUN>());
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) top = max(top, abs_bits(v[i]));
+            top = larger(top, largest<RUN>(v));
         }
-        g.sums(none, top, turn, [](uint32_t p, uint32_t q) { return max(p, q); });
+        g.sums(none, top, turn, larger);
         float first;
-        const float inv = code_factor(__uint_as_float(top), first);
-        if (g.at == 0) a.scale[t] = __uint_as_float(top) * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
+        const float inv = code_factor(top, first);
+        if (g.at == 0) a.scale[t] = top * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
         for (int c = 0; c < a.W; c += 512 * RUN) {
             const int e0 = c + g.place<RUN>();
             value(e0);

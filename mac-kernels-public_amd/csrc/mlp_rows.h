@@ -29,11 +29,12 @@ __device__ __forceinline__ Run<T, N> load_piece(const T* row, int e0, int W) {
     }
     return r;
 }
-// A piece's values in fp32, zeros past the row's end.  WHOLE: a piece is all in its row or all behind it.
+// A piece's values in fp32, zeros past the row's end.  WHOLE: a piece is all in its row, or all behind it and then a copy of the row's
+// last values, which the callers leave out of their sums.
 template <bool WHOLE, typename T, int N>
 __device__ __forceinline__ void trimmed(const Run<T, N>& r, int e0, int W, float* v) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = !WHOLE || e0 < W ? (float)r.v[i] : 0.0f;
+    for (int i = 0; i < N; ++i) v[i] = (float)r.v[i];
     if (!WHOLE && e0 + N > W) {
         const int d = e0 - (W - N);  // value i is the piece's i + d
 #pragma unroll
@@ -101,12 +102,24 @@ template <bool ONCE, typename T, int N>
 __device__ __forceinline__ void store_run(T* p, int n, const float* v) {
     Run<T, N> r;
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.v[i] = (T)v[i];
+    for (int i = 0; i < N; ++i) {
+        float x = v[i];
+        // fp16: a product and its rounding to 16 bits may become one instruction of another result, in some variants and not in others
+        if constexpr (__is_same(T, f16)) asm("" : "+v"(x));
+        r.v[i] = (T)x;
+    }
     store_raw<ONCE, T, N>(p, n, r);
 }
 
-// |v| as bits that order as the values do, a NaN above all.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// The larger magnitude, NaN if there is one.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(__builtin_fabsf(a), __builtin_fabsf(b)); }
+template <int N>
+__device__ __forceinline__ float largest(const float* v) {
+    float m = __builtin_fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = larger(m, v[i]);
+    return m;
+}
 
 // The codes rne(v * 127 / top) of a run, top the row's largest |v|, as bytes: v * inv added to 1.5 * 2^23 rounds once, to
 // an integer in the low bits (|v * inv| <= 127 and an ulp).
