@@ -166,9 +166,9 @@ __device__ __forceinline__ float code_factor(float top, float& first) {
 // which are its part of V as the first operand; the product's registers, taken as a first operand again, are its transpose, and the
 // second product comes out in the layout of the values.  Unnormalized: by sqrt(G).
 //
-// A value enters a product as two bf16 parts of 8 bits each, off by 2^-18 of it.  Over both products that is at most 2^-17 of
-// the group's norm, so, the row's largest value being at least a 16th of that, 127 * 16 * 2^-17 < 0.016 steps of a code.  (In
-// fp32 across the lanes, 10 vector instructions and 3 LDS exchanges a value against 6, 9504 x 13824 took 157 us; see gated_act.hip.)
+// A value enters a product as three bf16 parts that together are the value (8 bits of its 24 each), so that the rotation is as exact as
+// fp32's sums.  Two rounded parts, off by 2^-18, would change one code in 10^4 (9504 x 13824 in fp16, with the gate: two
+// parts 140 us, three 154; the matrix cores' fp32 products, of a 16th of the rate, 207; fp32 across the lanes 157).
 typedef short bf16x4_bits __attribute__((ext_vector_type(4)));
 struct RotationTable {
     uint64_t m[5][64];  // sizes 1, 2, 4, 8, 16: lane l's entries [4 (l / 16) + i][l % 16]
@@ -201,19 +201,22 @@ struct Rotation {
         norm = k % 2 ? 0.70710678118654752f / (float)(1 << (k / 2)) : 1.0f / (float)(1 << (k / 2));
     }
     static __device__ __forceinline__ f32x4 product(const f32x4 v, const bf16x4_bits m) {
-        typedef float F2 __attribute__((ext_vector_type(2)));
-        typedef __bf16 B2 __attribute__((ext_vector_type(2)));
-        u32x2 hi, lo;
+        // the parts of two values side by side, as the product takes them: the upper halves of their words, those of what is left
+        u32x2 part[3];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {  // two values an instruction, their parts side by side as the product takes them
-            const F2 a = {v[2 * i], v[2 * i + 1]};
-            hi[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(a, B2));
-            const F2 rest = {a.x - __uint_as_float(hi[i] << 16), a.y - __uint_as_float(hi[i] & 0xFFFF0000u)};
-            lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, B2));
+        for (int i = 0; i < 2; ++i) {
+            float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                part[p][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+                a -= __uint_as_float(part[p][i] << 16);
+                b -= __uint_as_float(part[p][i] & 0xFFFF0000u);
+            }
         }
         f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-        d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, lo), m, d, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, hi), m, d, 0, 0, 0);
+#pragma unroll
+        for (int p = 2; p >= 0; --p) d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, part[p]), m, d, 0, 0, 0);
+        return d;
     }
     __device__ __forceinline__ void operator()(float* v) const {
         const f32x4 d = product(product(f32x4{v[0], v[1], v[2], v[3]}, low), high);
