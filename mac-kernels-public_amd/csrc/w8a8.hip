@@ -391,6 +391,31 @@ hipError_t run_tiles(const W8A8Args& a, int shape, hipStream_t st) {
     return hipErrorInvalidValue;
 }
 
+// Operands as the path takes them.
+hipError_t run_shape(const W8A8Args& a, int path, hipStream_t st) {
+    if (path < GEMM) return run_tiles(a, path, st);
+    const int shape = GEMM_TILES[path - GEMM];
+    // Whole rounds of 256 x 256 tiles, and a call of their own for the rows that would start another of few tiles (9504 rows,
+    // 5120 -> 13824: the last 32 rows 15.4 us in tiles of 32 x 64, 34.6 in the GEMM's of 128 x 64).
+    if (const int64_t top = shape == I8_256x256 ? tail_split_rows(a.M, a.N) : 0) {
+        W8A8Args first = a, rest = a;
+        first.M = top;
+        rest.M = a.M - top;
+        rest.x = a.x + top * a.ldx;
+        rest.sx = a.sx + top;
+        rest.y = (uint8_t*)a.y + top * a.ldy * dt_bytes(a.y_dt);
+        if (a.res.r) rest.res.r = (const uint8_t*)a.res.r + top * a.res.ldr * dt_bytes(a.res.r_dt);
+        if (hipError_t e = run_shape(first, path, st)) return e;
+        return run_shape(rest, plan_of(rest.M, rest.N, rest.K, 0).path, st);
+    }
+    GemmI8Args p;
+    p.xq = a.x; p.ldx = a.ldx; p.sx = a.sx; p.M = a.M; p.N = a.N; p.K = a.K;
+    p.w8 = const_cast<int8_t*>(a.w); p.s_ch = a.sw;
+    p.bias = a.bias; p.bias_dtype = a.bias_dt; p.res = a.res;
+    p.y = a.y; p.y_dtype = a.y_dt; p.ldy = a.ldy;
+    return run_gemm_i8_dense(p, shape, st);
+}
+
 }  // namespace
 
 int w8a8_apart(const W8A8Args& a) {
@@ -424,13 +449,7 @@ hipError_t run_w8a8(const W8A8Args& call, hipStream_t st) {
         a.ldw = Kp;
     }
     if (plan.packs == (W8A8_X_ROWS | W8A8_W_ROWS)) a.K = Kp;
-    if (plan.path < GEMM) return run_tiles(a, plan.path, st);
-    GemmI8Args p;
-    p.xq = a.x; p.ldx = a.ldx; p.sx = a.sx; p.M = a.M; p.N = a.N; p.K = a.K;
-    p.w8 = const_cast<int8_t*>(a.w); p.s_ch = a.sw;
-    p.bias = a.bias; p.bias_dtype = a.bias_dt; p.res = a.res;
-    p.y = a.y; p.y_dtype = a.y_dt; p.ldy = a.ldy;
-    return run_gemm_i8_dense(p, GEMM_TILES[plan.path - GEMM], st);
+    return run_shape(a, plan.path, st);
 }
 
 }  // namespace qlin
