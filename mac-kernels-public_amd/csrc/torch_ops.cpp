@@ -443,22 +443,27 @@ at::Tensor rows_of(const char* op, const at::Tensor& t, const char* name, const 
     return dense(t.reshape({rows, t.size(-1)}));
 }
 
+// A new tensor, straight from the device's allocator: small calls are bound by the host.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const at::Tensor& like) {
+    return at::Tensor(at::detail::empty_cuda(sizes, dt, like.device(), c10::nullopt));
+}
+
 // A new tensor shaped like x [.., values], and its rows.
 struct Fresh {
     at::Tensor t;
     Opt rows;
     Fresh() = default;
-    Fresh(const at::Tensor& x, const at::Tensor& x2, at::ScalarType dt) : t(at::empty(x.sizes(), x.options().dtype(dt))), rows(x.dim() == 2 ? t : t.view(x2.sizes())) {}
+    Fresh(const at::Tensor& x, const at::Tensor& x2, at::ScalarType dt) : t(fresh(x.sizes(), dt, x)), rows(x.dim() == 2 ? t : t.view(x2.sizes())) {}
 };
 
 // int8 codes like x and a scale a row.
 struct Codes {
     at::Tensor q, scale;
     Opt dq, ds;
-    Codes(const at::Tensor& x, const at::Tensor& x2) : q(at::empty(x.sizes(), x.options().dtype(at::kChar))) {
+    Codes(const at::Tensor& x, const at::Tensor& x2) : q(fresh(x.sizes(), at::kChar, x)) {
         std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
         sizes.back() = 1;
-        scale = at::empty(sizes, x.options().dtype(at::kFloat));
+        scale = fresh(sizes, at::kFloat, x);
         dq = Opt(x.dim() == 2 ? q : q.view(x2.sizes()));
         ds = Opt(x.dim() == 2 ? scale : scale.view({x2.size(0), 1}));
     }
@@ -500,7 +505,7 @@ pybind11::tuple add_rms_norm_grad(const at::Tensor& dy, const OptTensor& dh, con
     const hipStream_t st = current_stream(dy);
     at::Tensor ws;
     if (weight_grad && weight) {
-        dw = Opt(at::empty_like(w.t));
+        dw = Opt(fresh(w.t.sizes(), w.t.scalar_type(), w.t));
         ws = workspace_for(qlin_workspace_size(QLIN_OP_ADD_RMS_NORM_GRAD, g2.t.size(0), 0, g2.t.size(1), 0, g2.d.dtype), dy, st);
     }
     check(qlin_add_rms_norm_grad(g2.p(), d2.p(), h2.p(), w.p(), (float)eps, dx.rows.p(), dw.p(), ws.defined() ? ws.data_ptr() : nullptr,
@@ -544,7 +549,7 @@ pybind11::tuple gated_act_grad(const at::Tensor& dy, const at::Tensor& gate, con
     u2 = Opt(rows_of(op, *up, "up", &gate));
     std::vector<int64_t> sizes(gate.sizes().begin(), gate.sizes().end());
     sizes.back() = 2 * n;
-    const at::Tensor both = at::empty(sizes, gate.options()), flat = both.view({g2.t.size(0), 2 * n});
+    const at::Tensor both = fresh(sizes, gate.scalar_type(), gate), flat = both.view({g2.t.size(0), 2 * n});
     Opt a(flat.narrow(1, 0, n)), b(flat.narrow(1, n, n));
     check(qlin_gated_act_grad(d2.p(), g2.p(), u2.p(), (int)act, a.p(), b.p(), current_stream(gate)));
     return pybind11::make_tuple(both.narrow(-1, 0, n), both.narrow(-1, n, n));
@@ -581,7 +586,7 @@ at::Tensor w8a8_int8_linear(const at::Tensor& x, const at::Tensor& x_scale, cons
     }
     const at::ScalarType dt = out_dtype.value_or(residual ? residual->scalar_type() : at::kBFloat16);
     if (!is_float(dt)) fail(QLIN_EUNSUPPORTED, "out_dtype unsupported");
-    const at::Tensor y = at::empty(sizes, x.options().dtype(dt));
+    const at::Tensor y = fresh(sizes, dt, x);
     const at::Tensor w = dense(qdata);
     at::Tensor ws_ = f32_1d(scale);
     if (ws_.numel() != n) ws_ = ws_.expand({n}).contiguous();
@@ -593,10 +598,12 @@ at::Tensor w8a8_int8_linear(const at::Tensor& x, const at::Tensor& x_scale, cons
     const int param = (off(x2.t) ? QLIN_W8A8_X_ROWS : 0) | (off(w) ? QLIN_W8A8_W_ROWS : 0) |
                       (n > 1 && w.stride(0) != k ? QLIN_W8A8_W_APART : 0);
     const hipStream_t st = current_stream(x);
-    const at::Tensor room = workspace_for(qlin_workspace_size(QLIN_OP_W8A8_LINEAR, m, n, k, param, 0), x, st);
+    const size_t need = qlin_workspace_size(QLIN_OP_W8A8_LINEAR, m, n, k, param, 0);
+    const at::Tensor room = need ? workspace_for(need, x, st) : at::Tensor();
     Opt xs(f32_1d(x_scale)), dw(w), ds(ws_), yo(x.dim() == 2 ? y : y.view({m, n}));
     qlin_tensor db;
-    check(qlin_w8a8_linear(x2.p(), xs.p(), dw.p(), ds.p(), opt(b, db), r.p(), rs.p(), yo.p(), room.data_ptr(), (size_t)room.numel(), st));
+    check(qlin_w8a8_linear(x2.p(), xs.p(), dw.p(), ds.p(), opt(b, db), r.p(), rs.p(), yo.p(), need ? room.data_ptr() : nullptr,
+                           need ? (size_t)room.numel() : 0, st));
     return y;
 }
 
