@@ -71,7 +71,7 @@ typedef enum {
     QLIN_OP_QK_NORM_ROPE_GRAD = 12,    /* qlin_qk_norm_rope_grad: M tokens, N heads of q and k together, K the head size */
     QLIN_OP_PAGED_ATTENTION = 13,      /* qlin_paged_attention: M rows, N query heads, K the head size, param = kv heads */
     QLIN_OP_ADD_RMS_NORM_GRAD = 14,    /* qlin_add_rms_norm_grad: M rows, K values a row (N, param unused) */
-    QLIN_OP_W8A8_LINEAR = 15,          /* qlin_w8a8_linear: param = QLIN_W8A8_X_ROWS | .. as they apply */
+    QLIN_OP_W8A8_LINEAR = 15,          /* qlin_w8a8_linear: param = QLIN_W8A8_X_ROWS | .. as they apply (x_dtype: QLIN_DT_I8) */
 } qlin_op;
 
 /* ggml type ids accepted by the GGUF entry points (enum ggml_type). */
@@ -431,7 +431,7 @@ qlin_status qlin_gated_act_int8(const qlin_tensor* gate, const qlin_tensor* up, 
 qlin_status qlin_gated_act_grad(const qlin_tensor* dy, const qlin_tensor* gate, const qlin_tensor* up, int act,
                                 qlin_tensor* dgate, qlin_tensor* dup, void* stream);
 
-/* qlin_workspace_size's param for QLIN_OP_W8A8_LINEAR: x's rows, the weights' rows are not all 16-byte aligned or 2^25 and more
+/* qlin_workspace_size's param for QLIN_OP_W8A8_LINEAR: x's rows, the weights' rows are not all 16-byte aligned or 2^24 and more
  * bytes apart (these two count only where K is a multiple of 16); the weights' rows are not one behind the other.  Some calls
  * copy such operands, and those of a K that is not a multiple of 128, to rows of their own in the workspace. */
 enum { QLIN_W8A8_X_ROWS = 1, QLIN_W8A8_W_ROWS = 2, QLIN_W8A8_W_APART = 4 };
@@ -440,7 +440,7 @@ enum { QLIN_W8A8_X_ROWS = 1, QLIN_W8A8_W_ROWS = 2, QLIN_W8A8_W_APART = 4 };
  * that; one rounding.  x i8 [M, K] with x_scale f32 [M] or [M, 1], as qlin_quantize_act_int8, qlin_add_rms_norm_int8
  * and qlin_gated_act_int8 give them; qdata i8 [N, K] with scale f32 [N] or [N, 1]; bias optional f32/f16/bf16 [N];
  * residual optional f32/f16/bf16 [M, N], residual_scale optional (NULL = 1) f32/f16/bf16 [N]; y f32/f16/bf16 [M, N].
- * The int32 sums are exact: K up to 131071.  Workspace: qlin_workspace_size(QLIN_OP_W8A8_LINEAR, M, N, K, param, 0). */
+ * The int32 sums are exact: K up to 131071.  M below 2^28, N below 2^26, M N up to 2^36.  Workspace: qlin_workspace_size(QLIN_OP_W8A8_LINEAR, M, N, K, param, 0). */
 qlin_status qlin_w8a8_linear(const qlin_tensor* x, const qlin_tensor* x_scale, const qlin_tensor* qdata, const qlin_tensor* scale,
                              const qlin_tensor* bias, const qlin_tensor* residual, const qlin_tensor* residual_scale,
                              qlin_tensor* y, void* workspace, size_t workspace_bytes, void* stream);

@@ -54,7 +54,7 @@ qlin_status vector_of(const qlin_tensor* t, const char* name, int64_t n, int dty
         if (t->shape[i] > 1) stride = t->stride[i];
     }
     if (dtype < 0 ? !is_float(t->dtype) : t->dtype != dtype) return fail(QLIN_EUNSUPPORTED, "%s has an unsupported dtype", name);
-    if (t->ndim > 2 || count != n) return fail(QLIN_EINVAL, "%s has %lld elements, expected %lld", name, (long long)count, (long long)n);
+    if (t->ndim > 2 || count != n || (t->ndim == 2 && t->shape[0] != 1 && t->shape[1] != 1)) return fail(QLIN_EINVAL, "%s has %lld elements, expected %lld", name, (long long)count, (long long)n);
     if (n > 0 && !t->data) return fail(QLIN_EINVAL, "%s is missing", name);
     if (n > 1 && stride != 1) return fail(QLIN_EUNSUPPORTED, "%s must be contiguous", name);
     return QLIN_OK;
@@ -253,7 +253,8 @@ qlin_status qlin_w8a8_linear(const qlin_tensor* x, const qlin_tensor* x_scale, c
     a.ldw = a.N > 1 ? v.ld : a.K;
     if (a.M == 1) a.ldx = a.K;
     if (a.K > W8A8_MAX_K) return fail(QLIN_EUNSUPPORTED, "K > %d", W8A8_MAX_K);
-    if (a.M >= MOST_ROWS || a.N >= MOST_ROWS || (a.N && a.M > ((int64_t)1 << 36) / a.N)) return fail(QLIN_EUNSUPPORTED, "more than 2^36 outputs");
+    if (a.M >= W8A8_MOST_ROWS || a.N >= W8A8_MOST_OUTPUTS || (a.N && a.M > W8A8_MOST_RESULTS / a.N))
+        return fail(QLIN_EUNSUPPORTED, "%lld rows by %lld outputs are too many", (long long)a.M, (long long)a.N);
     if (qlin_status s = vector_of(x_scale, "x_scale", a.M, QLIN_DT_F32)) return s;
     if (qlin_status s = vector_of(scale, "scale", a.N, QLIN_DT_F32)) return s;
     a.sx = (const float*)x_scale->data;

@@ -88,7 +88,9 @@ struct W8A8Args {
 };
 // What keeps a call's operands from being taken as they are (bits of `param`).
 enum { W8A8_X_ROWS = QLIN_W8A8_X_ROWS, W8A8_W_ROWS = QLIN_W8A8_W_ROWS, W8A8_W_APART = QLIN_W8A8_W_APART };
-constexpr int64_t W8A8_MOST_APART = 1 << 25;  // row strides below it: the kernels' offsets in a tile are 32 bits
+// Rows and outputs of a call below these, and at most 2^36 results: a launch has fewer than 2^32 threads whatever the tiles.
+constexpr int64_t W8A8_MOST_ROWS = 1 << 28, W8A8_MOST_OUTPUTS = 1 << 26, W8A8_MOST_RESULTS = (int64_t)1 << 36;
+constexpr int64_t W8A8_MOST_APART = 1 << 24;  // row strides below it: the kernels' offsets in a tile, of up to 256 rows, are 32 bits
 int w8a8_apart(const W8A8Args& a);
 size_t ws_w8a8(int64_t M, int64_t N, int64_t K, int apart);
 hipError_t run_w8a8(const W8A8Args& a, hipStream_t st);

@@ -593,7 +593,7 @@ at::Tensor w8a8_int8_linear(const at::Tensor& x, const at::Tensor& x_scale, cons
     const auto b = bias_1d(bias, n);
     const auto off = [k](const at::Tensor& t) {
         const int64_t ld = t.size(0) > 1 ? t.stride(0) : 0;
-        return k % 16 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || ld % 16 || ld >= (1 << 25));
+        return k % 16 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || ld % 16 || ld >= (1 << 24));
     };
     const int param = (off(x2.t) ? QLIN_W8A8_X_ROWS : 0) | (off(w) ? QLIN_W8A8_W_ROWS : 0) |
                       (n > 1 && w.stride(0) != k ? QLIN_W8A8_W_APART : 0);

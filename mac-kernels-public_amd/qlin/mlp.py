@@ -211,7 +211,7 @@ def _scale(scale, n):
 
 
 def _aligned(t):
-    return t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (t.stride(0) % 16 == 0 and t.stride(0) < 1 << 25))
+    return t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (t.stride(0) % 16 == 0 and t.stride(0) < 1 << 24))
 
 
 # ------------------------------------------------------------------------------------------------

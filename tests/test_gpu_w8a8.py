@@ -196,3 +196,18 @@ def test_trainable():
     want = Q.int8_linear(x.detach(), codes, scale, convrot=True, convrot_groupsize=128)
     rel = float((y.detach().double() - want.double()).norm() / want.double().norm())
     assert rel < 2e-2, rel
+
+
+def test_rows_far_apart():
+    """Rows almost 2^24 bytes apart as they are, at 2^24 copied: the bits of packed rows.  (Sizes whose tiles are 256 x 256, K long and short.)"""
+    Q = qlin()
+    for k in (256, 3584):
+        x, sx, w, sw = make(512, k, 32768, seed=k)
+        want = Q.w8a8_int8_linear(x, sx, w, sw)
+        buf = torch.empty(512 << 24, dtype=torch.int8, device=DEV)
+        for ld in ((1 << 24) - 16, 1 << 24):
+            far = buf.as_strided((512, k), (ld, 1))
+            far.copy_(x)
+            assert torch.equal(Q.w8a8_int8_linear(far, sx, w, sw), want)
+            assert torch.equal(Q.w8a8_int8_linear(far[:40], sx[:40], w, sw), want[:40])
+            assert torch.equal(Q.w8a8_int8_linear(far[:1], sx[:1], w[:100], sw[:100]), want[:1, :100])

@@ -30,6 +30,7 @@ BAD_INPUT = [
     (dict(w=z(63)), INVALID),
     (dict(w=z(128)[::2]), DECLINED),
     (dict(w=z(64, dtype=I8)), DECLINED),
+    (dict(w=z(4, 32)[:2]), INVALID),                          # no vector
     (dict(eps=-1.0), INVALID),
     (dict(eps=float("nan")), INVALID),
 ]
@@ -175,6 +176,11 @@ MANY = dict(x=z(300, 256, dtype=I8), sx=z(300, 1, dtype=F32), y=z(300, 20))
     (dict(y=z(1, 20).expand(3, 20)), INVALID),
     (dict(x=z(3, 0, dtype=I8), w=z(20, 0, dtype=I8)), DECLINED),
     (dict(x=z(1, 131072, dtype=I8), w=z(2, 131072, dtype=I8), sx=z(1, dtype=F32), sw=z(2, dtype=F32), y=z(1, 2)), DECLINED),
+    (dict(sx=z(4, 4, dtype=F32)[:2, :2].expand(2, 2)), INVALID),
+    (dict(x=z(4, 256, dtype=I8), y=z(4, 20), sx=z(2, 4, dtype=F32)[:, :2]), INVALID),   # four scales, but no vector
+    (dict(x=z(1, 256, dtype=I8).expand(1 << 28, 256), sx=z(1, 1, dtype=F32)), DECLINED),
+    (dict(x=z(1, 256, dtype=I8).expand(1 << 27, 256), w=z(1, 256, dtype=I8).expand(1 << 10, 256), sx=z(1, 1, dtype=F32)), DECLINED),
+    (dict(w=z(1, 256, dtype=I8).expand(1 << 26, 256), sw=z(1, dtype=F32)), DECLINED),
     (dict(MANY, x=z(300, 250, dtype=I8), w=z(20, 250, dtype=I8)), NO_ROOM),   # rows that are not whole are copied
     (dict(MANY, w=z(20, 257, dtype=I8)[:, :256]), NO_ROOM),
 ])
@@ -220,3 +226,23 @@ def test_workspaces():
     assert size(3000, 4096, 256, L.W8A8_W_ROWS) == a(4096 * 256) and size(3000, 4096, 256, L.W8A8_X_ROWS) == a(3000 * 256)
     assert size(9504, 4096, 4096, L.W8A8_W_APART) == a(4096 * 4096) and size(9504, 4096, 4096) == 0
     assert lb.qlin_workspace_size(L.OP_ADD_RMS_NORM_GRAD, 5, 0, 100, 0, L.DT_F16) >= 400
+
+
+def test_rows_far_apart_are_copied():
+    """Offsets in a tile are 32 bits: strides of 2^24 bytes and more go through the workspace, by both routes' rule and the library's."""
+    from qlin import mlp
+    L, lb = lib()
+    far = lambda ld: torch.empty(0, dtype=I8).as_strided((2, 0), (ld, 1))  # noqa: E731
+    assert mlp._aligned(far((1 << 24) - 16)) and not mlp._aligned(far(1 << 24)) and not mlp._aligned(far(40))
+    assert 255 * ((1 << 24) - 16) + 128 < 1 << 32
+
+
+def test_query():
+    L, lb = lib()
+    ask = lambda op, m, n, k, a, b: lb.qlin_query(op, m, n, k, 0, a, b)  # noqa: E731
+    assert ask(L.OP_W8A8_LINEAR, 8, 4096, 131071, L.DT_I8, L.DT_BF16) == 0
+    for bad in ((8, 4096, 131072, L.DT_I8, L.DT_BF16), (8, 4096, 0, L.DT_I8, L.DT_BF16), (8, 4096, 64, L.DT_F16, L.DT_F16), (8, 1 << 26, 64, L.DT_I8, L.DT_F16),
+                (1 << 28, 8, 64, L.DT_I8, L.DT_F16), (1 << 27, 1 << 10, 64, L.DT_I8, L.DT_F16), (8, 4096, 64, L.DT_I8, L.DT_I8)):
+        assert ask(L.OP_W8A8_LINEAR, *bad) == DECLINED
+    assert ask(L.OP_ADD_RMS_NORM_GRAD, 8, 0, 1 << 20, L.DT_F16, L.DT_F32) == ask(L.OP_ADD_RMS_NORM_GRAD, 8, 0, 1, L.DT_BF16, L.DT_BF16) == 0
+    assert ask(L.OP_ADD_RMS_NORM_GRAD, 8, 0, (1 << 20) + 1, L.DT_F16, L.DT_F16) == ask(L.OP_ADD_RMS_NORM_GRAD, 8, 0, 64, L.DT_F16, L.DT_BF16) == DECLINED
