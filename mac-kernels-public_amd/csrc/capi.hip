@@ -400,7 +400,8 @@ size_t qlin_workspace_size(int op, int64_t M, int64_t N, int64_t K, int param, i
 
 qlin_status qlin_query(int op, int64_t M, int64_t N, int64_t K, int param, int x_dtype, int out_dtype) {
     if (M < 0 || N < 0 || K < 0) return fail(QLIN_EINVAL, "negative shape");
-    if (!is_float(x_dtype) || !is_float(out_dtype)) return fail(QLIN_EUNSUPPORTED, "dtype unsupported");
+    if ((op == QLIN_OP_W8A8_LINEAR ? x_dtype != QLIN_DT_I8 : !is_float(x_dtype)) || !is_float(out_dtype))
+        return fail(QLIN_EUNSUPPORTED, "dtype unsupported");
     switch (op) {
         case QLIN_OP_INT8_LINEAR:
             if (!valid_group(param)) return fail(QLIN_EUNSUPPORTED, "ConvRot group %d unsupported", param);
@@ -429,6 +430,15 @@ qlin_status qlin_query(int op, int64_t M, int64_t N, int64_t K, int param, int x
             if (x_dtype != out_dtype || x_dtype == QLIN_DT_F32) return fail(QLIN_EUNSUPPORTED, "f16 or bf16, in and out");
             if (K < 8 || K > PAGED_MAX_DIM || K % 8) return fail(QLIN_EUNSUPPORTED, "heads of %lld values", (long long)K);
             if (param < 1 || N % param || N > 65535) return fail(QLIN_EUNSUPPORTED, "%lld heads over %d", (long long)N, param);
+            return QLIN_OK;
+        case QLIN_OP_ADD_RMS_NORM_GRAD:  // x_dtype: dy's, out_dtype: that of h and dx
+            if (out_dtype != x_dtype && out_dtype != QLIN_DT_F32) return fail(QLIN_EUNSUPPORTED, "h must have dy's dtype or float32");
+            if (K > MLP_MAX_WIDTH) return fail(QLIN_EUNSUPPORTED, "rows of %lld values, more than %d", (long long)K, MLP_MAX_WIDTH);
+            return QLIN_OK;
+        case QLIN_OP_W8A8_LINEAR:
+            if (K < 1 || K > W8A8_MAX_K) return fail(QLIN_EUNSUPPORTED, "rows of %lld values", (long long)K);
+            if (M >= W8A8_MOST_ROWS || N >= W8A8_MOST_OUTPUTS || (N && M > W8A8_MOST_RESULTS / N))
+                return fail(QLIN_EUNSUPPORTED, "%lld rows by %lld outputs are too many", (long long)M, (long long)N);
             return QLIN_OK;
     }
     return fail(QLIN_EUNSUPPORTED, "unknown op %d", op);
