@@ -4,8 +4,10 @@
 // A row stays in registers between its reads and its writes, 8 or 16 values a thread, a row (or a few short ones) a workgroup.  8
 // bits: the codes are rne(127 v / top) with v = w h (rotated, for weights that are stored so) and top the row's largest |v|;
 // rho cancels in them, so that one exchange between a row's threads gives both the sum of squares and top, and the scale is
-// top rho / 127.  (Workgroups that take rows in turn, the next one's reads in flight: 4608 x 6144 to bf16 50 us against 49 and, with
-// nontemporal writes, 40; the gradient is so because its workgroups keep partial sums.)
+// top rho / 127.  (Workgroups that take rows in turn, the next one's reads in flight, are no faster: 4608 x 6144 to bf16 50 us
+// against 49 before either wrote nontemporally; the gradient is so because its workgroups keep partial sums.)
+//
+// 4608 x 6144 to bf16 41 us (36 at 6.3 TB/s), to int8 36 (31), rotated by 128 41; gradient of 9504 x 5120 75 (62).
 #include "mlp_rows.h"
 
 namespace qlin {
@@ -239,9 +241,10 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs 
     }
 }
 
-// Rows of any length: the row's sums, then its gradient.
+// Rows of any length: the row's sums, then its gradient.  The partial sums stay in memory, a run the same thread's in every row.
 template <typename T, typename H>
 __global__ __launch_bounds__(512) void add_norm_grad_long_kernel(AddNormGradArgs a) {
+    constexpr int RUN = 8;
     const Group g(512);
     float* part = a.dw ? a.part + (int64_t)blockIdx.x * a.W : nullptr;
     int turn = 0;
@@ -251,19 +254,39 @@ __global__ __launch_bounds__(512) void add_norm_grad_long_kernel(AddNormGradArgs
         const H* h = (const H*)a.h.p + t * a.h.ld;
         const H* dh = a.dh.p ? (const H*)a.dh.p + t * a.dh.ld : nullptr;
         H* dx = (H*)a.dx.p + t * a.dx.ld;
+        float v[RUN], d[RUN], w[RUN];
+        auto load = [&](int e) {
+            load_run<H, RUN>(h + e, a.W - e, v);
+            load_run<T, RUN>(dy + e, a.W - e, d);
+            if (a.w) load_run_rt<RUN>(a.w, a.w_dt, e, a.W - e, w);
+            else
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) w[i] = 1.0f;
+        };
         float ss = 0.0f, gh = 0.0f;
-        for (int e = threadIdx.x; e < a.W; e += 512) {
-            const float v = (float)h[e], d = (float)dy[e] * (a.w ? load_rt(a.w, a.w_dt, e) : 1.0f);
-            ss = __builtin_fmaf(v, v, ss);
-            gh = __builtin_fmaf(d, v, gh);
+        for (int e = threadIdx.x * RUN; e < a.W; e += 512 * RUN) {
+            load(e);
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) {
+                ss = __builtin_fmaf(v[i], v[i], ss);
+                gh = __builtin_fmaf(d[i] * w[i], v[i], gh);
+            }
         }
         g.sums(ss, gh, turn, [](float p, float q) { return p + q; });
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
         const float c = rho * rho * (gh / (float)a.W);
-        for (int e = threadIdx.x; e < a.W; e += 512) {  // an element is the same thread's in every row
-            const float v = (float)h[e], d = (float)dy[e], w = a.w ? load_rt(a.w, a.w_dt, e) : 1.0f;
-            if (part) part[e] = __builtin_fmaf(d, v * rho, begun ? part[e] : 0.0f);
-            dx[e] = (H)__builtin_fmaf(rho, __builtin_fmaf(d, w, -(v * c)), dh ? (float)dh[e] : 0.0f);
+        for (int e = threadIdx.x * RUN; e < a.W; e += 512 * RUN) {
+            float sum[RUN] = {}, more[RUN] = {}, o[RUN];
+            if (part && begun) load_run<float, RUN>(part + e, a.W - e, sum);
+            if (dh) load_run<H, RUN>(dh + e, a.W - e, more);
+            load(e);
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) {
+                sum[i] = __builtin_fmaf(d[i], v[i] * rho, sum[i]);
+                o[i] = __builtin_fmaf(rho, __builtin_fmaf(d[i], w[i], -(v[i] * c)), more[i]);
+            }
+            if (part) store_run<false, float, RUN>(part + e, a.W - e, sum);
+            store_run<false, H, RUN>(dx + e, a.W - e, o);
         }
         begun = true;
     }

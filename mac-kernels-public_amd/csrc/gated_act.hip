@@ -4,6 +4,9 @@
 //
 // 8 bits: a row stays in registers until its largest |value| is known; the codes are rne(127 v / top), v rotated first for
 // weights that are stored so, the scale is top / 127.
+//
+// 9504 x 13824 with up: to bf16 127 us (125 at 6.3 TB/s), to int8 105 (104), rotated by 256 140 (the rotation's vector instructions,
+// and in fp16 the activation's conversions, 154); its gradient 217 (209).
 #include "mlp_rows.h"
 
 namespace qlin {

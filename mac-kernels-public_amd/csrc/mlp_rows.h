@@ -13,7 +13,8 @@ struct Run {
 };
 // Values e0 .. e0 + N - 1 of a row of W >= N, at any alignment (global loads take any), without a branch, so that a thread's loads
 // are in flight together: a run that reaches past the row's end gets its last N values, which trimmed() puts right once
-// all loads have been issued.  ONCE: nontemporal, whole 16-byte (8-byte: RUN 4 of 16 bits) pieces.
+// all loads have been issued.  ONCE: nontemporal, whole 16-byte (8-byte: RUN 4 of 16 bits) pieces: what is read and written once
+// takes no place in the caches (norm 4608 x 6144 to bf16, one row a workgroup: 49 us, 40 with both).
 template <bool ONCE, typename T, int N>
 __device__ __forceinline__ Run<T, N> load_piece(const T* row, int e0, int W) {
     const T* p = row + min(e0, W - N);
@@ -282,7 +283,8 @@ struct RowCut {
 };
 // 8-value runs: a slot more from 512 threads on (norm 4608 x 6144 to int8, 384 threads of two slots 35.5 us, 768 of one 38.2), up to
 // `most` slots and, with these, 1024 threads; fewer slots hold up to `threads`.  4-value runs: four slots, and eight where
-// `most` says so and a row has more than 20 times 256 values (activation 9504 x 13824: four 147 us, eight 120; 9504 x 5120: 47.6, 49.1).
+// `most` says so and a row has more than 20 times 256 values (activation 9504 x 13824 in bf16: four 144 us, eight 140; 9504 x 5120: both 56),
+// which also holds rows of up to 32768 values.
 // waves: that a CU is to hold, where workgroups take rows in turn.
 inline RowCut cut_rows(int64_t T, int W, int run, int most, int threads, int waves) {
     RowCut c;
@@ -297,6 +299,7 @@ inline RowCut cut_rows(int64_t T, int W, int run, int most, int threads, int wav
         break;
     }
     c.groups = c.slots && c.per < 256 ? 256 / c.per : 1;
+    if (!c.slots && !waves) waves = 32;  // rows longer than any slots hold, read twice (4096 x 20480 to int8: one workgroup a CU 261 us, four 158)
     const int64_t blocks = (T + c.groups - 1) / c.groups, held = 256 * (int64_t)std::max(1, waves * 64 / (c.per * c.groups));
     const int64_t rounds = (blocks + held - 1) / held;
     c.grid = (unsigned)((blocks + rounds - 1) / rounds);

@@ -233,3 +233,9 @@ def test_captured_and_on_other_streams():
     x.copy_(make(300, 1032, F16, F16, seed=4)[0])
     for a, b in zip(eager, step()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,h_dtype", KINDS)
+def test_gradient_of_many_long_rows(dtype, h_dtype):
+    """Rows longer than a workgroup holds, more than there are workgroups: partial sums over rows in turn."""
+    test_gradient(600, 16401, dtype, h_dtype)
