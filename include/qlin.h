@@ -393,7 +393,8 @@ qlin_status qlin_paged_attention(const qlin_tensor* q, const qlin_tensor* k_cach
  * (the same memory and strides); it may not overlap one otherwise.
  *
  * 8-bit outputs: with v the row's values (rotated by the ConvRot group first, convrot_groupsize 0: not) and top their largest
- * magnitude, scale = top / 127 and q = rne(127 v / top), ties to even; a row of zeros has scale 0 and codes 0.  A row
+ * magnitude, scale = top / 127 and q = rne(127 v / top), ties to even; a row of zeros has scale 0 and codes 0
+ * (in the norm with eps 0 its scale is 0 / 0, NaN).  A row
  * with an infinity or a NaN has a scale that is not finite, which makes every output of a linear over it NaN or infinite.
  * ---------------------------------------------------------------------------------------------- */
 
