@@ -44,6 +44,12 @@ def _rows(op, t, name, shape=None):
     return t if t.size(1) <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
+def _dtype(op, t, name, *known):
+    """Declines t before its dtype is looked up for a workspace's size."""
+    if t.dtype not in known:
+        raise NoCapableBackendError(op, {"hip": f"{name} dtype {t.dtype} unsupported"})
+
+
 def _codes(shape, device):
     q = torch.empty(shape, dtype=torch.int8, device=device)
     return q, torch.empty((*shape[:-1], 1), dtype=torch.float32, device=device)
@@ -102,6 +108,7 @@ def add_rms_norm_grad(dy, dh, h, weight=None, *, eps=1e-6, weight_grad=True):
         except ops._FastError as e:
             raise _fast_error(op, e) from None
     _check_device(op, dy, dh, h, weight)
+    _dtype(op, dy, "dy", *ops._FLOAT)
     g2, d2, h2 = _rows(op, dy, "dy"), _rows(op, dh, "dh", dy.shape), _rows(op, h, "h", dy.shape)
     dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     w = _vector(weight)
@@ -178,6 +185,8 @@ def w8a8_int8_linear(x, x_scale, qdata, scale, bias=None, out_dtype=None, *, res
         except ops._FastError as e:
             raise _fast_error(op, e) from None
     _check_device(op, x, x_scale, qdata, scale, bias, residual, residual_scale)
+    _dtype(op, x, "x", torch.int8)
+    _dtype(op, qdata, "qdata", torch.int8)
     x2 = _rows(op, x, "x")
     if qdata.dim() != 2:
         raise NoCapableBackendError(op, {"hip": "qdata must be a 2-D int8 tensor"})

@@ -1,0 +1,33 @@
+"""The MLP side's ctypes route without a GPU: what it refuses before the library is asked for a workspace."""
+import pytest
+import torch
+
+F16, F32, F64, I8 = torch.float16, torch.float32, torch.float64, torch.int8
+
+
+@pytest.fixture
+def route(monkeypatch):
+    """The ctypes route with tensors of the CPU let through to its checks."""
+    import qlin
+    from qlin import mlp, ops
+    monkeypatch.setattr(ops, "_FAST", None)
+    monkeypatch.setattr(mlp, "_check_device", lambda *a: None)
+    return qlin
+
+
+def z(*shape, dtype=F16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [F64, torch.int16, torch.complex64, torch.bool])
+def test_dtypes_that_the_library_does_not_know_are_declined(route, dtype):
+    """Also where the dtype would be looked up for the workspace's size first."""
+    x, w, odd = z(3, 64), z(64), z(3, 64, dtype=dtype)
+    calls = [lambda: route.add_rms_norm(odd, None, w), lambda: route.add_rms_norm_int8(odd, None, w), lambda: route.add_rms_norm_grad(odd, None, x, w),
+             lambda: route.add_rms_norm_grad(odd, None, odd, w), lambda: route.gated_act(odd), lambda: route.gated_act_int8(odd),
+             lambda: route.gated_act_grad(odd, odd),
+             lambda: route.w8a8_int8_linear(odd, z(3, 1, dtype=F32), z(20, 64, dtype=I8), z(20, dtype=F32)),
+             lambda: route.w8a8_int8_linear(z(3, 64, dtype=I8), z(3, 1, dtype=F32), z(20, 64, dtype=dtype), z(20, dtype=F32))]
+    for call in calls:
+        with pytest.raises(route.NoCapableBackendError):
+            call()
