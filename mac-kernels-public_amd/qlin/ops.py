@@ -14,6 +14,7 @@ approximation.
 """
 from __future__ import annotations
 
+import math
 import os
 
 import torch
@@ -107,7 +108,7 @@ def _residual_args(op, residual, residual_scale, shape, n):
     for t in (residual, residual_scale):
         if t is not None and t.dtype not in _FLOAT:
             raise NoCapableBackendError(op, {"hip": f"residual dtype {t.dtype} unsupported"})
-    r = residual.reshape(-1, n)
+    r = residual.reshape(math.prod(shape[:-1]), n)  # -1 has no meaning without outputs
     if r.shape[0] > 1 and (r.stride(1) != 1 or r.stride(0) < n):
         r = r.contiguous()
     rs = None

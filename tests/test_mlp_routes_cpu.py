@@ -31,3 +31,13 @@ def test_dtypes_that_the_library_does_not_know_are_declined(route, dtype):
     for call in calls:
         with pytest.raises(route.NoCapableBackendError):
             call()
+
+
+def test_a_residual_of_no_outputs():
+    """Rows of a linear without outputs have a residual without values."""
+    from qlin import ops
+    for shape in ((3, 0), (2, 3, 0), (0, 0)):
+        r, rs = ops._residual_args("linear", z(*shape), z(0), shape, 0)
+        assert r.shape == (shape[0] if len(shape) == 2 else 6, 0) and rs.shape == (0,)
+    r, _ = ops._residual_args("linear", z(2, 0, 5), None, (2, 0, 5), 5)
+    assert r.shape == (0, 5)
