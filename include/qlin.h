@@ -395,7 +395,8 @@ qlin_status qlin_paged_attention(const qlin_tensor* q, const qlin_tensor* k_cach
  * 8-bit outputs: with v the row's values (rotated by the ConvRot group first, convrot_groupsize 0: not) and top their largest
  * magnitude, scale = top / 127 and q = rne(127 v / top), ties to even; a row of zeros has scale 0 and codes 0
  * (in the norm with eps 0 its scale is 0 / 0, NaN).  A row
- * with an infinity or a NaN has a scale that is not finite, which makes every output of a linear over it NaN or infinite.
+ * with an infinity or a NaN has a scale that is not finite, which makes every output of a linear over it NaN or infinite; so may a
+ * row whose rotated values pass 2^126 (in the norm: weight times h).  Rotated values below 2^-110 lose bits.
  * ---------------------------------------------------------------------------------------------- */
 
 /* h = x + residual, y = weight * h / rms(h), rms(h) = sqrt(mean(h^2) + eps) over the row.  The norm is that of the unrounded

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void add_norm_kerne
         const float most = top;
         float first;
         const float inv = code_factor(most, first);
-        if (g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.norm : 1.0f) / 127.0f * rho;
+        if (g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.left : 1.0f) / 127.0f * rho;
         if (first != 1.0f)
 #pragma unroll
             for (int s = 0; s < SLOTS; ++s)
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps), most = top;
         float first = 1.0f;
         const float inv = INT8 ? code_factor(most, first) : 0.0f;
-        if (INT8 && g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.norm : 1.0f) / 127.0f * rho;
+        if (INT8 && g.at == 0) a.scale[t] = most * (RUN == 4 ? turned.left : 1.0f) / 127.0f * rho;
         for (int c = 0; c < a.W; c += 512 * RUN) {
             const int e0 = c + g.place<RUN>();
             sum_of(e0);

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void gated_act_int8
     if (!live) return;
     float first;
     const float inv = code_factor(top, first);
-    if (g.at == 0) a.scale[t] = top * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
+    if (g.at == 0) a.scale[t] = top * (RUN == 4 ? turned.left : 1.0f) / 127.0f;
     if (first != 1.0f)
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s)
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(512) void gated_act_int8_long_kernel(GatedActArgs a
         g.sums(none, top, turn, larger);
         float first;
         const float inv = code_factor(top, first);
-        if (g.at == 0) a.scale[t] = top * (RUN == 4 ? turned.norm : 1.0f) / 127.0f;
+        if (g.at == 0) a.scale[t] = top * (RUN == 4 ? turned.left : 1.0f) / 127.0f;
         for (int c = 0; c < a.W; c += 512 * RUN) {
             const int e0 = c + g.place<RUN>();
             value(e0);

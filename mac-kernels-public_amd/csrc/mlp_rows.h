@@ -163,16 +163,22 @@ __device__ __forceinline__ float code_factor(float top, float& first) {
 
 // The rotation of 256 values on the matrix cores.  As a 16 x 16 matrix V[a][b] of values 16 a + b they become M_a V M_b with M_b the
 // Hadamard matrix of the group's lowest (at most) two base-4 digits and M_a that of the higher ones, block diagonal where the
-// group is smaller than 256 values: entries 0, 1 and -1, exact in bf16.  Lane l holds values 16 (l % 16) + 4 (l / 16) .. + 3,
+// group is smaller than 256 values: entries 0, 1 and -1 (M_b's times a power of two), exact in bf16.  Lane l holds values 16 (l % 16) + 4 (l / 16) .. + 3,
 // which are its part of V as the first operand; the product's registers, taken as a first operand again, are its transpose, and the
-// second product comes out in the layout of the values.  Unnormalized: by sqrt(G).
+// second product comes out in the layout of the values.
+//
+// The factor 1 / sqrt(G) is in the first product's entries, as the power of two at or below it; what is left, 1 or sqrt(2), is the
+// scale's.  So no sum passes fp32's range where the rotated values stay below 2^126: among the values that take part in a first sum
+// one is at least as large, and the partial sums of 16 terms are at most 4 times the largest of the 16 sums.  (The factor behind the
+// sums gave finite rows infinite scales from 2^124 on.)
 //
 // A value enters a product as three bf16 parts that together are the value (8 bits of its 24 each), so that the rotation is as exact as
 // fp32's sums.  Two rounded parts, off by 2^-18, would change one code in 10^4 (9504 x 13824 in fp16, with the gate: two
 // parts 140 us, three 154; the matrix cores' fp32 products, of a 16th of the rate, 207; fp32 across the lanes 157).
 typedef short bf16x4_bits __attribute__((ext_vector_type(4)));
 struct RotationTable {
-    uint64_t m[5][64];  // sizes 1, 2, 4, 8, 16: lane l's entries [4 (l / 16) + i][l % 16]
+    // lane l's entries [4 (l / 16) + i][l % 16]: M_b by log2 G, its entries 2^-ceil(log2 G / 2), and M_a by log2 of its size
+    uint64_t low[9][64], high[5][64];
     static constexpr int entry(int size, int r, int c) {
         if (r / size != c / size) return 0;
         r %= size;
@@ -181,25 +187,31 @@ struct RotationTable {
         for (; size >= 4; size /= 4, r /= 4, c /= 4) s = r % 4 + c % 4 == 3 ? -s : s;
         return size == 2 && r && c ? -s : s;
     }
-    constexpr RotationTable() : m() {
-        for (int k = 0; k < 5; ++k)
-            for (int l = 0; l < 64; ++l)
-                for (int i = 0; i < 4; ++i) {
-                    const int e = entry(1 << k, 4 * (l / 16) + i, l % 16);
-                    m[k][l] |= (uint64_t)(e == 0 ? 0 : e == 1 ? 0x3F80 : 0xBF80) << (16 * i);
-                }
+    static constexpr uint64_t lane(int size, int halvings, int l) {
+        uint64_t m = 0;
+        for (int i = 0; i < 4; ++i) {
+            const int e = entry(size, 4 * (l / 16) + i, l % 16), one = 0x3F80 - 0x80 * halvings;
+            m |= (uint64_t)(e == 0 ? 0 : e == 1 ? one : one | 0x8000) << (16 * i);
+        }
+        return m;
+    }
+    constexpr RotationTable() : low(), high() {
+        for (int l = 0; l < 64; ++l) {
+            for (int k = 0; k < 9; ++k) low[k][l] = lane(1 << (k < 4 ? k : 4), (k + 1) / 2, l);
+            for (int k = 0; k < 5; ++k) high[k][l] = lane(1 << k, 0, l);
+        }
     }
 };
 __device__ const RotationTable rotation_table;
 
 struct Rotation {
     bf16x4_bits low, high;  // M_b, M_a
-    float norm;
+    float left;             // what the rotated values lack
     __device__ __forceinline__ Rotation(int G, int lane) {
         const int k = 31 - __clz(G);
-        low = __builtin_bit_cast(bf16x4_bits, rotation_table.m[min(k, 4)][lane]);
-        high = __builtin_bit_cast(bf16x4_bits, rotation_table.m[max(k - 4, 0)][lane]);
-        norm = k % 2 ? 0.70710678118654752f / (float)(1 << (k / 2)) : 1.0f / (float)(1 << (k / 2));
+        low = __builtin_bit_cast(bf16x4_bits, rotation_table.low[k][lane]);
+        high = __builtin_bit_cast(bf16x4_bits, rotation_table.high[max(k - 4, 0)][lane]);
+        left = k % 2 ? 1.41421356237309505f : 1.0f;
     }
     static __device__ __forceinline__ f32x4 product(const f32x4 v, const bf16x4_bits m) {
         // the parts of two values side by side, as the product takes them: the upper halves of their words, those of what is left
