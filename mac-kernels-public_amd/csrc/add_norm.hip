@@ -83,6 +83,20 @@ __global__ __launch_bounds__(1024, SLOTS * RUN > 16 ? 4 : 6) void add_norm_kerne
     }
 }
 
+// A thread's sum of a row of any length: of runs, sixteen of them at a time, so that 2^20 values meet 52 roundings in turn (4 + 16 + 32), where
+// one after the other they would 2048 (equal values: y off by 2^-16).
+struct LongSum {
+    float all = 0.0f, part = 0.0f;
+    int runs = 0;
+    __device__ __forceinline__ void add(float run) {
+        part += run;
+        if (++runs & 15) return;
+        all += part;
+        part = 0.0f;
+    }
+    __device__ __forceinline__ float sum() const { return all + part; }
+};
+
 // Rows of any length, read twice.
 template <typename T, typename H, int RUN, bool INT8>
 __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
@@ -111,18 +125,21 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
             }
             if constexpr (RUN == 4) turned(v);
         };
-        float ss = 0.0f;
+        LongSum squares;
         float top = 0.0f;
         for (int c = 0; c < a.W; c += 512 * RUN) {
             const int e0 = c + g.place<RUN>();
             sum_of(e0);
+            float sq = 0.0f;
 #pragma unroll
-            for (int i = 0; i < RUN; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+            for (int i = 0; i < RUN; ++i) sq = __builtin_fmaf(v[i], v[i], sq);
+            squares.add(sq);
             if constexpr (INT8) {
                 weigh(e0);
                 top = larger(top, largest<RUN>(v));
             }
         }
+        float ss = squares.sum();
         g.sums(ss, top, turn, larger);
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps), most = top;
         float first = 1.0f;
@@ -263,15 +280,19 @@ __global__ __launch_bounds__(512) void add_norm_grad_long_kernel(AddNormGradArgs
 #pragma unroll
                 for (int i = 0; i < RUN; ++i) w[i] = 1.0f;
         };
-        float ss = 0.0f, gh = 0.0f;
+        LongSum squares, products;
         for (int e = threadIdx.x * RUN; e < a.W; e += 512 * RUN) {
             load(e);
+            float sq = 0.0f, pr = 0.0f;
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                ss = __builtin_fmaf(v[i], v[i], ss);
-                gh = __builtin_fmaf(d[i] * w[i], v[i], gh);
+                sq = __builtin_fmaf(v[i], v[i], sq);
+                pr = __builtin_fmaf(d[i] * w[i], v[i], pr);
             }
+            squares.add(sq);
+            products.add(pr);
         }
+        float ss = squares.sum(), gh = products.sum();
         g.sums(ss, gh, turn, [](float p, float q) { return p + q; });
         const float rho = 1.0f / sqrtf(ss / (float)a.W + a.eps);
         const float c = rho * rho * (gh / (float)a.W);
