@@ -46,7 +46,7 @@ struct AddNormGradArgs {
     float eps = 0.0f;
     void* dw = nullptr;                // [W] or nullptr (not formed)
     int dw_dt = DT_F32;
-    float* part = nullptr;             // add_norm_grad_parts() x [W] partial sums
+    float* part = nullptr;             // ws_add_norm_grad() bytes: a row of W partial sums a workgroup
 };
 hipError_t run_add_norm_grad(const AddNormGradArgs& a, hipStream_t st);
 size_t ws_add_norm_grad(int64_t T, int64_t W);
@@ -88,7 +88,8 @@ struct W8A8Args {
 };
 // What keeps a call's operands from being taken as they are (bits of `param`).
 enum { W8A8_X_ROWS = QLIN_W8A8_X_ROWS, W8A8_W_ROWS = QLIN_W8A8_W_ROWS, W8A8_W_APART = QLIN_W8A8_W_APART };
-// Rows and outputs of a call below these, and at most 2^36 results: a launch has fewer than 2^32 threads whatever the tiles.
+// Rows and outputs of a call below these, and at most 2^36 results: 256 x 256 tiles are then fewer than 2^22, and shapes whose launch would have
+// 2^32 threads or more are not chosen (cost() in w8a8.hip).
 constexpr int64_t W8A8_MOST_ROWS = 1 << 28, W8A8_MOST_OUTPUTS = 1 << 26, W8A8_MOST_RESULTS = (int64_t)1 << 36;
 constexpr int64_t W8A8_MOST_APART = 1 << 24;  // row strides below it: the kernels' offsets in a tile, of up to 256 rows, are 32 bits
 int w8a8_apart(const W8A8Args& a);

@@ -344,8 +344,12 @@ constexpr Shape TILE_SHAPES[] = {{16, 16, 0.06f}, {16, 32, 0.09f}, {16, 64, 0.17
 constexpr Shape GEMM_SHAPES[] = {{128, 64, 0.43f}, {128, 128, 0.6f}, {256, 128, 0.95f}, {128, 256, 1.0f}, {256, 256, 1.22f}};
 constexpr int GEMM_TILES[] = {I8_128x64, I8_128x128, I8_256x128, I8_128x256, I8_256x256};
 
+// Tiles of up to 512 threads in a launch of fewer than 2^32.
+constexpr int64_t MOST_TILES = 1 << 23;
+
 float cost(const Shape& s, int64_t M, int64_t N, int64_t K) {
     const int64_t tiles = ((M + s.m - 1) / s.m) * ((N + s.n - 1) / s.n);
+    if (tiles >= MOST_TILES) return 1e20f;
     return 5.0f + s.us * (float)((K + 127) / 128) * (float)((tiles + 255) / 256);
 }
 
