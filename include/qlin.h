@@ -412,7 +412,9 @@ qlin_status qlin_add_rms_norm_int8(const qlin_tensor* x, const qlin_tensor* resi
 /* Gradients of qlin_add_rms_norm from those of y and h (dh NULL: none reaches h): with rho = 1 / rms(h) and g = weight dy,
  *   dx = rho (g - h rho^2 mean(g h)) + dh,  which is x's and the residual's gradient both, in h's dtype,
  *   dweight = sum over rows of dy h rho     (NULL: not formed; f32/f16/bf16 [values], summed in fp32 in a fixed order).
- * h is the forward call's (x itself where it had no residual); dy in x's dtype; dh, dx in h's.
+ * h is the forward call's (x itself where it had no residual); dy in x's dtype; dh, dx in h's.  The forward norm is that of the
+ * unrounded sum, these are taken at h as it was stored: with e half a step of its dtype, dweight is off by up to 2 e of its
+ * terms' magnitudes and dx by up to 5 e; an f32 residual leaves both to fp32's own roundings.
  * Workspace (only with dweight): qlin_workspace_size(QLIN_OP_ADD_RMS_NORM_GRAD, rows, 0, values, 0, dy's dtype). */
 qlin_status qlin_add_rms_norm_grad(const qlin_tensor* dy, const qlin_tensor* dh, const qlin_tensor* h, const qlin_tensor* weight,
                                    float eps, qlin_tensor* dx, qlin_tensor* dweight, void* workspace, size_t workspace_bytes,

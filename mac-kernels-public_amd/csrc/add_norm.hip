@@ -159,7 +159,9 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(AddNormArgs a) {
     }
 }
 
-// dx = rho (g - h rho^2 mean(g h)) + dh with g = w dy, and a workgroup's part of dw = sum_t dy h rho.
+// dx = rho (g - h rho^2 mean(g h)) + dh with g = w dy, and a workgroup's part of dw = sum_t dy h rho.  h is taken as it was stored: x and the
+// residual in its place would be 10 bytes a value where 8 are, and one tensor more to keep.  With h in bf16 that is 1.8e-3 of dw (1056
+// rows of 6144 normal values, root mean square: 2.4e-3 with dw's rounding to bf16, which alone is 1.65e-3) and 2e-5 of dx.
 template <typename T, typename H, int SLOTS, bool DH, bool ONCE, int THREADS>
 __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(AddNormGradArgs a, int per, int groups) {
     constexpr int RUN = 8;
