@@ -193,7 +193,7 @@ qlin_status qlin_add_rms_norm_grad(const qlin_tensor* dy, const qlin_tensor* dh,
     a.dw = const_cast<void*>(p);
     if (a.dw && a.T) {
         const size_t need = ws_add_norm_grad(a.T, W);
-        if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
+        if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
             return fail(QLIN_EWORKSPACE, "workspace of %zu bytes, needs %zu (16-byte aligned)", workspace_bytes, need);
         a.part = (float*)workspace;
     }

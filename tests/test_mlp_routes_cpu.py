@@ -1,4 +1,6 @@
 """The MLP side's ctypes route without a GPU: what it refuses before the library is asked for a workspace."""
+import ctypes
+
 import pytest
 import torch
 
@@ -41,3 +43,21 @@ def test_a_residual_of_no_outputs():
         assert r.shape == (shape[0] if len(shape) == 2 else 6, 0) and rs.shape == (0,)
     r, _ = ops._residual_args("linear", z(2, 0, 5), None, (2, 0, 5), 5)
     assert r.shape == (0, 5)
+
+
+def test_a_gradient_of_no_values_needs_no_workspace():
+    """qlin_workspace_size is 0 for it: a null workspace is taken, with pointers that are there."""
+    from qlin import _lib
+    L = _lib.load()
+    room = torch.zeros(8)
+
+    def of(*shape):
+        t = _lib.QlinTensor(data=room.data_ptr(), dtype=_lib.DT_F16, ndim=len(shape))
+        for i, n in enumerate(shape):
+            t.shape[i], t.stride[i] = n, 1
+        return t
+
+    rows, weight = of(3, 0), of(0)
+    assert L.qlin_workspace_size(_lib.OP_ADD_RMS_NORM_GRAD, 3, 0, 0, 0, _lib.DT_F16) == 0
+    a = ctypes.addressof
+    assert L.qlin_add_rms_norm_grad(a(rows), None, a(rows), a(weight), 1e-6, a(rows), a(weight), None, 0, None) == 0
