@@ -400,8 +400,8 @@ qlin_status qlin_paged_attention(const qlin_tensor* q, const qlin_tensor* k_cach
  * ---------------------------------------------------------------------------------------------- */
 
 /* h = x + residual, y = weight * h / rms(h), rms(h) = sqrt(mean(h^2) + eps) over the row.  The norm is that of the unrounded
- * sum.  A row whose squares' sum passes fp32's range comes out as zeros.  x, y f32/f16/bf16 of one dtype; residual, h of x's dtype or f32 (both NULL: h is x); weight optional
- * (NULL = 1) f32/f16/bf16 [values].  Rows of up to 2^20 values. */
+ * sum.  A row whose squares' sum passes fp32's range comes out as zeros.  x, y f32/f16/bf16 of one dtype; residual, h of x's
+ * dtype or f32 (both NULL: h is x); weight optional (NULL = 1) f32/f16/bf16 [values].  Rows of up to 2^20 values. */
 qlin_status qlin_add_rms_norm(const qlin_tensor* x, const qlin_tensor* residual, const qlin_tensor* weight, float eps,
                               qlin_tensor* y, qlin_tensor* h, void* stream);
 
